@@ -30,6 +30,7 @@ vp = ctypes.c_void_p
 ACT = dict(ELU=3, ISRLU=10, LINEAR=11, LEAKY_RELU=14, RELU=16, SELU=17, SOFTMAX=22)
 NORM = dict(NONE=0, BN=1, BRN=2)
 DROP = dict(NONE=0, BERNOULLI=2, BERNOULLI_INVERTED=3)
+DTYPE = dict(F32=0, BF16=1)
 DROP_BWD = dict(REFERENCE=0, MASKED=1)
 STATE = dict(INFERENCE=0, TRAINING=1, UPDATE_BATCH_NORM=2)
 
@@ -46,6 +47,7 @@ C_ABI_SYMBOLS = [
     "dlmi_fc_softmax_fwd", "dlmi_fc_softmax_ce_fwd", "dlmi_fc_bwd_dx_norm_act_bwd",
     "dlmi_ctx_reserve_layer", "dlmi_ctx_scratch_generation", "dlmi_ctx_norm_panel_enabled", "dlmi_ctx_norm_panel_poke",
     "dlmi_fc_bwd_dw_grouped", "dlmi_fused_norm_act_bwd_db", "dlmi_ctx_gemm_clock", "dlmi_ctx_gemm_timeline", "dlmi_probe_strip_stream",
+    "dlmi_orthogonalize", "dlmi_opt_muon",
 ]
 
 
@@ -54,6 +56,17 @@ class FusedDesc(ctypes.Structure):
     _fields_ = [("norm", c_int), ("act", c_int), ("dropout", c_int), ("mask_per_element", c_int),
                 ("dropout_bwd", c_int), ("momentum", c_f), ("eps", c_f), ("r_max", c_f), ("d_max", c_f),
                 ("drop_scale", c_f)]
+
+
+class MuonProblem(ctypes.Structure):
+    """dlmi_muon_problem of include/dlmi.h."""
+    _fields_ = [("rows", ctypes.c_size_t), ("cols", ctypes.c_size_t), ("params", ctypes.c_void_p), ("grads", ctypes.c_void_p),
+                ("momentum", ctypes.c_void_p), ("lr", c_f)]
+
+
+class NewtonSchulz(ctypes.Structure):
+    """dlmi_newton_schulz of include/dlmi.h."""
+    _fields_ = [("a", c_f), ("b", c_f), ("c", c_f), ("steps", c_int), ("eps", c_f)]
 
 
 class DwProblem(ctypes.Structure):
@@ -102,6 +115,7 @@ class Dlmi:
         if rc != 0:
             raise DlmiError("dlmi_ctx_create failed with %d" % rc)
         self.ctx = ctx
+        self._stream = stream
 
     def close(self):
         if getattr(self, "ctx", None):
@@ -125,6 +139,29 @@ class Dlmi:
                 continue
             assert t.is_cuda and t.is_contiguous(), "dlmi takes contiguous device tensors"
 
+    def _chk_is(self, t, what, dtype, *shape):
+        """One tensor of the calls that take more than fp32: its type, shape, device and layout."""
+        if t is None:
+            return
+        assert t.dtype == dtype, "%s must be %s, is %s" % (what, dtype, t.dtype)
+        assert tuple(t.shape) == shape, "%s must be %s, is %s" % (what, shape, tuple(t.shape))
+        assert t.device == self.device, "%s must be on %s, is on %s" % (what, self.device, t.device)
+        assert t.is_contiguous(), "dlmi takes contiguous device tensors: " + what
+
+    def _type(self, t):
+        """dlmi_dtype of a tensor of `type`."""
+        types = {self.torch.float32: DTYPE["F32"], self.torch.bfloat16: DTYPE["BF16"]}
+        assert t.dtype in types, "float32 or bfloat16 tensors, not %s" % t.dtype
+        return c_int(types[t.dtype])
+
+    def _out(self, dtype, *shape):
+        """An output that belongs to the context's stream, whichever stream is current."""
+        torch = self.torch
+        if torch.cuda.current_stream(self.device).cuda_stream == self._stream:
+            return torch.empty(shape, dtype=dtype, device=self.device)
+        with torch.cuda.stream(torch.cuda.ExternalStream(self._stream, device=self.device)):
+            return torch.empty(shape, dtype=dtype, device=self.device)
+
     def empty(self, *shape, dtype=None):
         return self.torch.empty(*shape, dtype=dtype or self.torch.float32, device=self.device)
 
@@ -133,6 +170,7 @@ class Dlmi:
 
     def set_stream(self, stream):
         self._ck(self.lib.dlmi_ctx_set_stream(self.ctx, vp(stream.cuda_stream)))
+        self._stream = stream.cuda_stream
 
     def synchronize(self):
         self._ck(self.lib.dlmi_ctx_synchronize(self.ctx))
@@ -336,6 +374,35 @@ class Dlmi:
         self._chk(p, g, m1, m2, vhat, mask)
         self._ck(self.lib.dlmi_opt_adam(self.ctx, c_sz(p.numel()), _p(p), _p(g), _p(m1), _p(m2), _p(vhat), _p(mask),
                                         c_f(lr_t), c_f(beta1), c_f(beta2), c_f(eps), c_f(wd)))
+
+    def orthogonalize(self, G, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7, out=None):
+        """The Newton-Schulz iteration on a [rows, cols] float32 or bfloat16 matrix (dlmi_orthogonalize)."""
+        assert G.dim() == 2
+        rows, cols = G.shape
+        self._chk_is(G, "G", G.dtype, rows, cols)
+        kind = self._type(G)
+        o = out if out is not None else self._out(G.dtype, rows, cols)
+        self._chk_is(o, "out", G.dtype, rows, cols)
+        ns = NewtonSchulz(*[float(c) for c in coefficients], int(steps), float(eps))
+        self._ck(self.lib.dlmi_orthogonalize(self.ctx, kind, c_sz(rows), c_sz(cols), _p(G), _p(o), ctypes.byref(ns)))
+        return o
+
+    def opt_muon(self, problems, lr, momentum=0.95, wd=0.0, nesterov=True, steps=5, coefficients=(3.4445, -4.7750, 2.0315),
+                 eps=1e-7):
+        """One Muon step of several float32 matrices, in place: problems is a list of (p, g, m) or, with a step size of
+        its own, (p, g, m, lr) (dlmi_opt_muon).  The gradients end up zero."""
+        arr = (MuonProblem * max(1, len(problems)))()
+        for a, q in zip(arr, problems):
+            p, g, m = q[:3]
+            assert p.dim() == 2
+            for t, what in ((p, "p"), (g, "g"), (m, "m")):
+                self._chk_is(t, what, self.torch.float32, *p.shape)
+            a.rows, a.cols = p.shape
+            a.params, a.grads, a.momentum = _p(p), _p(g), _p(m)
+            a.lr = float(q[3]) if len(q) > 3 else float(lr)
+        ns = NewtonSchulz(*[float(c) for c in coefficients], int(steps), float(eps))
+        self._ck(self.lib.dlmi_opt_muon(self.ctx, c_sz(len(problems)), arr, c_f(momentum), c_int(1 if nesterov else 0), c_f(wd),
+                                        ctypes.byref(ns)))
 
     def opt_adabound(self, p, g, m1, m2, vhat, mask, lr_t, beta1, beta2, eps, wd, rate_lower, rate_upper, nthreads=0):
         self._chk(p, g, m1, m2, vhat, mask)

@@ -108,6 +108,15 @@ inline int dlmi_fail(dlmi_ctx *ctx, int code, char const *fmt, ...) {
     if (!(cond)) return dlmi_fail((ctx), DLMI_E_INVALID, "%s: %s", __func__, (msg));      \
   } while (0)
 
+// Launches go to the current device: entry points that check refuse a call made with another one current, where the null
+// stream would run the kernels on the wrong device's memory.
+#define DLMI_REQUIRE_DEVICE(ctx)                                                         \
+  do {                                                                                   \
+    int d_ = -1;                                                                         \
+    if (hipGetDevice(&d_) != hipSuccess || d_ != (ctx)->device)                          \
+      return dlmi_fail((ctx), DLMI_E_INVALID, "%s: the context's device is not current", __func__); \
+  } while (0)
+
 // Makes sure the context's scratch holds at least `bytes`.
 // Growing allocates (and synchronizes the stream): it is refused while the
 // stream is being captured into a HIP graph.

@@ -1,0 +1,315 @@
+// Matrix products on the 16-bit matrix pipe: the K loop that the Muon step (muon_kernels.hip) and the vocabulary cross
+// entropy (vocab_ce.hip) share, and the operand format it reads.
+//
+// C[i][j] = sum_k P[i][k] Q[j][k], both operands given as "packed" matrices: 32 rows x 16 k are one fragment of
+// 1 KiB, lane l of a wavefront holding row l & 31 and the 8 consecutive k from 8 (l >> 5), which is how
+// v_mfma_f32_32x32x16_f16 takes its operands.  Fragments lie [row block][k block][plane].  So a fragment goes from
+// memory to LDS as one 16-byte-per-lane direct load, is read back as one ds_read_b128 in lane order (no bank is hit
+// twice), and the loop has no bounds to check: whoever packs pads rows and k with zeros.
+//
+// Planes.  One plane holds a value rounded to f16 (11 significant bits: what a bf16 input has, and more).  Two planes
+// hold x = hi + lo, each f16, 22 bits in all; the product is hi hi + hi lo + lo hi, three matrix instructions, accumulated
+// in fp32.  The dropped lo lo is below 2^-22 of a term, so the result is as good as a product of fp32 values, at a third
+// of the 16-bit rate = 833 TFLOP/s against 157 TFLOP/s on the fp32 matrix pipe.  f16 has 5 exponent bits: the packer
+// multiplies by a power of two so that the largest magnitude lies near the top of the range; what is 2^-18 of it or
+// smaller loses bits of its lo (an absolute error below 2^-40 of the largest).
+#pragma once
+
+#include "dlmi_common.hpp"
+
+namespace dlmi {
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kFragBytes = 1024;
+
+// Bytes of a packed matrix of `rows` x `k` (both already padded: rows to 32, k to 16).
+inline size_t packed_bytes(size_t rows, size_t k, int planes) { return rows * k * 2 * planes; }
+
+// One step of the K loop reads one stage of LDS: KS k blocks of all planes of the BM + BN rows.
+template <int BM, int BN, int NP>
+struct HalfTile {
+  static constexpr int kPlanes = NP;
+  static constexpr int KS = 2 / NP;                          // k blocks per stage
+  static constexpr int kBufs = 4;                            // stages in LDS
+  static constexpr int kMB = BM / 64, kNB = BN / 64;         // 32 x 32 blocks of a wavefront, 2 x 2 wavefronts
+  static constexpr int kFragsA = BM / 32 * 2, kFragsB = BN / 32 * 2;  // fragments of a stage (KS * NP == 2)
+  static constexpr int kStageBytes = (kFragsA + kFragsB) * kFragBytes;
+  static constexpr int kLoads = (kFragsA + kFragsB) / 4;     // direct loads of a wavefront per stage
+};
+
+template <class T>
+struct HalfAcc {
+  f32x16 v[T::kMB][T::kNB];
+};
+
+template <int BM, int BN, int NP>
+__device__ __forceinline__ void half_stage_load(char *lds, char const *P, char const *Q, size_t row_stride_p,
+                                                size_t row_stride_q, int wave, int lane) {
+  using T = HalfTile<BM, BN, NP>;
+  // fragment f of an operand: row block f >> 1, the (f & 1)-th KiB of its KS k blocks x NP planes
+#pragma unroll
+  for (int u = 0; u < T::kFragsA / 4; ++u) {
+    int const f = u * 4 + wave;
+    char const *src = P + static_cast<size_t>(f >> 1) * row_stride_p + (f & 1) * kFragBytes + lane * 16;
+    __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void const *)src,
+                                     (__attribute__((address_space(3))) void *)(lds + f * kFragBytes), 16, 0, 0);
+  }
+#pragma unroll
+  for (int u = 0; u < T::kFragsB / 4; ++u) {
+    int const f = u * 4 + wave;
+    char const *src = Q + static_cast<size_t>(f >> 1) * row_stride_q + (f & 1) * kFragBytes + lane * 16;
+    __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void const *)src,
+                                     (__attribute__((address_space(3))) void *)(lds + (T::kFragsA + f) * kFragBytes), 16,
+                                     0, 0);
+  }
+}
+
+// The fragments of one k block (all planes) that a wavefront multiplies.
+template <class T>
+struct HalfFrags {
+  half8 p[T::kPlanes][T::kMB], q[T::kPlanes][T::kNB];
+};
+
+template <class T>
+__device__ __forceinline__ void half_frags_read(HalfFrags<T> &f, char const *lds, int ks, int wm, int wn, int lane) {
+#pragma unroll
+  for (int pl = 0; pl < T::kPlanes; ++pl) {
+#pragma unroll
+    for (int m = 0; m < T::kMB; ++m)
+      f.p[pl][m] = *reinterpret_cast<half8 const *>(lds + (((wm * T::kMB + m) * 2 + ks * T::kPlanes + pl) * kFragBytes + lane * 16));
+#pragma unroll
+    for (int n = 0; n < T::kNB; ++n)
+      f.q[pl][n] = *reinterpret_cast<half8 const *>(
+          lds + ((T::kFragsA + (wn * T::kNB + n) * 2 + ks * T::kPlanes + pl) * kFragBytes + lane * 16));
+  }
+}
+
+template <class T>
+__device__ __forceinline__ void half_mfma(HalfAcc<T> &acc, HalfFrags<T> const &f) {
+#pragma unroll
+  for (int t = 0; t < (T::kPlanes == 2 ? 3 : 1); ++t) {
+    int const pp = t == 2 ? 1 : 0, qp = t == 1 ? 1 : 0;
+#pragma unroll
+    for (int m = 0; m < T::kMB; ++m)
+#pragma unroll
+      for (int n = 0; n < T::kNB; ++n)
+        acc.v[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.p[pp][m], f.q[qp][n], acc.v[m][n], 0, 0, 0);
+  }
+}
+
+// Waits until at most the last `flying` stages requested are still on their way and this wavefront's own LDS reads are
+// done, then lets all wavefronts of the workgroup pass together.  (The empty asm statements keep the compiler from
+// moving LDS accesses across the barrier, which by itself is no fence.)
+template <class T, int flying>
+__device__ __forceinline__ void half_stage_wait() {
+  constexpr int n = flying * T::kLoads;
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0070 | (n & 15) | ((n >> 4) << 14));  // vmcnt(n) lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// The K loop of one workgroup (256 threads, wavefronts 2 x 2) over `stages` >= 1 stages.  P, Q: the first fragment of the
+// tile's first row block at the first k block; row_stride_*: bytes from one row block to the next.
+template <int BM, int BN, int NP>
+__device__ __forceinline__ void half_gemm(HalfAcc<HalfTile<BM, BN, NP>> &acc, char const *P, char const *Q,
+                                          size_t row_stride_p, size_t row_stride_q, int stages) {
+  using T = HalfTile<BM, BN, NP>;
+  __shared__ __attribute__((aligned(1024))) char buf0[T::kStageBytes];
+  __shared__ __attribute__((aligned(1024))) char buf1[T::kStageBytes];
+  __shared__ __attribute__((aligned(1024))) char buf2[T::kStageBytes];
+  __shared__ __attribute__((aligned(1024))) char buf3[T::kStageBytes];
+  char *const bufs[4] = {buf0, buf1, buf2, buf3};
+  int const lane = threadIdx.x & 63;
+  int const wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int const wm = wave >> 1, wn = wave & 1;
+#pragma unroll
+  for (int m = 0; m < T::kMB; ++m)
+#pragma unroll
+    for (int n = 0; n < T::kNB; ++n) acc.v[m][n] = f32x16{};
+
+  auto const load = [&](char *buf, int t) {
+    half_stage_load<BM, BN, NP>(buf, P + static_cast<size_t>(t) * 2 * kFragBytes, Q + static_cast<size_t>(t) * 2 * kFragBytes,
+                                row_stride_p, row_stride_q, wave, lane);
+  };
+  // the first three stages are requested before the first is waited for
+  load(bufs[0], 0);
+  if (stages > 1) load(bufs[1], 1);
+  if (stages > 2) load(bufs[2], 2);
+  if (stages > 2)
+    half_stage_wait<T, 2>();
+  else if (stages > 1)
+    half_stage_wait<T, 1>();
+  else
+    half_stage_wait<T, 0>();
+  HalfFrags<T> cur, nxt;
+  half_frags_read<T>(cur, bufs[0], 0, wm, wn, lane);
+  // One stage: the fragments of a k block are multiplied while those of the next are read.  Before the last k block is
+  // multiplied the next stage has landed and every wavefront has read all of the stage before this one, whose buffer
+  // is then filled again.
+  int t0 = 0;
+  for (; t0 + 6 < stages; t0 += 4) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+#pragma unroll
+      for (int ks = 0; ks < T::KS; ++ks) {
+        if (ks + 1 < T::KS) {
+          half_frags_read<T>(nxt, bufs[u], ks + 1, wm, wn, lane);
+        } else {
+          half_stage_wait<T, 1>();
+          load(bufs[(u + 3) & 3], t0 + u + 3);
+          half_frags_read<T>(nxt, bufs[(u + 1) & 3], 0, wm, wn, lane);
+        }
+        half_mfma<T>(acc, cur);
+        cur = nxt;
+      }
+    }
+  }
+  for (; t0 < stages; t0 += 4) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      int const t = t0 + u;
+      if (t < stages) {
+#pragma unroll
+        for (int ks = 0; ks < T::KS; ++ks) {
+          if (ks + 1 < T::KS) {
+            half_frags_read<T>(nxt, bufs[u], ks + 1, wm, wn, lane);
+          } else if (t + 1 < stages) {
+            if (t + 2 < stages)
+              half_stage_wait<T, 1>();
+            else
+              half_stage_wait<T, 0>();
+            if (t + 3 < stages) load(bufs[(u + 3) & 3], t + 3);
+            half_frags_read<T>(nxt, bufs[(u + 1) & 3], 0, wm, wn, lane);
+          }
+          half_mfma<T>(acc, cur);
+          cur = nxt;
+        }
+      }
+    }
+  }
+}
+
+// ---- a 32 x 32 block of C in registers (lane l: column j = l & 31, rows i = 8 (r >> 2) + 4 (l >> 5) + (r & 3)) -------------
+
+// The block as two packed fragments of the transposed matrix (row j, k = i): k block 0 and 1.
+struct HalfPair {
+  half8 k0, k1;
+};
+
+__device__ __forceinline__ half8 half_join(half4 a, half4 b) {
+  // rows 0-31 of a lane pair hold k 0-3 | 4-7 of two k octets: swapping the upper half of the first with the lower half
+  // of the second leaves every lane one whole octet
+  typedef unsigned u2 __attribute__((ext_vector_type(2)));
+  u2 const ua = __builtin_bit_cast(u2, a), ub = __builtin_bit_cast(u2, b);
+  auto const x = __builtin_amdgcn_permlane32_swap(ua[0], ub[0], false, false);
+  auto const y = __builtin_amdgcn_permlane32_swap(ua[1], ub[1], false, false);
+  u32x4 const r = {x[0], y[0], x[1], y[1]};
+  return __builtin_bit_cast(half8, r);
+}
+__device__ __forceinline__ void half_part(half8 v, half4 &a, half4 &b) {  // the inverse
+  typedef unsigned u2 __attribute__((ext_vector_type(2)));
+  u32x4 const r = __builtin_bit_cast(u32x4, v);
+  auto const x = __builtin_amdgcn_permlane32_swap(r[0], r[2], false, false);
+  auto const y = __builtin_amdgcn_permlane32_swap(r[1], r[3], false, false);
+  u2 const ua = {x[0], y[0]}, ub = {x[1], y[1]};
+  a = __builtin_bit_cast(half4, ua);
+  b = __builtin_bit_cast(half4, ub);
+}
+
+template <int NP>
+struct HalfBlock {
+  HalfPair pl[NP];
+};
+
+// Rounds the block to its planes (each to nearest even; the second holds what the first lost).
+template <int NP>
+__device__ __forceinline__ HalfBlock<NP> half_split(f32x16 const &v) {
+  half4 h[4], l[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      float const x = v[q * 4 + t];
+      _Float16 const hi = static_cast<_Float16>(x);
+      h[q][t] = hi;
+      if constexpr (NP == 2) l[q][t] = static_cast<_Float16>(x - static_cast<float>(hi));
+    }
+  HalfBlock<NP> b;
+  b.pl[0].k0 = half_join(h[0], h[1]);
+  b.pl[0].k1 = half_join(h[2], h[3]);
+  if constexpr (NP == 2) {
+    b.pl[1].k0 = half_join(l[0], l[1]);
+    b.pl[1].k1 = half_join(l[2], l[3]);
+  }
+  return b;
+}
+
+// dst: fragment (row block of j, k block of i) of the packed matrix; the block's second k block follows its planes.
+template <int NP>
+__device__ __forceinline__ void half_store(char *dst, HalfBlock<NP> const &b, int lane) {
+#pragma unroll
+  for (int p = 0; p < NP; ++p) {
+    *reinterpret_cast<half8 *>(dst + p * kFragBytes + lane * 16) = b.pl[p].k0;
+    *reinterpret_cast<half8 *>(dst + (NP + p) * kFragBytes + lane * 16) = b.pl[p].k1;
+  }
+}
+
+template <int NP>
+__device__ __forceinline__ f32x16 half_load(char const *src, int lane) {
+  f32x16 v = {};
+#pragma unroll
+  for (int p = 0; p < NP; ++p) {
+    half4 a[4];
+    half_part(*reinterpret_cast<half8 const *>(src + p * kFragBytes + lane * 16), a[0], a[1]);
+    half_part(*reinterpret_cast<half8 const *>(src + (NP + p) * kFragBytes + lane * 16), a[2], a[3]);
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int t = 0; t < 4; ++t) v[q * 4 + t] += static_cast<float>(a[q][t]);
+  }
+  return v;
+}
+
+// Lane l's octet of rows 0-15 (half 0) or 16-31 (half 1) of the 32-column identity.
+__device__ __forceinline__ half8 half_identity(int half, int lane) {
+  half8 r;
+#pragma unroll
+  for (int t = 0; t < 8; ++t) r[t] = static_cast<_Float16>((lane & 31) == half * 16 + (lane >> 5) * 8 + t ? 1.0f : 0.0f);
+  return r;
+}
+
+// The plane of a block (fragments of the transposed matrix) times the identity: lane l then holds, in the layout of C, the
+// transposed block (column i = l & 31, rows j).  One term per sum: exact.
+__device__ __forceinline__ f32x16 half_transposed(HalfPair const &p, half8 id0, half8 id1) {
+  f32x16 z = {};
+  z = __builtin_amdgcn_mfma_f32_32x32x16_f16(p.k0, id0, z, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(p.k1, id1, z, 0, 0, 0);
+}
+
+// The same block packed the other way round (row i, k = j).
+template <int NP>
+__device__ __forceinline__ HalfBlock<NP> half_flip(HalfBlock<NP> const &b, half8 id0, half8 id1) {
+  HalfBlock<NP> r;
+#pragma unroll
+  for (int p = 0; p < NP; ++p) {
+    f32x16 const t = half_transposed(b.pl[p], id0, id1);
+    HalfBlock<1> const o = half_split<1>(t);
+    r.pl[p] = o.pl[0];
+  }
+  return r;
+}
+
+// Workgroup number -> number in an order in which the workgroups of one XCD (numbers equal modulo 8) are consecutive.
+__device__ __forceinline__ unsigned xcd_consecutive(unsigned id, unsigned n) {
+  unsigned const q = n >> 3, r = n & 7, x = id & 7;
+  return x * q + (x < r ? x : r) + (id >> 3);
+}
+
+}  // namespace dlmi

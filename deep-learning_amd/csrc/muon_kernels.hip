@@ -1,0 +1,434 @@
+// Newton-Schulz orthogonalization of a matrix and the Muon optimizer step built on it, for gfx950.
+//
+//   m <- momentum m + g;  u = nesterov ? g + momentum m : m
+//   X <- u / (|u|_F + eps), on its short side (transposed when rows > cols)
+//   `steps` times:  A = X X^T;  X <- a X + (b A + c A A) X
+//   p <- p - lr X - wd p
+//
+// Each step maps the singular values of X by a s + b s^3 + c s^5 and leaves its singular vectors: all of them end near 1.
+// Bound by the 16-bit matrix pipe: per step s^2 l (X X^T, half of it: A is symmetric) + s^3 (A A, half) + 2 s^2 l
+// operations, s the short and l the long side, times three for the two planes of half_gemm.hpp.
+//
+// Precision.  The polynomial multiplies what lies in weak directions by up to a^steps (485 for 5 steps of 3.4445), the
+// rounding of the operands among it.  With one f16 plane a random matrix ends 1.3e-3 off and a matrix of rank 32 plus 1 %
+// noise 2.7e-2; with two planes (22 bits) 1.8e-6 and 1.2e-5, as far as a computation in fp32 (1.1e-5 and 1.9e-5).  So X,
+// A and b A + c A A keep two planes throughout, whatever the type of the result.  Singular values stay below about 1.3
+// and the polynomial in A below 3, so all three matrices are held times 2^12: far from the ends of f16's range.
+//
+// X is kept both ways round (rows i, k = j for X X^T; rows j, k = i for the product by X), each written by the product
+// that makes it: a block of C in registers is a fragment of the transposed matrix as it stands, and two matrix
+// instructions by the identity turn it.
+#include <algorithm>
+#include <cmath>
+#include <new>
+#include <vector>
+
+#include "half_gemm.hpp"
+
+namespace dlmi {
+
+constexpr int kMuonMax = 32;         // matrices per launch
+constexpr int kMuonBlock = 256;
+constexpr float kMuonScale = 4096.0f;
+
+struct MuonBatch {
+  void *p[kMuonMax];        // parameters (step) or output (orthogonalize)
+  void *g[kMuonMax];        // gradient or input
+  float *m[kMuonMax];
+  float lr[kMuonMax];
+};
+
+__device__ __forceinline__ double muon_block_sum(double s, double *lds) {
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = s;
+  __syncthreads();
+  s = (lds[0] + lds[1]) + (lds[2] + lds[3]);
+  __syncthreads();
+  return s;
+}
+
+// The momentum, and partial[matrix][block] = sum of u^2 (double: the norm of a tiny gradient does not underflow).
+template <class T, bool STEP>
+__global__ __launch_bounds__(kMuonBlock) void k_muon_moment(MuonBatch b, size_t n, float momentum, int nesterov, double *partial) {
+  __shared__ double lds[kMuonBlock / 64];
+  T const *const g = static_cast<T const *>(b.g[blockIdx.y]);
+  float *const m = b.m[blockIdx.y];
+  double s = 0.0;
+  for (size_t i = static_cast<size_t>(blockIdx.x) * kMuonBlock + threadIdx.x; i < n; i += static_cast<size_t>(gridDim.x) * kMuonBlock) {
+    float u = static_cast<float>(g[i]);
+    if constexpr (STEP) {
+      float const v = momentum * m[i] + u;
+      m[i] = v;
+      u = nesterov ? u + momentum * v : v;
+    }
+    s += static_cast<double>(u) * u;
+  }
+  s = muon_block_sum(s, lds);
+  if (threadIdx.x == 0) partial[static_cast<size_t>(blockIdx.y) * gridDim.x + blockIdx.x] = s;
+}
+
+// One 64 x 64 tile of u / (|u| + eps), packed as it stands (row r, k = c: `rc`) and transposed (row c, k = r: `cr`);
+// padding is zero.  A step's gradient is cleared on the way.
+template <class T, bool STEP>
+__global__ __launch_bounds__(kMuonBlock) void k_muon_pack(MuonBatch b, unsigned R, unsigned C, unsigned Rp, unsigned Cp, float momentum,
+                                                          int nesterov, float eps, double const *partial, unsigned nparts, char *rc,
+                                                          char *cr, size_t stride) {
+  __shared__ double sums[kMuonBlock / 64];
+  __shared__ float tile[64][65];
+  unsigned const mat = blockIdx.z;
+  double s = 0.0;
+  for (unsigned i = threadIdx.x; i < nparts; i += kMuonBlock) s += partial[static_cast<size_t>(mat) * nparts + i];
+  s = muon_block_sum(s, sums);
+  double const inv = static_cast<double>(kMuonScale) / (sqrt(s) + static_cast<double>(eps));  // double: of a tiny gradient it passes fp32's range
+  T *const g = static_cast<T *>(b.g[mat]);
+  float const *const m = b.m[mat];
+  unsigned const r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
+  unsigned const tc = threadIdx.x & 63;
+#pragma unroll
+  for (int q = 0; q < 16; ++q) {
+    unsigned const tr = q * 4 + (threadIdx.x >> 6);
+    unsigned const r = r0 + tr, c = c0 + tc;
+    float u = 0.0f;
+    if (r < R && c < C) {
+      size_t const at = static_cast<size_t>(r) * C + c;
+      u = static_cast<float>(g[at]);
+      if constexpr (STEP) {
+        float const v = m[at];
+        u = nesterov ? u + momentum * v : v;
+        g[at] = static_cast<T>(0.0f);
+      }
+    }
+    tile[tr][tc] = static_cast<float>(u * inv);
+  }
+  __syncthreads();
+  int const lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  char *const drc = rc + mat * stride, *const dcr = cr + mat * stride;
+  unsigned const kbs = Cp / 16, kbr = Rp / 16;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    int const f = q * 4 + wave;       // 16 fragments: 8 as it stands, 8 transposed
+    bool const flip = f >= 8;
+    int const rb = (f >> 2) & 1, kb = f & 3;
+    half8 hi, lo;
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+      int const row = rb * 32 + (lane & 31), k = kb * 16 + (lane >> 5) * 8 + t;
+      float const x = flip ? tile[k][row] : tile[row][k];
+      _Float16 const h = static_cast<_Float16>(x);
+      hi[t] = h;
+      lo[t] = static_cast<_Float16>(x - static_cast<float>(h));
+    }
+    size_t const frag = flip ? static_cast<size_t>(c0 / 32 + rb) * kbr + r0 / 16 + kb : static_cast<size_t>(r0 / 32 + rb) * kbs + c0 / 16 + kb;
+    char *const dst = (flip ? dcr : drc) + frag * 2 * kFragBytes + lane * 16;
+    *reinterpret_cast<half8 *>(dst) = hi;
+    *reinterpret_cast<half8 *>(dst + kFragBytes) = lo;
+  }
+}
+
+// A tile of a symmetric product C = P P^T (P: [mp, k] packed), only the tiles on and below the diagonal; written packed
+// with its mirror image.  POLY: C = b P + c P P^T (P symmetric itself).  Products of two values held times 2^12.
+template <int T, bool POLY>
+__global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_muon_symmetric(char const *P, char *C, size_t stride_p, size_t stride_c,
+                                                                         unsigned tiles, unsigned kblocks, unsigned kblocks_c,
+                                                                         float cb, float cc) {
+  using H = HalfTile<T, T, 2>;
+  unsigned const tri = tiles * (tiles + 1) / 2;
+  unsigned const id = xcd_consecutive(blockIdx.x, gridDim.x);
+  unsigned const mat = id / tri, t = id - mat * tri;
+  unsigned ti = static_cast<unsigned>((sqrtf(8.0f * static_cast<float>(t) + 1.0f) - 1.0f) * 0.5f);
+  while (ti * (ti + 1) / 2 > t) --ti;
+  while ((ti + 1) * (ti + 2) / 2 <= t) ++ti;
+  unsigned const tj = t - ti * (ti + 1) / 2;
+  char const *const p = P + mat * stride_p;
+  size_t const rs = static_cast<size_t>(kblocks) * 2 * kFragBytes;
+  HalfAcc<H> acc;
+  half_gemm<T, T, 2>(acc, p + ti * (T / 32) * rs, p + tj * (T / 32) * rs, rs, rs, kblocks);
+  int const lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  half8 const id0 = half_identity(0, lane), id1 = half_identity(1, lane);
+  char *const c = C + mat * stride_c;
+  size_t const rc = static_cast<size_t>(kblocks_c) * 2 * kFragBytes;
+#pragma unroll
+  for (int m = 0; m < H::kMB; ++m)
+#pragma unroll
+    for (int n = 0; n < H::kNB; ++n) {
+      unsigned const ib = ti * (T / 32) + (wave >> 1) * H::kMB + m, jb = tj * (T / 32) + (wave & 1) * H::kNB + n;
+      f32x16 v = acc.v[m][n] * (cc / kMuonScale);
+      if constexpr (POLY) v += cb * half_load<2>(p + jb * rs + ib * 4 * kFragBytes, lane);
+      HalfBlock<2> const blk = half_split<2>(v);
+      half_store<2>(c + jb * rc + ib * 4 * kFragBytes, blk, lane);
+      if (ti != tj) half_store<2>(c + ib * rc + jb * 4 * kFragBytes, half_flip<2>(blk, id0, id1), lane);
+    }
+}
+
+enum { kMuonMore = 0, kMuonOut = 1, kMuonStep = 2 };
+
+struct MuonOut {
+  unsigned rows, cols;   // of the caller's matrix
+  int flipped;           // X is the transposed matrix
+  float wd;
+};
+
+// A tile of X' = a X + Bm X; XT = X^T packed (row j, k = i).  MORE: written packed both ways; OUT, STEP: the last of the
+// iteration, written to the caller's matrix.
+template <int T, int MODE, class O>
+__global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_muon_update(char const *Bm, char const *XT, char *XTn, char *XP,
+                                                                      size_t stride_b, size_t stride_x, unsigned mt, unsigned nt,
+                                                                      unsigned kbm, unsigned kbn, float ca, MuonBatch b, MuonOut o) {
+  using H = HalfTile<T, T, 2>;
+  unsigned const id = xcd_consecutive(blockIdx.x, gridDim.x);
+  unsigned const mat = id / (mt * nt), t = id - mat * (mt * nt);
+  unsigned const ti = t % mt, tj = t / mt;
+  size_t const rs = static_cast<size_t>(kbm) * 2 * kFragBytes, rn = static_cast<size_t>(kbn) * 2 * kFragBytes;
+  char const *const xt = XT + mat * stride_x;
+  HalfAcc<H> acc;
+  half_gemm<T, T, 2>(acc, Bm + mat * stride_b + ti * (T / 32) * rs, xt + tj * (T / 32) * rs, rs, rs, kbm);
+  int const lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  half8 const id0 = half_identity(0, lane), id1 = half_identity(1, lane);
+#pragma unroll
+  for (int m = 0; m < H::kMB; ++m)
+#pragma unroll
+    for (int n = 0; n < H::kNB; ++n) {
+      unsigned const ib = ti * (T / 32) + (wave >> 1) * H::kMB + m, jb = tj * (T / 32) + (wave & 1) * H::kNB + n;
+      f32x16 v = acc.v[m][n] * (1.0f / kMuonScale) + ca * half_load<2>(xt + jb * rs + ib * 4 * kFragBytes, lane);
+      if constexpr (MODE == kMuonMore) {
+        HalfBlock<2> const blk = half_split<2>(v);
+        half_store<2>(XTn + mat * stride_x + jb * rs + ib * 4 * kFragBytes, blk, lane);
+        half_store<2>(XP + mat * stride_x + ib * rn + jb * 4 * kFragBytes, half_flip<2>(blk, id0, id1), lane);
+      } else {
+        v *= 1.0f / kMuonScale;
+        O *const p = static_cast<O *>(b.p[mat]);
+        unsigned const j = jb * 32 + (lane & 31);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          unsigned const i = ib * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+          unsigned const row = o.flipped ? j : i, col = o.flipped ? i : j;
+          if (row < o.rows && col < o.cols) {
+            size_t const at = static_cast<size_t>(row) * o.cols + col;
+            if constexpr (MODE == kMuonStep) {
+              float const w = static_cast<float>(p[at]);
+              p[at] = static_cast<O>(w - (b.lr[mat] * v[r] + o.wd * w));
+            } else {
+              p[at] = static_cast<O>(v[r]);
+            }
+          }
+        }
+      }
+    }
+}
+
+// The iteration's bounds for singular values in [0, 1]: largest magnitude of X X^T and of b A + c A A on the way.
+static double muon_reach(float const *coefs, int steps) {
+  double most = 1.0;
+  for (int i = 0; i <= 2048; ++i) {
+    double s = i / 2048.0;
+    for (int k = 0; k < steps; ++k) {
+      double const q = s * s, poly = coefs[1] * q + coefs[2] * q * q;
+      s = coefs[0] * s + poly * s;
+      if (!(std::fabs(poly) <= 1e6) || !(std::fabs(s) <= 1e6)) return 1e6;
+      if (std::fabs(poly) > most) most = std::fabs(poly);
+      if (s * s > most) most = s * s;
+    }
+  }
+  return most;
+}
+
+struct MuonPlan {
+  int flipped;
+  size_t mp, np, bytes_x, bytes_a, per_matrix;
+  int tile;
+  unsigned nparts;
+};
+
+static MuonPlan muon_plan(dlmi_ctx const *ctx, size_t rows, size_t cols, size_t count) {
+  MuonPlan pl;
+  pl.flipped = rows > cols;
+  size_t const s = pl.flipped ? cols : rows, l = pl.flipped ? rows : cols;
+  pl.tile = 64;
+  for (int T : {256, 128}) {
+    size_t const tiles = dlmi_ceil_div(s, T) * dlmi_ceil_div(l, T) * count;
+    if (tiles >= static_cast<size_t>(ctx->num_cu) * 3 / 4) {
+      pl.tile = T;
+      break;
+    }
+  }
+  pl.mp = dlmi_ceil_div(s, pl.tile) * pl.tile;
+  pl.np = dlmi_ceil_div(l, pl.tile) * pl.tile;
+  pl.bytes_x = packed_bytes(pl.mp, pl.np, 2);
+  pl.bytes_a = packed_bytes(pl.mp, pl.mp, 2);
+  pl.nparts = static_cast<unsigned>(dlmi_ceil_div(rows * cols, kMuonBlock * 8));
+  if (pl.nparts > 256) pl.nparts = 256;
+  pl.per_matrix = 3 * pl.bytes_x + 2 * pl.bytes_a + dlmi_ceil_div(pl.nparts * sizeof(double), 1024) * 1024;
+  return pl;
+}
+
+template <int T, class O>
+static int muon_iterate(dlmi_ctx *ctx, MuonBatch const &b, MuonPlan const &pl, unsigned count, float const *coefs, int steps,
+                        MuonOut const &o, int last_mode, char *XP, char *XT, char *XTn, char *A, char *Bm) {
+  unsigned const mt = static_cast<unsigned>(pl.mp / T), nt = static_cast<unsigned>(pl.np / T);
+  unsigned const kbm = static_cast<unsigned>(pl.mp / 16), kbn = static_cast<unsigned>(pl.np / 16);
+  dim3 const tri(mt * (mt + 1) / 2 * count), all(mt * nt * count);
+  for (int s = 0; s < steps; ++s) {
+    hipLaunchKernelGGL((k_muon_symmetric<T, false>), tri, dim3(256), 0, ctx->stream, XP, A, pl.bytes_x, pl.bytes_a, mt, kbn, kbm, 0.0f,
+                       1.0f);
+    DLMI_LAUNCH_CHECK(ctx, "k_muon_symmetric");
+    hipLaunchKernelGGL((k_muon_symmetric<T, true>), tri, dim3(256), 0, ctx->stream, A, Bm, pl.bytes_a, pl.bytes_a, mt, kbm, kbm,
+                       coefs[1], coefs[2]);
+    DLMI_LAUNCH_CHECK(ctx, "k_muon_symmetric");
+    if (s + 1 < steps)
+      hipLaunchKernelGGL((k_muon_update<T, kMuonMore, O>), all, dim3(256), 0, ctx->stream, Bm, XT, XTn, XP, pl.bytes_a, pl.bytes_x, mt, nt,
+                         kbm, kbn, coefs[0], b, o);
+    else if (last_mode == kMuonStep)
+      hipLaunchKernelGGL((k_muon_update<T, kMuonStep, O>), all, dim3(256), 0, ctx->stream, Bm, XT, XTn, XP, pl.bytes_a, pl.bytes_x, mt, nt,
+                         kbm, kbn, coefs[0], b, o);
+    else
+      hipLaunchKernelGGL((k_muon_update<T, kMuonOut, O>), all, dim3(256), 0, ctx->stream, Bm, XT, XTn, XP, pl.bytes_a, pl.bytes_x, mt, nt,
+                         kbm, kbn, coefs[0], b, o);
+    DLMI_LAUNCH_CHECK(ctx, "k_muon_update");
+    std::swap(XT, XTn);
+  }
+  return DLMI_OK;
+}
+
+// `count` matrices of one shape, at most kMuonMax of them; the scratch has been reserved.
+template <class T, bool STEP>
+static int muon_batch(dlmi_ctx *ctx, MuonBatch const &b, size_t rows, size_t cols, unsigned count, MuonPlan const &pl, float momentum,
+                      int nesterov, float wd, int steps, float const *coefs, float eps) {
+  char *const XP = dlmi_scratch_data(ctx), *const XT = XP + count * pl.bytes_x, *const XTn = XT + count * pl.bytes_x;
+  char *const A = XTn + count * pl.bytes_x, *const Bm = A + count * pl.bytes_a;
+  double *const partial = reinterpret_cast<double *>(Bm + count * pl.bytes_a);
+  size_t const n = rows * cols;
+  hipLaunchKernelGGL((k_muon_moment<T, STEP>), dim3(pl.nparts, count), dim3(kMuonBlock), 0, ctx->stream, b, n, momentum, nesterov, partial);
+  DLMI_LAUNCH_CHECK(ctx, "k_muon_moment");
+  size_t const Rp = pl.flipped ? pl.np : pl.mp, Cp = pl.flipped ? pl.mp : pl.np;
+  hipLaunchKernelGGL((k_muon_pack<T, STEP>), dim3(static_cast<unsigned>(Cp / 64), static_cast<unsigned>(Rp / 64), count), dim3(kMuonBlock), 0,
+                     ctx->stream, b, static_cast<unsigned>(rows), static_cast<unsigned>(cols), static_cast<unsigned>(Rp),
+                     static_cast<unsigned>(Cp), momentum, nesterov, eps, partial, pl.nparts, pl.flipped ? XT : XP, pl.flipped ? XP : XT,
+                     pl.bytes_x);
+  DLMI_LAUNCH_CHECK(ctx, "k_muon_pack");
+  MuonOut const o{static_cast<unsigned>(rows), static_cast<unsigned>(cols), pl.flipped, wd};
+  int const mode = STEP ? kMuonStep : kMuonOut;
+  if (pl.tile == 256) return muon_iterate<256, T>(ctx, b, pl, count, coefs, steps, o, mode, XP, XT, XTn, A, Bm);
+  if (pl.tile == 128) return muon_iterate<128, T>(ctx, b, pl, count, coefs, steps, o, mode, XP, XT, XTn, A, Bm);
+  return muon_iterate<64, T>(ctx, b, pl, count, coefs, steps, o, mode, XP, XT, XTn, A, Bm);
+}
+
+static char const *muon_check(dlmi_newton_schulz const *ns) {
+  if (ns == nullptr) return "null pointer";
+  if (ns->steps < 1 || ns->steps > 64) return "1 to 64 steps";
+  if (!(ns->eps >= 0.0f)) return "eps must not be negative";
+  float const c[3] = {ns->a, ns->b, ns->c};
+  if (!(muon_reach(c, ns->steps) <= 8.0)) return "coefficients that take singular values of [0, 1] out of the range the iteration is held in";
+  return nullptr;
+}
+
+// Scratch that the matrices of one launch may take together.
+constexpr size_t kMuonBudget = size_t(2) << 30;
+
+static unsigned muon_group(MuonPlan const &pl, size_t left) {
+  size_t n = kMuonBudget / pl.per_matrix;
+  if (n < 1) n = 1;
+  if (n > kMuonMax) n = kMuonMax;
+  return static_cast<unsigned>(n < left ? n : left);
+}
+
+}  // namespace dlmi
+
+using namespace dlmi;
+
+extern "C" {
+
+int dlmi_orthogonalize(dlmi_ctx *ctx, dlmi_dtype type, size_t rows, size_t cols, void const *G, void *O, dlmi_newton_schulz const *ns) {
+  if (ctx == nullptr) return DLMI_E_INVALID;
+  DLMI_REQUIRE(ctx, type == DLMI_F32 || type == DLMI_BF16, "unknown type");
+  char const *const wrong = muon_check(ns);
+  DLMI_REQUIRE(ctx, wrong == nullptr, wrong);
+  DLMI_REQUIRE(ctx, rows <= DLMI_MUON_MAX_SIDE && cols <= DLMI_MUON_MAX_SIDE, "matrix too large");
+  if (rows * cols == 0) return DLMI_OK;
+  DLMI_REQUIRE_DEVICE(ctx);
+  DLMI_REQUIRE(ctx, G != nullptr && O != nullptr, "null pointer");
+  MuonBatch b = {};
+  b.p[0] = O;
+  b.g[0] = const_cast<void *>(G);
+  float const c[3] = {ns->a, ns->b, ns->c};
+  MuonPlan const pl = muon_plan(ctx, rows, cols, 1);
+  int const rc = dlmi_scratch_reserve(ctx, pl.per_matrix);
+  if (rc != DLMI_OK) return rc;
+  if (type == DLMI_F32) return muon_batch<float, false>(ctx, b, rows, cols, 1, pl, 0.0f, 0, 0.0f, ns->steps, c, ns->eps);
+  return muon_batch<__bf16, false>(ctx, b, rows, cols, 1, pl, 0.0f, 0, 0.0f, ns->steps, c, ns->eps);
+}
+
+int dlmi_opt_muon(dlmi_ctx *ctx, size_t n, dlmi_muon_problem const *problems, float momentum, int nesterov, float wd,
+                  dlmi_newton_schulz const *ns) try {
+  if (ctx == nullptr) return DLMI_E_INVALID;
+  DLMI_REQUIRE(ctx, n == 0 || problems != nullptr, "null pointer");
+  char const *const wrong = muon_check(ns);
+  DLMI_REQUIRE(ctx, wrong == nullptr, wrong);
+  if (n == 0) return DLMI_OK;
+  DLMI_REQUIRE_DEVICE(ctx);
+  // every array is updated in place, so none may be named twice
+  struct Range {
+    uintptr_t from, to;
+  };
+  std::vector<Range> ranges;
+  for (size_t i = 0; i < n; ++i) {
+    dlmi_muon_problem const &q = problems[i];
+    DLMI_REQUIRE(ctx, q.rows <= DLMI_MUON_MAX_SIDE && q.cols <= DLMI_MUON_MAX_SIDE, "matrix too large");
+    size_t const bytes = q.rows * q.cols * sizeof(float);
+    if (bytes == 0) continue;
+    DLMI_REQUIRE(ctx, q.params != nullptr && q.grads != nullptr && q.momentum != nullptr, "null pointer");
+    for (float const *a : {q.params, q.grads, q.momentum})
+      ranges.push_back({reinterpret_cast<uintptr_t>(a), reinterpret_cast<uintptr_t>(a) + bytes});
+  }
+  std::sort(ranges.begin(), ranges.end(), [](Range const &x, Range const &y) { return x.from < y.from; });
+  for (size_t i = 1; i < ranges.size(); ++i) DLMI_REQUIRE(ctx, ranges[i].from >= ranges[i - 1].to, "two of the arrays overlap");
+  // the launches and the scratch that the largest needs are settled before the first array is touched
+  struct Launch {
+    MuonBatch b;
+    MuonPlan pl;
+    size_t rows, cols;
+    unsigned count;
+  };
+  std::vector<Launch> launches;
+  std::vector<char> done(n, 0);
+  std::vector<size_t> same;
+  size_t scratch = 0;
+  for (size_t i = 0; i < n; ++i) {
+    size_t const rows = problems[i].rows, cols = problems[i].cols;
+    if (done[i] || rows * cols == 0) continue;
+    same.clear();
+    for (size_t k = i; k < n; ++k)
+      if (!done[k] && problems[k].rows == rows && problems[k].cols == cols) {
+        same.push_back(k);
+        done[k] = 1;
+      }
+    for (size_t at = 0; at < same.size();) {
+      size_t const left = same.size() - at;
+      Launch l = {};
+      l.pl = muon_plan(ctx, rows, cols, left < kMuonMax ? left : kMuonMax);
+      l.rows = rows;
+      l.cols = cols;
+      l.count = muon_group(l.pl, left);
+      for (unsigned k = 0; k < l.count; ++k) {
+        dlmi_muon_problem const &q = problems[same[at + k]];
+        l.b.p[k] = q.params;
+        l.b.g[k] = q.grads;
+        l.b.m[k] = q.momentum;
+        l.b.lr[k] = q.lr;
+      }
+      if (l.pl.per_matrix * l.count > scratch) scratch = l.pl.per_matrix * l.count;
+      at += l.count;
+      launches.push_back(l);
+    }
+  }
+  int rc = scratch != 0 ? dlmi_scratch_reserve(ctx, scratch) : DLMI_OK;
+  float const c[3] = {ns->a, ns->b, ns->c};
+  for (size_t i = 0; rc == DLMI_OK && i < launches.size(); ++i) {
+    Launch const &l = launches[i];
+    rc = muon_batch<float, true>(ctx, l.b, l.rows, l.cols, l.count, l.pl, momentum, nesterov, wd, ns->steps, c, ns->eps);
+  }
+  return rc;
+} catch (std::bad_alloc const &) {
+  return dlmi_fail(ctx, DLMI_E_NOMEM, "dlmi_opt_muon: out of host memory");
+}
+
+}  // extern "C"

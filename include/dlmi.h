@@ -60,6 +60,9 @@ typedef enum { DLMI_DROP_NONE = 0, DLMI_DROP_BERNOULLI = 2, DLMI_DROP_BERNOULLI_
  *   with q the pre-dropout activation. */
 typedef enum { DLMI_DROP_BWD_REFERENCE = 0, DLMI_DROP_BWD_MASKED = 1 } dlmi_dropout_bwd;
 
+/* Element type of the tensors of the entry points that take `void *` and a type; everything else is fp32. */
+typedef enum { DLMI_F32 = 0, DLMI_BF16 = 1 } dlmi_dtype;
+
 typedef struct dlmi_ctx dlmi_ctx;
 
 /* ---- context ------------------------------------------------------------- */
@@ -487,6 +490,36 @@ int dlmi_opt_adabound(dlmi_ctx *ctx, size_t n, float *params, float *grads, floa
 int dlmi_opt_irprop_plus(dlmi_ctx *ctx, size_t n, float *params, float *grads, float *prev_grads,
                          float *prev_moves, float *step_sizes, float increase, float decrease,
                          float step_min, float step_max, int loss_got_worse);
+
+/* ---- Muon: the update of a weight matrix, orthogonalized (no counterpart in the reference) ----------------------
+ * The Newton-Schulz iteration that takes the singular values of X = u / (|u|_F + eps) towards 1 and leaves its singular
+ * vectors: `steps` times A = X X^T, X <- a X + (b A + c A A) X, on the shorter side of the matrix.  The usual values are
+ * a, b, c = 3.4445, -4.7750, 2.0315 in 5 steps.  Computed to the precision of fp32 products whatever the type of the
+ * result.  Coefficients that would take a singular value of [0, 1] (or b s^2 + c s^4 of one) beyond 8 are refused.  A
+ * zero matrix gives zero; a non-finite element makes every element of the result non-finite. */
+typedef struct {
+  float a, b, c;
+  int steps;  /* 1 .. 64 */
+  float eps;  /* added to the Frobenius norm, >= 0 (with 0 a zero matrix gives NaN) */
+} dlmi_newton_schulz;
+#define DLMI_MUON_MAX_SIDE 65536
+
+/* O = the iteration applied to G; G, O [rows, cols] device, of `type`; O may alias G. */
+int dlmi_orthogonalize(dlmi_ctx *ctx, dlmi_dtype type, size_t rows, size_t cols, void const *G, void *O,
+                       dlmi_newton_schulz const *ns);
+
+/* One step of several weight matrices: m = momentum*m + g; u = nesterov ? g + momentum*m : m;
+ * p -= lr * orthogonalize(u) + wd*p; the gradient is zeroed.  fp32, updated in place.  Matrices of the same shape
+ * share their launches.  No two of the arrays may overlap.  `problems` is a host array; the pointers in it are device.
+ * The context's scratch grows to about 20 bytes per element of the matrices launched together (at most 2 GiB of it,
+ * more for a single larger matrix). */
+typedef struct {
+  size_t rows, cols;
+  float *params, *grads, *momentum; /* [rows, cols] each */
+  float lr;                         /* this matrix's step size, with whatever factor for its shape the caller uses */
+} dlmi_muon_problem;
+int dlmi_opt_muon(dlmi_ctx *ctx, size_t n, dlmi_muon_problem const *problems, float momentum, int nesterov, float wd,
+                  dlmi_newton_schulz const *ns);
 
 /* ---- Euclidean-norm constraints either side of the optimizer step -----------
  * (euclidean_norm_{st,mp}, v1/ops/constraints/euclidean.cpp:24-62: when the norm
