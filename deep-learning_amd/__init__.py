@@ -31,6 +31,8 @@ ACT = dict(ELU=3, ISRLU=10, LINEAR=11, LEAKY_RELU=14, RELU=16, SELU=17, SOFTMAX=
 NORM = dict(NONE=0, BN=1, BRN=2)
 DROP = dict(NONE=0, BERNOULLI=2, BERNOULLI_INVERTED=3)
 DTYPE = dict(F32=0, BF16=1)
+ROW_NORM = dict(NONE=0, RMS=1, LAYER=2)
+GATE_ACT = dict(LINEAR=11, SIGMOID=18, TANH=23)
 DROP_BWD = dict(REFERENCE=0, MASKED=1)
 STATE = dict(INFERENCE=0, TRAINING=1, UPDATE_BATCH_NORM=2)
 
@@ -47,7 +49,7 @@ C_ABI_SYMBOLS = [
     "dlmi_fc_softmax_fwd", "dlmi_fc_softmax_ce_fwd", "dlmi_fc_bwd_dx_norm_act_bwd",
     "dlmi_ctx_reserve_layer", "dlmi_ctx_scratch_generation", "dlmi_ctx_norm_panel_enabled", "dlmi_ctx_norm_panel_poke",
     "dlmi_fc_bwd_dw_grouped", "dlmi_fused_norm_act_bwd_db", "dlmi_ctx_gemm_clock", "dlmi_ctx_gemm_timeline", "dlmi_probe_strip_stream",
-    "dlmi_orthogonalize", "dlmi_opt_muon",
+    "dlmi_orthogonalize", "dlmi_opt_muon", "dlmi_block_norm_fwd", "dlmi_block_norm_bwd",
 ]
 
 
@@ -56,6 +58,12 @@ class FusedDesc(ctypes.Structure):
     _fields_ = [("norm", c_int), ("act", c_int), ("dropout", c_int), ("mask_per_element", c_int),
                 ("dropout_bwd", c_int), ("momentum", c_f), ("eps", c_f), ("r_max", c_f), ("d_max", c_f),
                 ("drop_scale", c_f)]
+
+
+class BlockNormDesc(ctypes.Structure):
+    """dlmi_block_norm_desc of include/dlmi.h."""
+    _fields_ = [("post", c_int), ("pre", c_int), ("gate_act", c_int), ("gate_rows", ctypes.c_size_t), ("eps_post", c_f),
+                ("eps_pre", c_f), ("residual_scale", c_f), ("branch_scale", c_f)]
 
 
 class MuonProblem(ctypes.Structure):
@@ -569,3 +577,57 @@ class Dlmi:
         self._ck(self.lib.dlmi_fused_norm_act_infer(self.ctx, ctypes.byref(desc), c_sz(B), c_sz(H), _p(x), _p(gamma),
                                                     _p(beta), _p(mov_mean), _p(mov_std), _p(y)))
         return y
+
+    # ------------------------------------------------------------ residual blocks with row norms
+    @staticmethod
+    def block_norm_desc(post=ROW_NORM["RMS"], pre=ROW_NORM["RMS"], gate_act=GATE_ACT["LINEAR"], gate_rows=0, eps_post=1e-5,
+                        eps_pre=1e-5, residual_scale=1.0, branch_scale=1.0):
+        return BlockNormDesc(post, pre, gate_act, gate_rows, eps_post, eps_pre, residual_scale, branch_scale)
+
+    def _chk_block_norm(self, desc, like, rows, gate, params):
+        B, H = like.shape
+        for what, t in rows.items():
+            self._chk_is(t, what, like.dtype, B, H)
+        if gate is not None and desc.gate_rows:
+            self._chk_is(gate, "gate", like.dtype, -(-B // desc.gate_rows), H)
+        for what, t in params.items():
+            self._chk_is(t, what, self.torch.float32, H)
+        return B, H
+
+    def block_norm_fwd(self, desc, x, u, gate=None, w_post=None, b_post=None, w_pre=None, b_pre=None, y=None, h=None):
+        """y = residual_scale x + branch_scale f(gate) post(u), h = pre(y) (dlmi_block_norm_fwd).  Returns (y, h)."""
+        assert u.dim() == 2
+        kind = self._type(u)
+        y = y if y is not None else self._out(u.dtype, *u.shape)
+        h = h if h is not None else self._out(u.dtype, *u.shape)
+        B, H = self._chk_block_norm(desc, u, dict(x=x, u=u, y=y, h=h), gate,
+                                    dict(w_post=w_post, b_post=b_post, w_pre=w_pre, b_pre=b_pre))
+        self._ck(self.lib.dlmi_block_norm_fwd(self.ctx, kind, ctypes.byref(desc), c_sz(B), c_sz(H), _p(x), _p(u), _p(gate),
+                                              _p(w_post), _p(b_post), _p(w_pre), _p(b_pre), _p(y), _p(h)))
+        return y, h
+
+    def block_norm_bwd(self, desc, u, y, dy, dh, gate=None, w_post=None, b_post=None, w_pre=None, b_pre=None, dx=None, du=None,
+                       dgate=None, grads=None, accumulate=False):
+        """Its gradient (dlmi_block_norm_bwd).  Returns dict(dx, du, dgate, dw_post, db_post, dw_pre, db_pre), None for what
+        is not there; grads: a dict of fp32 tensors for the last four (needed to accumulate), made where missing."""
+        assert u.dim() == 2
+        kind = self._type(u)
+        H = u.shape[1]
+        o = dict(dx=dx if dx is not None else self._out(u.dtype, *u.shape),
+                 du=du if du is not None else self._out(u.dtype, *u.shape),
+                 dgate=dgate if dgate is not None or gate is None else self._out(gate.dtype, *gate.shape))
+        for k, p in (("dw_post", w_post), ("db_post", b_post), ("dw_pre", w_pre), ("db_pre", b_pre)):
+            o[k] = (grads or {}).get(k)
+            if o[k] is None and p is not None:
+                assert not accumulate, "accumulating needs the gradients so far"
+                o[k] = self._out(self.torch.float32, H)
+        self._chk_block_norm(desc, u, dict(u=u, y=y, dy=dy, dh=dh, dx=o["dx"], du=o["du"]), gate,
+                             dict(w_post=w_post, b_post=b_post, w_pre=w_pre, b_pre=b_pre, dw_post=o["dw_post"],
+                                  db_post=o["db_post"], dw_pre=o["dw_pre"], db_pre=o["db_pre"]))
+        if o["dgate"] is not None and gate is not None:
+            self._chk_is(o["dgate"], "dgate", gate.dtype, *gate.shape)
+        self._ck(self.lib.dlmi_block_norm_bwd(
+            self.ctx, kind, ctypes.byref(desc), c_sz(u.shape[0]), c_sz(H), _p(u), _p(y), _p(gate), _p(w_post), _p(b_post),
+            _p(w_pre), _p(dy), _p(dh), _p(o["dx"]), _p(o["du"]), _p(o["dgate"]), _p(o["dw_post"]), _p(o["db_post"]),
+            _p(o["dw_pre"]), _p(o["db_pre"]), c_int(1 if accumulate else 0)))
+        return o

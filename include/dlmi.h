@@ -440,6 +440,38 @@ int dlmi_fused_norm_act_infer(dlmi_ctx *ctx, dlmi_fused_desc const *desc, size_t
                               float const *x, float const *gamma, float const *beta,
                               float const *mov_mean, float const *mov_std, float *y);
 
+/* ---- the tail of a residual block with row norms (no counterpart in the reference, whose blocks normalize over the
+ * batch) ----------------------------------------------------------------------------------------------------------
+ *   y = residual_scale * x + branch_scale * f(gate) * post(u),   h = pre(y)
+ * u is the block's output, x the stream it is added to, h what the next block reads.  post and pre: nothing (NONE),
+ * v / sqrt(mean(v^2) + eps) (RMS) or (v - mean(v)) / sqrt(var(v) + eps) (LAYER) over a row, times a weight [H], plus a
+ * bias [H] (each may be NULL).  f: DLMI_ACT_LINEAR, SIGMOID or TANH.  gate [ceil(B / gate_rows), H]: gate_rows
+ * consecutive rows share one of its rows (1: one each, B: one for all); gate_rows == 0 and gate == NULL: no gate.
+ * x, u, gate, y, h [B, H] are of `type`, weights and biases fp32; a row is computed in fp32 and rounded once, h from the
+ * y before rounding.  y may alias x, h may alias u.  H up to DLMI_BLOCK_NORM_MAX_WIDTH (DLMI_E_UNSUPPORTED beyond). */
+typedef enum { DLMI_ROW_NORM_NONE = 0, DLMI_ROW_NORM_RMS = 1, DLMI_ROW_NORM_LAYER = 2 } dlmi_row_norm;
+#define DLMI_BLOCK_NORM_MAX_WIDTH 16384
+typedef struct {
+  dlmi_row_norm post, pre;
+  dlmi_activation gate_act;
+  size_t gate_rows;
+  float eps_post, eps_pre;
+  float residual_scale, branch_scale;
+} dlmi_block_norm_desc;
+int dlmi_block_norm_fwd(dlmi_ctx *ctx, dlmi_dtype type, dlmi_block_norm_desc const *desc, size_t B, size_t H, void const *x,
+                        void const *u, void const *gate, float const *w_post, float const *b_post, float const *w_pre,
+                        float const *b_pre, void *y, void *h);
+
+/* Its gradient: dy and dh (either may be NULL: zero) are those of y and h; u, y, gate and the weights are the forward's
+ * (the statistics are formed again from u and y; y may be NULL where dh is or pre is NONE).  dx, du [B, H] and dgate
+ * [ceil(B / gate_rows), H] (may be NULL) are written; the weights' and biases' gradients (fp32 [H], each may be NULL) are
+ * added to where accumulate != 0, written otherwise.  All sums over rows are taken in an order that depends on the sizes
+ * only.  dx may alias dy, du may alias dh. */
+int dlmi_block_norm_bwd(dlmi_ctx *ctx, dlmi_dtype type, dlmi_block_norm_desc const *desc, size_t B, size_t H, void const *u,
+                        void const *y, void const *gate, float const *w_post, float const *b_post, float const *w_pre,
+                        void const *dy, void const *dh, void *dx, void *du, void *dgate, float *dw_post, float *db_post,
+                        float *dw_pre, float *db_pre, int accumulate);
+
 /* ---- optimizer steps over n packed parameters (the caller-side neighbour of
  * the path: Model::Update_Parameter, v1/learner/model.cpp:4703-4866) ----------
  * All arrays are device memory of n floats and are updated in place; every
