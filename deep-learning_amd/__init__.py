@@ -50,6 +50,7 @@ C_ABI_SYMBOLS = [
     "dlmi_ctx_reserve_layer", "dlmi_ctx_scratch_generation", "dlmi_ctx_norm_panel_enabled", "dlmi_ctx_norm_panel_poke",
     "dlmi_fc_bwd_dw_grouped", "dlmi_fused_norm_act_bwd_db", "dlmi_ctx_gemm_clock", "dlmi_ctx_gemm_timeline", "dlmi_probe_strip_stream",
     "dlmi_orthogonalize", "dlmi_opt_muon", "dlmi_block_norm_fwd", "dlmi_block_norm_bwd",
+    "dlmi_vocab_ce_fwd", "dlmi_vocab_ce_bwd",
 ]
 
 
@@ -577,6 +578,47 @@ class Dlmi:
         self._ck(self.lib.dlmi_fused_norm_act_infer(self.ctx, ctypes.byref(desc), c_sz(B), c_sz(H), _p(x), _p(gamma),
                                                     _p(beta), _p(mov_mean), _p(mov_std), _p(y)))
         return y
+
+    # ------------------------------------------------------------ cross entropy over a large vocabulary
+    def _chk_vocab_ce(self, X, W, labels, bias, rows):
+        assert X.dim() == 2 and W.dim() == 2
+        (B, K), V = X.shape, W.shape[0]
+        self._chk_is(X, "X", X.dtype, B, K)
+        self._chk_is(W, "W", X.dtype, V, K)
+        self._chk_is(labels, "labels", self.torch.int32, B)
+        self._chk_is(bias, "bias", self.torch.float32, V)
+        for what, t in rows.items():
+            self._chk_is(t, what, self.torch.float32, B)
+        return B, K, V
+
+    def vocab_ce_fwd(self, X, W, labels, bias=None, loss=None, lse=None):
+        """Cross entropy of softmax(X W^T + bias) at int32 labels, the logits not kept (dlmi_vocab_ce_fwd); a label outside
+        [0, V) leaves its row out.  Returns (loss, lse), float32 [B]."""
+        kind = self._type(X)
+        loss = loss if loss is not None else self._out(self.torch.float32, X.shape[0])
+        lse = lse if lse is not None else self._out(self.torch.float32, X.shape[0])
+        B, K, V = self._chk_vocab_ce(X, W, labels, bias, dict(loss=loss, lse=lse))
+        self._ck(self.lib.dlmi_vocab_ce_fwd(self.ctx, kind, c_sz(B), c_sz(K), c_sz(V), _p(X), _p(W), _p(bias), _p(labels),
+                                            _p(loss), _p(lse)))
+        return loss, lse
+
+    def vocab_ce_bwd(self, X, W, labels, lse, bias=None, dloss=None, scale=1.0, dX=None, dW=None, db=None, accumulate=False):
+        """Its gradient (dlmi_vocab_ce_bwd), times scale * dloss per row.  Returns (dX, dW, db), made where missing (db only
+        with a bias); accumulate adds into dW and db."""
+        kind = self._type(X)
+        B, K, V = self._chk_vocab_ce(X, W, labels, bias, dict(lse=lse, dloss=dloss))
+        assert not accumulate or (dW is not None and (db is not None or bias is None)), "accumulating needs the gradients so far"
+        dX = dX if dX is not None else self._out(X.dtype, B, K)
+        dW = dW if dW is not None else self._out(X.dtype, V, K)
+        if db is None and bias is not None:
+            db = self._out(self.torch.float32, V)
+        self._chk_is(dX, "dX", X.dtype, B, K)
+        self._chk_is(dW, "dW", X.dtype, V, K)
+        self._chk_is(db, "db", self.torch.float32, V)
+        self._ck(self.lib.dlmi_vocab_ce_bwd(self.ctx, kind, c_sz(B), c_sz(K), c_sz(V), _p(X), _p(W), _p(bias), _p(labels),
+                                            _p(lse), _p(dloss), c_f(scale), _p(dX), _p(dW), _p(db),
+                                            c_int(1 if accumulate else 0)))
+        return dX, dW, db
 
     # ------------------------------------------------------------ residual blocks with row norms
     @staticmethod

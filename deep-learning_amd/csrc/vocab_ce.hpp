@@ -1,0 +1,672 @@
+// Softmax cross entropy of a fully connected output layer over a large vocabulary, and its gradient, for gfx950, without
+// keeping the logits:
+//
+//   z = X W^T + bias,  lse_b = log sum_v exp z_bv,  loss_b = lse_b - z_b,label
+//   dL_bv = exp(z_bv - lse_b) - [v = label_b],  dX = g dL W,  dW = (g dL)^T X,  db = sum_b g_b dL_b,   g_b = scale dloss_b
+//
+// The vocabulary is walked in pieces.  Forward: one product per piece whose epilogue reduces each 128 (T / 2) classes of a
+// row to a maximum and a sum of exponentials; nothing of size [B, V] is written.  Backward: per piece the logits again
+// (a third of the work, against B V values kept and read), dL rounded to f16 planes, the two products that read it.
+// Bound by the 16-bit matrix pipe: 2 B K V operations forward, 6 B K V backward, times three for the two planes of an fp32
+// input (half_gemm.hpp); by reading W where there are few rows.
+//
+// Operands are packed as f16 planes of powers-of-two multiples: a row of X by its own largest magnitude (a padding row
+// full of garbage spoils nobody's scale), a piece of W by its own.  bf16 values have 8 bits and one plane holds them
+// exactly; fp32 values take two planes.  dL is in [-1, 1] and held times 2^15, rounded to 11 bits (bf16; the result keeps 8)
+// or 22 (fp32).  For dW, whose sum runs over the rows, X is packed times dloss (one more rounding for bf16, none without
+// dloss), rows left out as zeros; the common factor comes last.
+#pragma once
+
+#include "half_gemm.hpp"
+
+namespace dlmi {
+
+struct CeArgs {
+  size_t B, K, V;
+  void const *X, *W;
+  float const *bias;
+  int const *labels;
+  float *loss, *lse;
+  // backward
+  float const *lse_in, *dloss;
+  float scale;
+  void *dX, *dW;
+  float *db;
+  int accumulate;
+};
+
+template <class T>
+int ce_forward(dlmi_ctx *ctx, CeArgs const &a);
+template <class T>
+int ce_backward(dlmi_ctx *ctx, CeArgs const &a);
+
+#ifdef DLMI_CE_IMPLEMENTATION
+
+constexpr int kCeBlock = 256;
+constexpr unsigned kCeMaxParts = 256;     // partial maxima of a piece of W
+constexpr float kCeDl = 32768.0f;         // dL is held times this
+
+template <class T>
+struct __attribute__((packed, aligned(sizeof(T)))) CeOct {
+  T v[8];
+};
+
+// 2^e with the largest magnitude m times it in [2^14, 2^15); 1 for m = 0, at most 2^126.
+__device__ __forceinline__ float ce_scale(float m) {
+  if (!(m > 0.0f)) return 1.0f;
+  int e = 14 - (static_cast<int>(__float_as_uint(m) >> 23) - 127);
+  e = e > 126 ? 126 : e;
+  return __uint_as_float(static_cast<unsigned>(e + 127) << 23);
+}
+// Its inverse: a power of two of at least 2^-126.
+__device__ __forceinline__ float ce_unscale(float s) { return __uint_as_float((254u << 23) - __float_as_uint(s)); }
+
+__device__ __forceinline__ float ce_finite_max(float m, float x) {
+  x = fabsf(x);
+  return x <= 3.402823466e+38f && x > m ? x : m;  // infinities and NaN set no scale
+}
+
+__device__ __forceinline__ float ce_wave_max(float m) {
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  return m;
+}
+
+// What a row counts in the gradient, but for the common factor `scale`.
+__device__ __forceinline__ float ce_row_weight(CeArgs const &a, size_t b) {
+  int const l = a.labels[b];
+  if (l < 0 || static_cast<size_t>(l) >= a.V) return 0.0f;
+  return a.dloss != nullptr ? a.dloss[b] : 1.0f;
+}
+
+// A wavefront per row: rowmax[row] (may be null) and the largest of all rows per block in parts (may be null); `weighted`:
+// of dloss x instead of x, rows left out not looked at.
+template <class T>
+__global__ __launch_bounds__(kCeBlock) void k_ce_max(CeArgs a, T const *src, size_t rows, size_t cols, float *rowmax, float *parts,
+                                                     int weighted) {
+  __shared__ float lds[kCeBlock / 64];
+  int const lane = threadIdx.x & 63;
+  float all = 0.0f;
+  for (size_t r = static_cast<size_t>(blockIdx.x) * (kCeBlock / 64) + (threadIdx.x >> 6); r < rows;
+       r += static_cast<size_t>(gridDim.x) * (kCeBlock / 64)) {
+    float const g = weighted ? ce_row_weight(a, r) : 1.0f;
+    float m = 0.0f;
+    if (g != 0.0f) {
+      T const *const row = src + r * cols;
+      size_t c = static_cast<size_t>(lane) * 8;
+      for (; c + 8 <= cols; c += 512) {
+        CeOct<T> const o = *reinterpret_cast<CeOct<T> const *>(row + c);
+#pragma unroll
+        for (int t = 0; t < 8; ++t) m = ce_finite_max(m, static_cast<float>(o.v[t]) * g);
+      }
+      for (; c < cols; ++c) m = ce_finite_max(m, static_cast<float>(row[c]) * g);
+    }
+    m = ce_wave_max(m);
+    if (rowmax != nullptr && lane == 0) rowmax[r] = m;
+    all = fmaxf(all, m);
+  }
+  if (parts == nullptr) return;
+  if (lane == 0) lds[threadIdx.x >> 6] = all;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < kCeBlock / 64; ++w) all = fmaxf(all, lds[w]);
+    parts[blockIdx.x] = all;
+  }
+}
+
+// A 64 x 64 tile of src [rows, cols], scaled and packed as it stands (`as`: row r, k = c) and / or transposed (`across`: row
+// c, k = r), padding zero.  The scale: of the row (rowmax) or of the largest of parts[nparts]; its inverse goes to
+// unscale (one value per row, or one).  weighted: times dloss of the row, rows left out zero.
+template <class T, int NP>
+__global__ __launch_bounds__(kCeBlock) void k_ce_pack(CeArgs a, T const *src, size_t rows, size_t cols, unsigned kblocks_as,
+                                                      unsigned kblocks_across, float const *rowmax, float const *parts, unsigned nparts,
+                                                      float *unscale, int weighted, char *as, char *across) {
+  __shared__ float tile[64][65];
+  __shared__ float lds[kCeBlock / 64];
+  int const lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  float scale = 1.0f;
+  if (parts != nullptr) {
+    float m = threadIdx.x < nparts ? parts[threadIdx.x] : 0.0f;
+    m = ce_wave_max(m);
+    if (lane == 0) lds[wave] = m;
+    __syncthreads();
+    scale = ce_scale(fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3])));
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) unscale[0] = ce_unscale(scale);
+  }
+  size_t const r0 = static_cast<size_t>(blockIdx.y) * 64, c0 = static_cast<size_t>(blockIdx.x) * 64;
+  // a thread takes 8 columns of two rows
+  int const tc = (threadIdx.x & 7) * 8;
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    int const tr = q * 32 + (threadIdx.x >> 3);
+    size_t const r = r0 + tr, c = c0 + tc;
+    float x[8];
+#pragma unroll
+    for (int t = 0; t < 8; ++t) x[t] = 0.0f;
+    float s = scale, g = 1.0f;
+    if (r < rows) {
+      if (rowmax != nullptr) {
+        s = ce_scale(rowmax[r]);
+        if (blockIdx.x == 0 && tc == 0) unscale[r] = ce_unscale(s);
+      }
+      bool live = true;
+      if (weighted) {
+        int const l = a.labels[r];
+        live = l >= 0 && static_cast<size_t>(l) < a.V;
+        g = ce_row_weight(a, r);
+      }
+      if (live) {
+        T const *const p = src + r * cols + c;
+        if (c + 8 <= cols) {
+          CeOct<T> const o = *reinterpret_cast<CeOct<T> const *>(p);
+#pragma unroll
+          for (int t = 0; t < 8; ++t) x[t] = static_cast<float>(o.v[t]) * g * s;
+        } else {
+#pragma unroll
+          for (int t = 0; t < 8; ++t)
+            if (c + t < cols) x[t] = static_cast<float>(p[t]) * g * s;
+        }
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < 8; ++t) tile[tr][tc + t] = x[t];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    int const f = q * 4 + wave;  // 16 fragments: 8 as it stands, 8 transposed
+    bool const flip = f >= 8;
+    if (flip ? across == nullptr : as == nullptr) continue;
+    int const rb = (f >> 2) & 1, kb = f & 3;
+    half8 hi, lo;
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+      int const row = rb * 32 + (lane & 31), k = kb * 16 + (lane >> 5) * 8 + t;
+      float const x = flip ? tile[k][row] : tile[row][k];
+      _Float16 const h = static_cast<_Float16>(x);
+      hi[t] = h;
+      if constexpr (NP == 2) lo[t] = static_cast<_Float16>(x - static_cast<float>(h));
+    }
+    size_t const frag = flip ? (c0 / 32 + rb) * kblocks_across + r0 / 16 + kb : (r0 / 32 + rb) * kblocks_as + c0 / 16 + kb;
+    char *const dst = (flip ? across : as) + frag * NP * kFragBytes + lane * 16;
+    *reinterpret_cast<half8 *>(dst) = hi;
+    if constexpr (NP == 2) *reinterpret_cast<half8 *>(dst + kFragBytes) = lo;
+  }
+}
+
+// Tile number -> (ti, tj) in bands of 8 ti: the tiles that run together on an XCD share operand rows.
+__device__ __forceinline__ void ce_tile(unsigned id, unsigned ni, unsigned nj, unsigned &ti, unsigned &tj) {
+  unsigned const band = id / (8 * nj), left = ni - band * 8, w = left < 8 ? left : 8, r = id - band * 8 * nj;
+  tj = r / w;
+  ti = band * 8 + r - tj * w;
+}
+
+// What a sum of exponentials around m counts in one around `most` >= m.  Nothing has been summed around -infinity (or NaN,
+// which times zero stays NaN).
+__device__ __forceinline__ float ce_join_factor(float m, float most) { return m > -INFINITY ? __expf(m - most) : 0.0f; }
+
+// The logits of a tile: classes i of the piece (P = W packed), rows j of the batch (Q = X packed).
+struct CeLogits {
+  char const *P, *Q;
+  float const *unscale_x, *unscale_w;
+  unsigned ni, nj, kblocks, stages;  // kblocks: of a row block in memory
+  size_t v0, vn;                     // first class of the piece, classes in it
+};
+
+// z of one 32 x 32 block; classes beyond the piece are -infinity.
+template <int T>
+__device__ __forceinline__ f32x16 ce_block_logits(CeArgs const &a, CeLogits const &g, f32x16 v, size_t c0, float ux, float uw, int lane) {
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    size_t const c = c0 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+    float z = v[r] * ux * uw;
+    if (c < g.vn) {
+      if (a.bias != nullptr) z += a.bias[g.v0 + c];
+    } else {
+      z = -INFINITY;
+    }
+    v[r] = z;
+  }
+  return v;
+}
+
+// part[half tile of classes][Bp] = (max, sum of exp(z - max)); target[b] = the label's logit.
+template <int T, int NP>
+__global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_stats(CeArgs a, CeLogits g, float2 *part, size_t part_stride, size_t part_row0,
+                                                                   float *target) {
+  using H = HalfTile<T, T, NP>;
+  unsigned ti, tj;
+  ce_tile(xcd_consecutive(blockIdx.x, gridDim.x), g.ni, g.nj, ti, tj);
+  size_t const rs = static_cast<size_t>(g.kblocks) * NP * kFragBytes;
+  HalfAcc<H> acc;
+  half_gemm<T, T, NP>(acc, g.P + ti * (T / 32) * rs, g.Q + tj * (T / 32) * rs, rs, rs, g.stages);
+  int const lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  float const uw = g.unscale_w[0];
+  size_t const c0 = static_cast<size_t>(ti) * T + (wave >> 1) * (T / 2);
+#pragma unroll
+  for (int n = 0; n < H::kNB; ++n) {
+    size_t const b = static_cast<size_t>(tj) * T + (wave & 1) * (T / 2) + n * 32 + (lane & 31);
+    bool const in = b < a.B;
+    float const ux = in ? g.unscale_x[b] : 0.0f;
+    float top = -INFINITY;
+#pragma unroll
+    for (int m = 0; m < H::kMB; ++m) {
+      acc.v[m][n] = ce_block_logits<T>(a, g, acc.v[m][n], c0 + m * 32, ux, uw, lane);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, acc.v[m][n][r]);
+    }
+    float sum = 0.0f;
+    float const base = top > -INFINITY ? top : 0.0f;
+#pragma unroll
+    for (int m = 0; m < H::kMB; ++m)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sum += __expf(acc.v[m][n][r] - base);
+    // the label's class, where it lies in this wavefront's rows
+    long long const at = in ? static_cast<long long>(a.labels[b]) - static_cast<long long>(g.v0 + c0) : -1;
+    if (__any(at >= 0 && at < T / 2)) {
+#pragma unroll
+      for (int m = 0; m < H::kMB; ++m)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (at == m * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3) && static_cast<size_t>(at) + c0 < g.vn) target[b] = acc.v[m][n][r];
+    }
+    float const top2 = __shfl_xor(top, 32), sum2 = __shfl_xor(sum, 32);
+    float const most = fmaxf(top, top2);
+    sum = sum * ce_join_factor(top, most) + sum2 * ce_join_factor(top2, most);
+    if (lane < 32 && in) part[(part_row0 + ti * 2 + (wave >> 1)) * part_stride + b] = make_float2(most, sum);
+  }
+}
+
+// 64 rows of the batch per workgroup: 16 threads each join every 16th partial, then one another's, in a fixed order.
+template <int kParts>
+__global__ __launch_bounds__(64 * kParts) void k_ce_join(CeArgs a, float2 const *part, size_t part_stride, size_t parts, float const *target) {
+  __shared__ float2 lds[kParts][64];
+  size_t const b = static_cast<size_t>(blockIdx.x) * 64 + (threadIdx.x & 63);
+  int const w = threadIdx.x >> 6;
+  float m = -INFINITY, s = 0.0f;
+  auto const join = [&](float2 p) {
+    float const most = fmaxf(m, p.x);
+    s = s * ce_join_factor(m, most) + p.y * ce_join_factor(p.x, most);
+    m = most;
+  };
+  if (b < a.B)
+    for (size_t p = w; p < parts; p += kParts) join(part[p * part_stride + b]);
+  lds[w][threadIdx.x & 63] = make_float2(m, s);
+  __syncthreads();
+  if (w != 0 || b >= a.B) return;
+  for (int o = 1; o < kParts; ++o) join(lds[o][threadIdx.x & 63]);
+  float const lse = m + logf(s);
+  a.lse[b] = lse;
+  int const l = a.labels[b];
+  a.loss[b] = l >= 0 && static_cast<size_t>(l) < a.V ? lse - target[b] : 0.0f;
+}
+
+// dL of a tile, packed for dX (rows of the batch, k = classes) and for dW (rows are classes, k = rows of the batch);
+// DB: also the sums of dloss dL over each half tile of rows.
+template <int T, int NP, bool DB>
+__global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_grad(CeArgs a, CeLogits g, char *dlb, char *dlv, unsigned kblocks_v,
+                                                                  unsigned kblocks_b, float *dbpart, size_t dbpart_stride) {
+  using H = HalfTile<T, T, NP>;
+  unsigned ti, tj;
+  ce_tile(xcd_consecutive(blockIdx.x, gridDim.x), g.ni, g.nj, ti, tj);
+  size_t const rs = static_cast<size_t>(g.kblocks) * NP * kFragBytes;
+  HalfAcc<H> acc;
+  half_gemm<T, T, NP>(acc, g.P + ti * (T / 32) * rs, g.Q + tj * (T / 32) * rs, rs, rs, g.stages);
+  int const lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  half8 const id0 = half_identity(0, lane), id1 = half_identity(1, lane);
+  float const uw = g.unscale_w[0];
+  size_t const c0 = static_cast<size_t>(ti) * T + (wave >> 1) * (T / 2);
+  size_t const b0 = static_cast<size_t>(tj) * T + (wave & 1) * (T / 2);
+  size_t const rb = static_cast<size_t>(kblocks_v) * NP * kFragBytes, rv = static_cast<size_t>(kblocks_b) * NP * kFragBytes;
+  float dsum[H::kMB];
+#pragma unroll
+  for (int m = 0; m < H::kMB; ++m) dsum[m] = 0.0f;
+#pragma unroll
+  for (int n = 0; n < H::kNB; ++n) {
+    size_t const b = b0 + n * 32 + (lane & 31);
+    bool const in = b < a.B;
+    float const ux = in ? g.unscale_x[b] : 0.0f;
+    int const label = in ? a.labels[b] : -1;
+    bool const live = label >= 0 && static_cast<size_t>(label) < a.V;
+    float const lse = live ? a.lse_in[b] : 0.0f;
+    long long const at = static_cast<long long>(label) - static_cast<long long>(g.v0 + c0);
+#pragma unroll
+    for (int m = 0; m < H::kMB; ++m) {
+      f32x16 z = ce_block_logits<T>(a, g, acc.v[m][n], c0 + m * 32, ux, uw, lane);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        float p = __expf(z[r] - lse);
+        if (at == m * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3)) p -= 1.0f;
+        // (a class beyond the piece: z is -infinity, but a row's lse may be too)
+        z[r] = live && c0 + m * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3) < g.vn ? p * kCeDl : 0.0f;
+      }
+      size_t const ib = c0 / 32 + m, jb = b0 / 32 + n;
+      HalfBlock<NP> const blk = half_split<NP>(z);
+      half_store<NP>(dlb + jb * rb + ib * 2 * NP * kFragBytes, blk, lane);
+      HalfBlock<NP> const flip = half_flip<NP>(blk, id0, id1);
+      half_store<NP>(dlv + ib * rv + jb * 2 * NP * kFragBytes, flip, lane);
+      if constexpr (DB) {
+        // the transposed block in fp32 (22 bits): a lane has a class, 16 rows of the batch
+        HalfBlock<2> const two = half_split<2>(z);
+        f32x16 const t = half_transposed(two.pl[0], id0, id1) + half_transposed(two.pl[1], id0, id1);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          size_t const bb = b0 + n * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+          float const w = bb < a.B ? ce_row_weight(a, bb) : 0.0f;
+          dsum[m] += bb < a.B ? w * t[r] : 0.0f;
+        }
+      }
+    }
+  }
+  if constexpr (DB) {
+#pragma unroll
+    for (int m = 0; m < H::kMB; ++m) {
+      float const s = dsum[m] + __shfl_xor(dsum[m], 32);
+      if (lane < 32) dbpart[(tj * 2 + (wave & 1)) * dbpart_stride + c0 + m * 32 + lane] = s * (1.0f / kCeDl);
+    }
+  }
+}
+
+static __global__ __launch_bounds__(kCeBlock) void k_ce_db(float const *part, size_t stride, unsigned parts, size_t n, float *db, float scale, int accumulate) {
+  size_t const c = static_cast<size_t>(blockIdx.x) * kCeBlock + threadIdx.x;
+  if (c >= n) return;
+  float s = 0.0f;
+  for (unsigned p = 0; p < parts; ++p) s += part[p * stride + c];
+  s *= scale;
+  db[c] = accumulate ? db[c] + s : s;
+}
+
+// dW of a piece: classes i (P = dL packed by classes), features j (Q = dloss X packed by features), times `scale`.
+template <int T, int NP, class O>
+__global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_dw(char const *P, char const *Q, unsigned ni, unsigned nj, unsigned kblocks,
+                                                                unsigned stages, float const *unscale, float scale, O *out, size_t rows,
+                                                                size_t cols, int accumulate) {
+  using H = HalfTile<T, T, NP>;
+  unsigned ti, tj;
+  ce_tile(xcd_consecutive(blockIdx.x, gridDim.x), ni, nj, ti, tj);
+  size_t const rs = static_cast<size_t>(kblocks) * NP * kFragBytes;
+  HalfAcc<H> acc;
+  half_gemm<T, T, NP>(acc, P + ti * (T / 32) * rs, Q + tj * (T / 32) * rs, rs, rs, stages);
+  int const lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  float const us = unscale[0];
+#pragma unroll
+  for (int m = 0; m < H::kMB; ++m)
+#pragma unroll
+    for (int n = 0; n < H::kNB; ++n) {
+      size_t const j = static_cast<size_t>(tj) * T + (wave & 1) * (T / 2) + n * 32 + (lane & 31);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        size_t const i = static_cast<size_t>(ti) * T + (wave >> 1) * (T / 2) + m * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+        if (i < rows && j < cols) {
+          O *const p = out + i * cols + j;
+          float v = acc.v[m][n][r] * (1.0f / kCeDl) * us * scale;
+          if (accumulate) v += static_cast<float>(*p);
+          *p = static_cast<O>(v);
+        }
+      }
+    }
+}
+
+// A slice of a piece's share of dX: rows of the batch i (P = dL packed by rows), features j (Q = W packed by features), summed
+// over the piece's classes of the slice into out [slice][rows][cols]; the first piece writes, later ones add.
+template <int T, int NP>
+__global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_dx(char const *P, char const *Q, unsigned ni, unsigned nj, unsigned kblocks,
+                                                                unsigned stages, unsigned per_slice, float const *unscale, float *out,
+                                                                size_t rows, size_t cols, int first) {
+  using H = HalfTile<T, T, NP>;
+  unsigned ti, tj;
+  unsigned const id = xcd_consecutive(blockIdx.x, gridDim.x), slice = id / (ni * nj);
+  ce_tile(id - slice * ni * nj, ni, nj, ti, tj);
+  unsigned const s0 = slice * per_slice;
+  if (s0 >= stages) return;  // a shorter last piece (the first has work for every slice)
+  unsigned const count = stages - s0 < per_slice ? stages - s0 : per_slice;
+  size_t const rs = static_cast<size_t>(kblocks) * NP * kFragBytes, skip = static_cast<size_t>(s0) * 2 * kFragBytes;
+  HalfAcc<H> acc;
+  half_gemm<T, T, NP>(acc, P + ti * (T / 32) * rs + skip, Q + tj * (T / 32) * rs + skip, rs, rs, count);
+  int const lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  float const us = unscale[0];
+  out += slice * rows * cols;
+#pragma unroll
+  for (int m = 0; m < H::kMB; ++m)
+#pragma unroll
+    for (int n = 0; n < H::kNB; ++n) {
+      size_t const j = static_cast<size_t>(tj) * T + (wave & 1) * (T / 2) + n * 32 + (lane & 31);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        size_t const i = static_cast<size_t>(ti) * T + (wave >> 1) * (T / 2) + m * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+        if (i < rows && j < cols) {
+          float const v = acc.v[m][n][r] * (1.0f / kCeDl) * us;
+          float *const p = out + i * cols + j;
+          *p = first ? v : *p + v;
+        }
+      }
+    }
+}
+
+// dX = scale dloss sum over slices, rows left out zero.
+template <class O>
+__global__ __launch_bounds__(kCeBlock) void k_ce_dx_finish(CeArgs a, float const *acc, unsigned slices, O *dX) {
+  size_t const n = a.B * a.K;
+  for (size_t i = static_cast<size_t>(blockIdx.x) * kCeBlock + threadIdx.x; i < n; i += static_cast<size_t>(gridDim.x) * kCeBlock) {
+    size_t const b = i / a.K;
+    int const l = a.labels[b];
+    float s = 0.0f;
+    if (l >= 0 && static_cast<size_t>(l) < a.V) {
+      for (unsigned q = 0; q < slices; ++q) s += acc[q * n + i];
+      s *= ce_row_weight(a, b) * a.scale;
+    }
+    dX[i] = static_cast<O>(s);
+  }
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------
+struct CePlan {
+  int T;
+  size_t Bp, Kp, Vc, pieces;       // padded rows and features; classes of a piece (a multiple of T)
+  unsigned slices, per_slice;      // of dX
+  size_t row_blocks, wparts;
+  // offsets in the scratch
+  size_t xp, xg, wp, wt, dlb, dlv, rowmax, parts, unscale, part, target, dxacc, dbpart, bytes;
+};
+
+template <int NP>
+CePlan ce_plan(dlmi_ctx const *ctx, size_t B, size_t K, size_t V, bool back) {
+  CePlan p = {};
+  p.T = B > 512 ? 256 : (B > 64 ? 128 : 64);
+  size_t const T = p.T;
+  auto const up = [](size_t x, size_t m) { return dlmi_ceil_div(x, m) * m; };
+  p.Bp = up(B, T);
+  p.Kp = back ? up(K, T) : up(K, 64);
+  // a piece: about four rounds of tiles, at most 1 GiB of packed operands
+  size_t const nj = p.Bp / T;
+  size_t tiles = dlmi_ceil_div(static_cast<size_t>(ctx->num_cu) * 4, nj);
+  size_t const row_bytes = 2 * NP * (back ? 2 * (p.Kp + p.Bp) : p.Kp);
+  size_t const fit = (size_t(1) << 30) / (row_bytes * T);
+  if (tiles > fit) tiles = fit > 0 ? fit : 1;
+  size_t const all = dlmi_ceil_div(V, T);
+  p.pieces = dlmi_ceil_div(all, tiles);
+  p.Vc = dlmi_ceil_div(all, p.pieces) * T;
+  p.pieces = dlmi_ceil_div(V, p.Vc);
+  size_t at = 0;
+  auto const take = [&](size_t bytes) {
+    size_t const o = at;
+    at += up(bytes, 1024);
+    return o;
+  };
+  p.xp = take(packed_bytes(p.Bp, p.Kp, NP));
+  p.wp = take(packed_bytes(p.Vc, p.Kp, NP));
+  p.rowmax = take(B * sizeof(float));
+  p.parts = take(2 * kCeMaxParts * sizeof(float));
+  p.unscale = take((B + 2) * sizeof(float));
+  if (!back) {
+    p.part = take(dlmi_ceil_div(V, T) * 2 * p.Bp * sizeof(float2));
+    p.target = take(B * sizeof(float));
+  } else {
+    p.xg = take(packed_bytes(p.Kp, p.Bp, NP));
+    p.wt = take(packed_bytes(p.Kp, p.Vc, NP));
+    p.dlb = take(packed_bytes(p.Bp, p.Vc, NP));
+    p.dlv = take(packed_bytes(p.Vc, p.Bp, NP));
+    size_t const dxt = p.Bp / T * (p.Kp / T), stages = p.Vc / 16 * NP / 2;
+    size_t s = static_cast<size_t>(ctx->num_cu) * (T >= 256 ? 1 : 2) / dxt;
+    if (s < 1) s = 1;
+    if (s > 16) s = 16;
+    if (s > stages / 16) s = stages / 16 > 0 ? stages / 16 : 1;
+    p.per_slice = static_cast<unsigned>(dlmi_ceil_div(stages, s));
+    p.slices = static_cast<unsigned>(dlmi_ceil_div(stages, p.per_slice));
+    p.dxacc = take(p.slices * B * K * sizeof(float));
+    p.dbpart = take(p.Bp / T * 2 * p.Vc * sizeof(float));
+  }
+  p.bytes = at;
+  return p;
+}
+
+template <class E, int NP>
+struct CeRun {
+  dlmi_ctx *ctx;
+  CeArgs a;
+  CePlan p;
+  char *s;
+
+  float *floats(size_t at) const { return reinterpret_cast<float *>(s + at); }
+
+  int pack_rows() const {
+    unsigned const blocks = static_cast<unsigned>(dlmi_ceil_div(a.B, 4) < kCeMaxParts ? dlmi_ceil_div(a.B, 4) : kCeMaxParts);
+    E const *const x = static_cast<E const *>(a.X);
+    hipLaunchKernelGGL(k_ce_max<E>, dim3(blocks), dim3(kCeBlock), 0, ctx->stream, a, x, a.B, a.K, floats(p.rowmax), nullptr, 0);
+    DLMI_LAUNCH_CHECK(ctx, "k_ce_max");
+    dim3 const grid(static_cast<unsigned>(p.Kp / 64), static_cast<unsigned>(p.Bp / 64));
+    hipLaunchKernelGGL((k_ce_pack<E, NP>), grid, dim3(kCeBlock), 0, ctx->stream, a, x, a.B, a.K, static_cast<unsigned>(p.Kp / 16), 0u,
+                       floats(p.rowmax), nullptr, 0u, floats(p.unscale) + 2, 0, s + p.xp, nullptr);
+    DLMI_LAUNCH_CHECK(ctx, "k_ce_pack");
+    return DLMI_OK;
+  }
+  int pack_rows_weighted() const {
+    unsigned const blocks = static_cast<unsigned>(dlmi_ceil_div(a.B, 4) < kCeMaxParts ? dlmi_ceil_div(a.B, 4) : kCeMaxParts);
+    E const *const x = static_cast<E const *>(a.X);
+    float *const parts = floats(p.parts) + kCeMaxParts;
+    hipLaunchKernelGGL(k_ce_max<E>, dim3(blocks), dim3(kCeBlock), 0, ctx->stream, a, x, a.B, a.K, nullptr, parts, 1);
+    DLMI_LAUNCH_CHECK(ctx, "k_ce_max");
+    dim3 const grid(static_cast<unsigned>(p.Kp / 64), static_cast<unsigned>(p.Bp / 64));
+    hipLaunchKernelGGL((k_ce_pack<E, NP>), grid, dim3(kCeBlock), 0, ctx->stream, a, x, a.B, a.K, 0u, static_cast<unsigned>(p.Bp / 16), nullptr,
+                       parts, blocks, floats(p.unscale) + 1, 1, nullptr, s + p.xg);
+    DLMI_LAUNCH_CHECK(ctx, "k_ce_pack");
+    return DLMI_OK;
+  }
+  int pack_classes(size_t v0, size_t vn, size_t vp, bool back) const {
+    unsigned const blocks = static_cast<unsigned>(dlmi_ceil_div(vn, 4) < kCeMaxParts ? dlmi_ceil_div(vn, 4) : kCeMaxParts);
+    E const *const w = static_cast<E const *>(a.W) + v0 * a.K;
+    hipLaunchKernelGGL(k_ce_max<E>, dim3(blocks), dim3(kCeBlock), 0, ctx->stream, a, w, vn, a.K, nullptr, floats(p.parts), 0);
+    DLMI_LAUNCH_CHECK(ctx, "k_ce_max");
+    dim3 const grid(static_cast<unsigned>(p.Kp / 64), static_cast<unsigned>(vp / 64));
+    hipLaunchKernelGGL((k_ce_pack<E, NP>), grid, dim3(kCeBlock), 0, ctx->stream, a, w, vn, a.K, static_cast<unsigned>(p.Kp / 16),
+                       static_cast<unsigned>(vp / 16), nullptr, floats(p.parts), blocks, floats(p.unscale), 0, s + p.wp,
+                       back ? s + p.wt : nullptr);
+    DLMI_LAUNCH_CHECK(ctx, "k_ce_pack");
+    return DLMI_OK;
+  }
+  CeLogits logits(size_t v0, size_t vn, size_t vp) const {
+    CeLogits g = {};
+    g.P = s + p.wp;
+    g.Q = s + p.xp;
+    g.unscale_w = floats(p.unscale);
+    g.unscale_x = floats(p.unscale) + 2;
+    g.ni = static_cast<unsigned>(vp / p.T);
+    g.nj = static_cast<unsigned>(p.Bp / p.T);
+    g.kblocks = static_cast<unsigned>(p.Kp / 16);
+    g.stages = static_cast<unsigned>(dlmi_ceil_div(a.K, 32 / NP));
+    g.v0 = v0;
+    g.vn = vn;
+    return g;
+  }
+
+  template <int T>
+  int forward() const {
+    int rc = pack_rows();
+    for (size_t v0 = 0; rc == DLMI_OK && v0 < a.V; v0 += p.Vc) {
+      size_t const vn = a.V - v0 < p.Vc ? a.V - v0 : p.Vc, vp = dlmi_ceil_div(vn, T) * T;
+      rc = pack_classes(v0, vn, vp, false);
+      if (rc != DLMI_OK) return rc;
+      CeLogits const g = logits(v0, vn, vp);
+      hipLaunchKernelGGL((k_ce_stats<T, NP>), dim3(g.ni * g.nj), dim3(256), 0, ctx->stream, a, g, reinterpret_cast<float2 *>(s + p.part), p.Bp,
+                         v0 / T * 2, floats(p.target));
+      DLMI_LAUNCH_CHECK(ctx, "k_ce_stats");
+    }
+    if (rc != DLMI_OK) return rc;
+    hipLaunchKernelGGL(k_ce_join<16>, dim3(static_cast<unsigned>(dlmi_ceil_div(a.B, 64))), dim3(1024), 0, ctx->stream, a,
+                       reinterpret_cast<float2 *>(s + p.part), p.Bp, dlmi_ceil_div(a.V, static_cast<size_t>(T)) * 2, floats(p.target));
+    DLMI_LAUNCH_CHECK(ctx, "k_ce_join");
+    return DLMI_OK;
+  }
+
+  template <int T>
+  int backward() const {
+    int rc = pack_rows();
+    if (rc == DLMI_OK) rc = pack_rows_weighted();
+    unsigned const nb = static_cast<unsigned>(p.Bp / T), nk = static_cast<unsigned>(p.Kp / T), kb = static_cast<unsigned>(p.Bp / 16);
+    for (size_t v0 = 0; rc == DLMI_OK && v0 < a.V; v0 += p.Vc) {
+      size_t const vn = a.V - v0 < p.Vc ? a.V - v0 : p.Vc, vp = dlmi_ceil_div(vn, T) * T;
+      rc = pack_classes(v0, vn, vp, true);
+      if (rc != DLMI_OK) return rc;
+      CeLogits const g = logits(v0, vn, vp);
+      unsigned const kv = static_cast<unsigned>(vp / 16);
+      if (a.db != nullptr)
+        hipLaunchKernelGGL((k_ce_grad<T, NP, true>), dim3(g.ni * g.nj), dim3(256), 0, ctx->stream, a, g, s + p.dlb, s + p.dlv, kv, kb,
+                           floats(p.dbpart), p.Vc);
+      else
+        hipLaunchKernelGGL((k_ce_grad<T, NP, false>), dim3(g.ni * g.nj), dim3(256), 0, ctx->stream, a, g, s + p.dlb, s + p.dlv, kv, kb,
+                           nullptr, p.Vc);
+      DLMI_LAUNCH_CHECK(ctx, "k_ce_grad");
+      if (a.db != nullptr) {
+        hipLaunchKernelGGL(k_ce_db, dim3(static_cast<unsigned>(dlmi_ceil_div(vn, kCeBlock))), dim3(kCeBlock), 0, ctx->stream, floats(p.dbpart),
+                           p.Vc, nb * 2, vn, a.db + v0, a.scale, a.accumulate);
+        DLMI_LAUNCH_CHECK(ctx, "k_ce_db");
+      }
+      if (a.dX != nullptr) {
+        hipLaunchKernelGGL((k_ce_dx<T, NP>), dim3(nb * nk * p.slices), dim3(256), 0, ctx->stream, s + p.dlb, s + p.wt, nb, nk, kv, kv * NP / 2,
+                           p.per_slice, floats(p.unscale), floats(p.dxacc), a.B, a.K, v0 == 0 ? 1 : 0);
+        DLMI_LAUNCH_CHECK(ctx, "k_ce_dx");
+      }
+      if (a.dW != nullptr) {
+        hipLaunchKernelGGL((k_ce_dw<T, NP, E>), dim3(g.ni * nk), dim3(256), 0, ctx->stream, s + p.dlv, s + p.xg, g.ni, nk, kb,
+                           static_cast<unsigned>(dlmi_ceil_div(a.B, 32 / NP)), floats(p.unscale) + 1, a.scale, static_cast<E *>(a.dW) + v0 * a.K, vn, a.K,
+                           a.accumulate);
+        DLMI_LAUNCH_CHECK(ctx, "k_ce_dw");
+      }
+    }
+    if (rc != DLMI_OK || a.dX == nullptr) return rc;
+    size_t const blocks = dlmi_ceil_div(a.B * a.K, kCeBlock * 4), cap = static_cast<size_t>(ctx->num_cu) * 16;
+    hipLaunchKernelGGL(k_ce_dx_finish<E>, dim3(static_cast<unsigned>(blocks < cap ? blocks : cap)), dim3(kCeBlock), 0, ctx->stream, a,
+                       floats(p.dxacc), p.slices, static_cast<E *>(a.dX));
+    DLMI_LAUNCH_CHECK(ctx, "k_ce_dx_finish");
+    return DLMI_OK;
+  }
+};
+
+template <class E>
+constexpr int kCePlanes = sizeof(E) == 4 ? 2 : 1;
+
+template <class E>
+static int ce_run(dlmi_ctx *ctx, CeArgs const &a, bool back) {
+  constexpr int NP = kCePlanes<E>;
+  CeRun<E, NP> r{ctx, a, ce_plan<NP>(ctx, a.B, a.K, a.V, back), nullptr};
+  int const rc = dlmi_scratch_reserve(ctx, r.p.bytes);
+  if (rc != DLMI_OK) return rc;
+  r.s = dlmi_scratch_data(ctx);
+  switch (r.p.T) {
+    case 256: return back ? r.template backward<256>() : r.template forward<256>();
+    case 128: return back ? r.template backward<128>() : r.template forward<128>();
+    default: return back ? r.template backward<64>() : r.template forward<64>();
+  }
+}
+
+template <class E>
+int ce_forward(dlmi_ctx *ctx, CeArgs const &a) {
+  return ce_run<E>(ctx, a, false);
+}
+template <class E>
+int ce_backward(dlmi_ctx *ctx, CeArgs const &a) {
+  return ce_run<E>(ctx, a, true);
+}
+
+#endif  // DLMI_CE_IMPLEMENTATION
+
+}  // namespace dlmi
