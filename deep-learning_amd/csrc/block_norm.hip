@@ -22,6 +22,8 @@ namespace dlmi {
 
 constexpr int kBnMaxWidth = DLMI_BLOCK_NORM_MAX_WIDTH;
 
+typedef float f32x4v __attribute__((ext_vector_type(4)));
+
 template <class T>
 constexpr int kBnVec = 16 / static_cast<int>(sizeof(T));  // elements of a 16-byte access
 
@@ -61,30 +63,54 @@ __device__ __forceinline__ void bn_param(float const *p, float dflt, int col, in
   for (int i = 0; i < N; ++i) o[i] = p != nullptr && col + i < H ? p[col + i] : dflt;
 }
 
-// Sums of two values over the NT threads of a row, the same in every thread.
-template <int NT>
-__device__ __forceinline__ void bn_sum2(float &a, float &b, float2 *lds) {
+// Sum over each 16 lanes, the same in all of them (DPP).
+__device__ __forceinline__ float bn_row_sum(float v) {
+  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xB1, 0xf, 0xf, false));   // lane ^ 1
+  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x4E, 0xf, 0xf, false));   // lane ^ 2
+  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x141, 0xf, 0xf, false));  // mirrored in 8
+  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x140, 0xf, 0xf, false));  // mirrored in 16
+  return v;
+}
+// Over the 64 lanes, without LDS: rows of 16 and halves are swapped.
+__device__ __forceinline__ float bn_wave_sum(float v) {
+  v = bn_row_sum(v);
+  unsigned const r = __float_as_uint(v);
+  auto const p = __builtin_amdgcn_permlane16_swap(r, r, false, false);
+  v = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+  unsigned const h = __float_as_uint(v);
+  auto const q = __builtin_amdgcn_permlane32_swap(h, h, false, false);
+  return __uint_as_float(q[0]) + __uint_as_float(q[1]);
+}
+
+// Sums of K values over the NT threads of a row, the same in every thread.  Consecutive sums use alternating halves of
+// `lds` (flip), so one barrier each is enough: who writes a half again has passed the barrier behind its last reading.
+template <int NT, int K>
+__device__ __forceinline__ void bn_sums(float (&v)[K], float (*lds)[16][4], int &flip) {
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    a += __shfl_xor(a, o);
-    b += __shfl_xor(b, o);
-  }
+  for (int k = 0; k < K; ++k) v[k] = bn_wave_sum(v[k]);
   if constexpr (NT > 64) {
-    __syncthreads();  // the previous sums have been read
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = make_float2(a, b);
-    __syncthreads();
-    a = b = 0.0f;
+    if ((threadIdx.x & 63) == 0) {
 #pragma unroll
-    for (int w = 0; w < NT / 64; ++w) {
-      a += lds[w].x;
-      b += lds[w].y;
+      for (int k = 0; k < K; ++k) lds[flip][threadIdx.x >> 6][k] = v[k];
     }
+    __syncthreads();
+    // a row of 16 lanes takes the wavefronts' shares, one each
+    int const w = threadIdx.x & 15;
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = bn_row_sum(w < NT / 64 ? lds[flip][w][k] : 0.0f);
+    flip ^= 1;
   }
 }
 
+// tanh near 0 by its Taylor series (the next term is below 5e-8 of it), where 1 - e of the quotient cancels.
 __device__ __forceinline__ float bn_gate(int act, float g) {
-  if (act == DLMI_ACT_SIGMOID) return 1.0f / (1.0f + expf(-g));
-  if (act == DLMI_ACT_TANH) return tanhf(g);
+  if (act == DLMI_ACT_SIGMOID) return __builtin_amdgcn_rcpf(1.0f + __expf(-g));
+  if (act == DLMI_ACT_TANH) {
+    float const m = fabsf(g), e = __expf(-2.0f * m), q = g * g;
+    float const far = copysignf((1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e), g);
+    float const near = g + g * q * (-1.0f / 3.0f + q * (2.0f / 15.0f + q * (-17.0f / 315.0f + q * (62.0f / 2835.0f))));
+    return m < 0.3f ? near : far;
+  }
   return g;
 }
 __device__ __forceinline__ float bn_gate_slope(int act, float f) {
@@ -100,8 +126,10 @@ struct BnArgs {
   // backward
   void const *dy, *dh;
   void *dx, *du, *dgate;
-  float *partial;       // [workgroups][5][H]: dw_post, db_post, dw_pre, db_pre, the gate's
-  int want_gate_direct;  // a workgroup covers whole runs of rows that share a gate: it writes dgate itself
+  float *partial;       // [workgroups][planes][H]
+  int plane[5];         // of dw_post, db_post, dw_pre, db_pre, the shared gate; -1: not asked for
+  int planes;
+  int direct;           // a workgroup covers whole runs of rows that share a gate: it writes dgate itself
   size_t B;
   int H;
   int post, pre, act;
@@ -111,12 +139,54 @@ struct BnArgs {
   float rs, bs, eps_post, eps_pre;
 };
 
+// A row's 16-byte pieces of one thread, as they lie in memory.
+template <class T, int C>
+struct BnRaw {
+  BnVec<T> v[C];
+};
+
+template <class T, int NT, int C>
+__device__ __forceinline__ void bn_fetch(BnRaw<T, C> &o, T const *row, int H) {
+  constexpr int N = kBnVec<T>;
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    int const col = (c * NT + threadIdx.x) * N;
+    if (col + N <= H) {
+      o.v[c] = *reinterpret_cast<BnVec<T> const *>(row + col);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) o.v[c].v[i] = col + i < H ? row[col + i] : static_cast<T>(0.0f);
+    }
+  }
+}
+template <class T, int C>
+__device__ __forceinline__ void bn_widen(float (&o)[C][kBnVec<T>], BnRaw<T, C> const &r) {
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+#pragma unroll
+    for (int i = 0; i < kBnVec<T>; ++i) o[c][i] = static_cast<float>(r.v[c].v[i]);
+}
+
+#define BN_EACH                     \
+  _Pragma("unroll") for (int c = 0; c < C; ++c) _Pragma("unroll") for (int i = 0; i < N; ++i)
+#define BN_IN ((c * NT + static_cast<int>(threadIdx.x)) * N + i < H)
+
 template <class T, int NT, int C>
 __global__ __launch_bounds__(NT) void k_block_norm_fwd(BnArgs a) {
   constexpr int N = kBnVec<T>;
-  __shared__ float2 lds[16];
+  __shared__ float lds[2][16][4];
+  int flip = 0;
   int const H = a.H;
   float const inv_h = 1.0f / static_cast<float>(H);
+  BnRaw<T, C> ru, rx, rg;
+  auto const fetch = [&](size_t r) {
+    size_t const at = r * static_cast<size_t>(H);
+    bn_fetch<T, NT, C>(ru, static_cast<T const *>(a.u) + at, H);
+    bn_fetch<T, NT, C>(rx, static_cast<T const *>(a.x) + at, H);
+    if (a.gate_rows != 0)
+      bn_fetch<T, NT, C>(rg, static_cast<T const *>(a.gate) + (a.gate_rows == 1 ? r : r / a.gate_rows) * static_cast<size_t>(H), H);
+  };
+  if (blockIdx.x < a.B) fetch(blockIdx.x);
   float w1[C][N], b1[C][N], w2[C][N], b2[C][N];
 #pragma unroll
   for (int c = 0; c < C; ++c) {
@@ -126,89 +196,85 @@ __global__ __launch_bounds__(NT) void k_block_norm_fwd(BnArgs a) {
     bn_param(a.w_pre, 1.0f, col, H, w2[c]);
     bn_param(a.b_pre, 0.0f, col, H, b2[c]);
   }
+  // the columns beyond the row are zero; what centring makes of them stays out of the sums
+  auto const norm = [&](float (&v)[C][N], int how, float eps) {
+    if (how == DLMI_ROW_NORM_NONE) return;
+    if (how == DLMI_ROW_NORM_LAYER) {
+      float s[1] = {0.0f};
+      BN_EACH s[0] += v[c][i];
+      bn_sums<NT>(s, lds, flip);
+      float const mean = s[0] * inv_h;
+      BN_EACH v[c][i] = BN_IN ? v[c][i] - mean : 0.0f;
+    }
+    float q[1] = {0.0f};
+    BN_EACH q[0] += v[c][i] * v[c][i];
+    bn_sums<NT>(q, lds, flip);
+    float const rstd = 1.0f / sqrtf(q[0] * inv_h + eps);
+    BN_EACH v[c][i] *= rstd;
+  };
   for (size_t r = blockIdx.x; r < a.B; r += gridDim.x) {
     size_t const at = r * static_cast<size_t>(H);
     float u[C][N], x[C][N], g[C][N];
-#pragma unroll
-    for (int c = 0; c < C; ++c) bn_load(static_cast<T const *>(a.u) + at, (c * NT + threadIdx.x) * N, H, u[c]);
-#pragma unroll
-    for (int c = 0; c < C; ++c) bn_load(static_cast<T const *>(a.x) + at, (c * NT + threadIdx.x) * N, H, x[c]);
-    if (a.gate_rows != 0) {
-      T const *const gr = static_cast<T const *>(a.gate) + (a.gate_rows == 1 ? r : r / a.gate_rows) * static_cast<size_t>(H);
-#pragma unroll
-      for (int c = 0; c < C; ++c) bn_load(gr, (c * NT + threadIdx.x) * N, H, g[c]);
-    }
-    // the columns beyond the row are zero in u and x; what centring makes of them stays out of the sums
-    auto const norm = [&](float (&v)[C][N], int how, float eps) {
-      if (how == DLMI_ROW_NORM_NONE) return;
-      float s = 0.0f, q = 0.0f;
-      if (how == DLMI_ROW_NORM_LAYER) {
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-          for (int i = 0; i < N; ++i) s += v[c][i];
-        bn_sum2<NT>(s, q, lds);
-        float const mean = s * inv_h;
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-          for (int i = 0; i < N; ++i) v[c][i] = (c * NT + threadIdx.x) * N + i < static_cast<unsigned>(H) ? v[c][i] - mean : 0.0f;
-        s = q = 0.0f;
-      }
-#pragma unroll
-      for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int i = 0; i < N; ++i) q += v[c][i] * v[c][i];
-      bn_sum2<NT>(s, q, lds);
-      float const rstd = 1.0f / sqrtf(q * inv_h + eps);
-#pragma unroll
-      for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[c][i] *= rstd;
-    };
+    bn_widen(u, ru);
+    bn_widen(x, rx);
+    if (a.gate_rows != 0) bn_widen(g, rg);
+    // the next row is on its way while this one is worked on (y may be x and h may be u: this row's only)
+    if (r + gridDim.x < a.B) fetch(r + gridDim.x);
     norm(u, a.post, a.eps_post);
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        float n = u[c][i] * w1[c][i] + b1[c][i];
-        if (a.gate_rows != 0) n *= bn_gate(a.act, g[c][i]);
-        x[c][i] = a.rs * x[c][i] + a.bs * n;
-      }
-      bn_store(static_cast<T *>(a.y) + at, (c * NT + threadIdx.x) * N, H, x[c]);
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        if ((c * NT + threadIdx.x) * N + i >= static_cast<unsigned>(H)) x[c][i] = 0.0f;
+    BN_EACH {
+      float n = u[c][i] * w1[c][i] + b1[c][i];
+      if (a.gate_rows != 0) n *= bn_gate(a.act, g[c][i]);
+      x[c][i] = a.rs * x[c][i] + a.bs * n;
     }
+#pragma unroll
+    for (int c = 0; c < C; ++c) bn_store(static_cast<T *>(a.y) + at, (c * NT + threadIdx.x) * N, H, x[c]);
+    BN_EACH x[c][i] = BN_IN ? x[c][i] : 0.0f;
     norm(x, a.pre, a.eps_pre);
+    BN_EACH x[c][i] = x[c][i] * w2[c][i] + b2[c][i];
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) x[c][i] = x[c][i] * w2[c][i] + b2[c][i];
-      bn_store(static_cast<T *>(a.h) + at, (c * NT + threadIdx.x) * N, H, x[c]);
-    }
+    for (int c = 0; c < C; ++c) bn_store(static_cast<T *>(a.h) + at, (c * NT + threadIdx.x) * N, H, x[c]);
   }
 }
 
-template <class T, int NT, int C>
-__global__ __launch_bounds__(NT) void k_block_norm_bwd(BnArgs a) {
-  constexpr int N = kBnVec<T>;
-  __shared__ float2 lds[16];
+enum { kBnNoGate = 0, kBnGateEach = 1, kBnGateShared = 2 };
+
+// GATE: none, one row each, or shared by rows (f is formed once per run then, and its slope multiplies the finished sum).
+// BIAS: post has a bias, or a bias's gradient is asked for.
+// A thread keeps its columns' sums and the row at hand and the next in registers; the weights (and a shared gate's f) it
+// reads again every row from LDS, which only it uses: with them in registers too, two workgroups of 8 wavefronts did not
+// fit a CU without spilling ([16384 x 4096] bf16, shared gate: 511 us then).
+template <class T, int NT, int C, int GATE, bool BIAS>
+__global__ __launch_bounds__(NT, NT <= 512 && C * kBnVec<T> <= 8 ? 4 : 1) void k_block_norm_bwd(BnArgs a) {
+  constexpr int N = kBnVec<T>, Q = C * N / 4;
+  constexpr bool kLds = C * N <= 8;  // wider rows read the weights from memory
+  __shared__ float lds[2][16][4];
+  __shared__ f32x4v kept[kLds ? 2 + (BIAS ? 1 : 0) + (GATE == kBnGateShared ? 1 : 0) : 1][kLds ? Q : 1][kLds ? NT : 1];
+  constexpr int kW1 = 0, kW2 = 1, kF = 2, kB1 = GATE == kBnGateShared ? 3 : 2;
+  int flip = 0;
   int const H = a.H;
   float const inv_h = 1.0f / static_cast<float>(H);
-  float w1[C][N], b1[C][N], w2[C][N];
-  float dw1[C][N], db1[C][N], dw2[C][N], db2[C][N], dg[C][N];
+  auto const keep = [&](int k, float const (&v)[C][N]) {
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    int const col = (c * NT + threadIdx.x) * N;
-    bn_param(a.w_post, 1.0f, col, H, w1[c]);
-    bn_param(a.b_post, 0.0f, col, H, b1[c]);
-    bn_param(a.w_pre, 1.0f, col, H, w2[c]);
+    for (int q = 0; q < Q; ++q) {
+      int const c = q / (N / 4), i = q % (N / 4) * 4;
+      kept[k][q][threadIdx.x] = f32x4v{v[c][i], v[c][i + 1], v[c][i + 2], v[c][i + 3]};
+    }
+  };
+  auto const back = [&](int k, float (&v)[C][N]) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) dw1[c][i] = db1[c][i] = dw2[c][i] = db2[c][i] = dg[c][i] = 0.0f;
-  }
+    for (int q = 0; q < Q; ++q) {
+      int const c = q / (N / 4), i = q % (N / 4) * 4;
+      f32x4v const x = kept[k][q][threadIdx.x];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[c][i + j] = x[j];
+    }
+  };
+  auto const params = [&](float const *p, float dflt, float (&v)[C][N]) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) bn_param(p, dflt, (c * NT + threadIdx.x) * N, H, v[c]);
+  };
   size_t r0, r1;
-  if (a.want_gate_direct) {
+  if (a.direct) {
     r0 = blockIdx.x * a.rows_per_wg;
     r1 = r0 + a.rows_per_wg;
   } else {
@@ -219,172 +285,234 @@ __global__ __launch_bounds__(NT) void k_block_norm_bwd(BnArgs a) {
   }
   if (r1 > a.B) r1 = a.B;
   bool const live_y = a.dh != nullptr && a.pre != DLMI_ROW_NORM_NONE;
+  BnRaw<T, C> ru, ry, rt, re, rg;
+  auto const fetch = [&](size_t r) {
+    size_t const at = r * static_cast<size_t>(H);
+    bn_fetch<T, NT, C>(ru, static_cast<T const *>(a.u) + at, H);
+    if (live_y) bn_fetch<T, NT, C>(ry, static_cast<T const *>(a.y) + at, H);
+    if (a.dy != nullptr) bn_fetch<T, NT, C>(rt, static_cast<T const *>(a.dy) + at, H);
+    if (a.dh != nullptr) bn_fetch<T, NT, C>(re, static_cast<T const *>(a.dh) + at, H);
+    if constexpr (GATE == kBnGateEach) bn_fetch<T, NT, C>(rg, static_cast<T const *>(a.gate) + at, H);
+  };
+  if (r0 < r1) fetch(r0);
+  if constexpr (kLds) {
+    float v[C][N];
+    params(a.w_post, 1.0f, v);
+    keep(kW1, v);
+    params(a.w_pre, 1.0f, v);
+    keep(kW2, v);
+    if constexpr (BIAS) {
+      params(a.b_post, 0.0f, v);
+      keep(kB1, v);
+    }
+  }
+  // the weights and the shared gate of this thread's columns, for the moment
+  auto const weight = [&](int k, float (&v)[C][N]) {
+    if constexpr (kLds)
+      back(k, v);
+    else
+      params(k == kW1 ? a.w_post : a.w_pre, 1.0f, v);
+  };
+  auto const bias = [&](float (&v)[C][N]) {
+    if constexpr (kLds)
+      back(kB1, v);
+    else
+      params(a.b_post, 0.0f, v);
+  };
+  auto const gate_row = [&](size_t r, float (&v)[C][N]) {
+    bn_fetch<T, NT, C>(rg, static_cast<T const *>(a.gate) + r / a.gate_rows * static_cast<size_t>(H), H);
+    bn_widen(v, rg);
+    BN_EACH v[c][i] = bn_gate(a.act, v[c][i]);
+  };
+  auto const shared_gate = [&](size_t r, float (&v)[C][N]) {
+    if constexpr (kLds)
+      back(kF, v);
+    else
+      gate_row(r, v);
+  };
+  float dw1[C][N], db1[C][N], dw2[C][N], db2[C][N], dg[C][N];
+  BN_EACH dw1[c][i] = db1[c][i] = dw2[c][i] = db2[c][i] = dg[c][i] = 0.0f;
   for (size_t r = r0; r < r1; ++r) {
     size_t const at = r * static_cast<size_t>(H);
-    float u[C][N], y[C][N], t[C][N], e[C][N], g[C][N];
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-      int const col = (c * NT + threadIdx.x) * N;
-      bn_load(static_cast<T const *>(a.u) + at, col, H, u[c]);
-      if (live_y) bn_load(static_cast<T const *>(a.y) + at, col, H, y[c]);
-      if (a.dy != nullptr) {
-        bn_load(static_cast<T const *>(a.dy) + at, col, H, t[c]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) t[c][i] = 0.0f;
+    float u[C][N], y[C][N], t[C][N], e[C][N];
+    bn_widen(u, ru);
+    if (live_y) bn_widen(y, ry);
+    if (a.dy != nullptr)
+      bn_widen(t, rt);
+    else
+      BN_EACH t[c][i] = 0.0f;
+    if (a.dh != nullptr)
+      bn_widen(e, re);
+    else
+      BN_EACH e[c][i] = 0.0f;
+    BnRaw<T, C> rgr;
+    if constexpr (GATE == kBnGateEach) rgr = rg;
+    if constexpr (GATE == kBnGateShared && kLds) {
+      if (r == r0 || r % a.gate_rows == 0) {
+        float v[C][N];
+        gate_row(r, v);
+        keep(kF, v);
       }
-      if (a.dh != nullptr) bn_load(static_cast<T const *>(a.dh) + at, col, H, e[c]);
     }
-    if (a.gate_rows != 0) {
-      T const *const gr = static_cast<T const *>(a.gate) + (a.gate_rows == 1 ? r : r / a.gate_rows) * static_cast<size_t>(H);
-#pragma unroll
-      for (int c = 0; c < C; ++c) bn_load(gr, (c * NT + threadIdx.x) * N, H, g[c]);
-    }
+    // the next row is on its way while this one is worked on (dx may be dy and du may be dh: this row's only)
+    if (r + 1 < r1) fetch(r + 1);
     // the means, where a layer norm asks for them
     if (a.post == DLMI_ROW_NORM_LAYER || (live_y && a.pre == DLMI_ROW_NORM_LAYER)) {
-      float su = 0.0f, sy = 0.0f;
-#pragma unroll
-      for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          su += u[c][i];
-          if (live_y) sy += y[c][i];
-        }
-      bn_sum2<NT>(su, sy, lds);
-      float const mu = a.post == DLMI_ROW_NORM_LAYER ? su * inv_h : 0.0f;
-      float const my = a.pre == DLMI_ROW_NORM_LAYER ? sy * inv_h : 0.0f;
-#pragma unroll
-      for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          bool const in = (c * NT + threadIdx.x) * N + i < static_cast<unsigned>(H);
-          u[c][i] = in ? u[c][i] - mu : 0.0f;
-          if (live_y) y[c][i] = in ? y[c][i] - my : 0.0f;
-        }
+      float s[2] = {0.0f, 0.0f};
+      BN_EACH {
+        s[0] += u[c][i];
+        if (live_y) s[1] += y[c][i];
+      }
+      bn_sums<NT>(s, lds, flip);
+      float const mu = a.post == DLMI_ROW_NORM_LAYER ? s[0] * inv_h : 0.0f;
+      float const my = a.pre == DLMI_ROW_NORM_LAYER ? s[1] * inv_h : 0.0f;
+      BN_EACH {
+        u[c][i] = BN_IN ? u[c][i] - mu : 0.0f;
+        if (live_y) y[c][i] = BN_IN ? y[c][i] - my : 0.0f;
+      }
     }
     // pre's gradient
-    float qu = 0.0f, qy = 0.0f, sg = 0.0f, sgy = 0.0f;
-#pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        qu += u[c][i] * u[c][i];
-        if (live_y) {
-          float const gh = e[c][i] * w2[c][i];
-          qy += y[c][i] * y[c][i];
-          sg += gh;
-          sgy += gh * y[c][i];
-        }
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    float w[C][N];
+    if (live_y) weight(kW2, w);
+    BN_EACH {
+      s[0] += u[c][i] * u[c][i];
+      if (live_y) {
+        float const gh = e[c][i] * w[c][i];
+        s[1] += y[c][i] * y[c][i];
+        s[2] += gh;
+        s[3] += gh * y[c][i];
       }
-    bn_sum2<NT>(qu, qy, lds);
-    float const ru = a.post != DLMI_ROW_NORM_NONE ? 1.0f / sqrtf(qu * inv_h + a.eps_post) : 1.0f;
+    }
+    bn_sums<NT>(s, lds, flip);
+    float const ru_ = a.post != DLMI_ROW_NORM_NONE ? 1.0f / sqrtf(s[0] * inv_h + a.eps_post) : 1.0f;
     if (live_y) {
-      bn_sum2<NT>(sg, sgy, lds);
-      float const ry = 1.0f / sqrtf(qy * inv_h + a.eps_pre);
-      float const c1 = a.pre == DLMI_ROW_NORM_LAYER ? sg * inv_h : 0.0f;
-      float const c2 = sgy * ry * inv_h;
-#pragma unroll
-      for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          float const yh = y[c][i] * ry;
-          dw2[c][i] += e[c][i] * yh;
-          db2[c][i] += e[c][i];
-          t[c][i] += ry * (e[c][i] * w2[c][i] - c1 - yh * c2);
-        }
-    } else if (a.dh != nullptr) {
-#pragma unroll
-      for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int i = 0; i < N; ++i) t[c][i] += e[c][i];
-    }
-    // the gate, then post's gradient; e becomes dn, y becomes dx
-    float s1 = 0.0f, s2 = 0.0f;
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        bool const in = (c * NT + threadIdx.x) * N + i < static_cast<unsigned>(H);
-        float const uh = u[c][i] * ru;
-        float d = a.bs * t[c][i];
-        if (a.gate_rows != 0) {
-          float const f = bn_gate(a.act, g[c][i]);
-          dg[c][i] += d * bn_gate_slope(a.act, f) * (uh * w1[c][i] + b1[c][i]);
-          d *= f;
-        }
-        d = in ? d : 0.0f;
-        dw1[c][i] += d * uh;
-        db1[c][i] += d;
-        float const gd = d * w1[c][i];
-        s1 += gd;
-        s2 += gd * uh;
-        e[c][i] = d;
-        t[c][i] *= a.rs;
-        u[c][i] = uh;
+      float const ry_ = 1.0f / sqrtf(s[1] * inv_h + a.eps_pre);
+      float const c1 = a.pre == DLMI_ROW_NORM_LAYER ? s[2] * inv_h : 0.0f;
+      float const c2 = s[3] * ry_ * inv_h;
+      weight(kW2, w);
+      BN_EACH {
+        float const yh = y[c][i] * ry_;
+        dw2[c][i] += e[c][i] * yh;
+        if constexpr (BIAS) db2[c][i] += e[c][i];
+        t[c][i] += ry_ * (e[c][i] * w[c][i] - c1 - yh * c2);
       }
-      bn_store(static_cast<T *>(a.dx) + at, (c * NT + threadIdx.x) * N, H, t[c]);
+    } else {
+      BN_EACH t[c][i] += e[c][i];
     }
+    // the gate, then post's gradient; e becomes dn
+    float p[2] = {0.0f, 0.0f};
+    float f[C][N], b1[C][N];
+    weight(kW1, w);
+    if constexpr (GATE == kBnGateEach) {
+      bn_widen(f, rgr);
+      BN_EACH f[c][i] = bn_gate(a.act, f[c][i]);
+    }
+    if constexpr (GATE == kBnGateShared) shared_gate(r, f);
+    if constexpr (BIAS && GATE != kBnNoGate) bias(b1);
+    BN_EACH {
+      float const uh = u[c][i] * ru_;
+      float d = BN_IN ? a.bs * t[c][i] : 0.0f;
+      if constexpr (GATE != kBnNoGate) {
+        float n = uh * w[c][i];
+        if constexpr (BIAS) n += b1[c][i];
+        if constexpr (GATE == kBnGateEach)
+          dg[c][i] = d * bn_gate_slope(a.act, f[c][i]) * n;
+        else
+          dg[c][i] += d * n;
+        d *= f[c][i];
+      }
+      dw1[c][i] += d * uh;
+      if constexpr (BIAS) db1[c][i] += d;
+      float const gd = d * w[c][i];
+      p[0] += gd;
+      p[1] += gd * uh;
+      e[c][i] = d;
+      t[c][i] *= a.rs;
+      u[c][i] = uh;
+    }
+#pragma unroll
+    for (int c = 0; c < C; ++c) bn_store(static_cast<T *>(a.dx) + at, (c * NT + threadIdx.x) * N, H, t[c]);
     if (a.post != DLMI_ROW_NORM_NONE) {
-      bn_sum2<NT>(s1, s2, lds);
-      float const c1 = a.post == DLMI_ROW_NORM_LAYER ? s1 * inv_h : 0.0f, c2 = s2 * inv_h;
-#pragma unroll
-      for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int i = 0; i < N; ++i) e[c][i] = ru * (e[c][i] * w1[c][i] - c1 - u[c][i] * c2);
+      bn_sums<NT>(p, lds, flip);
+      weight(kW1, w);
+      float const c1 = a.post == DLMI_ROW_NORM_LAYER ? p[0] * inv_h : 0.0f, c2 = p[1] * inv_h;
+      BN_EACH e[c][i] = ru_ * (e[c][i] * w[c][i] - c1 - u[c][i] * c2);
     }
 #pragma unroll
     for (int c = 0; c < C; ++c) bn_store(static_cast<T *>(a.du) + at, (c * NT + threadIdx.x) * N, H, e[c]);
-    if (a.want_gate_direct && a.gate_rows != 0 && ((r + 1) % a.gate_rows == 0 || r + 1 == a.B)) {
-      T *const out = static_cast<T *>(a.dgate) + r / a.gate_rows * static_cast<size_t>(H);
+    if constexpr (GATE == kBnGateEach) {
+      if (a.dgate != nullptr) {
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        if (a.dgate != nullptr) bn_store(out, (c * NT + threadIdx.x) * N, H, dg[c]);
+        for (int c = 0; c < C; ++c) bn_store(static_cast<T *>(a.dgate) + at, (c * NT + threadIdx.x) * N, H, dg[c]);
+      }
+    }
+    if constexpr (GATE == kBnGateShared) {
+      if (a.direct && ((r + 1) % a.gate_rows == 0 || r + 1 == a.B)) {
+        shared_gate(r, f);
+        BN_EACH dg[c][i] *= bn_gate_slope(a.act, f[c][i]);
+        if (a.dgate != nullptr) {
+          T *const out = static_cast<T *>(a.dgate) + r / a.gate_rows * static_cast<size_t>(H);
 #pragma unroll
-        for (int i = 0; i < N; ++i) dg[c][i] = 0.0f;
+          for (int c = 0; c < C; ++c) bn_store(out, (c * NT + threadIdx.x) * N, H, dg[c]);
+        }
+        BN_EACH dg[c][i] = 0.0f;
       }
     }
   }
   if (a.partial == nullptr) return;
-  float *const out = a.partial + static_cast<size_t>(blockIdx.x) * 5 * H;
-#pragma unroll
-  for (int c = 0; c < C; ++c)
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
+  float *const out = a.partial + static_cast<size_t>(blockIdx.x) * a.planes * H;
+  auto const leave = [&](int plane, float const (&v)[C][N]) {
+    if (plane < 0) return;
+    BN_EACH {
       int const col = (c * NT + threadIdx.x) * N + i;
-      if (col >= H) continue;
-      if (a.post != DLMI_ROW_NORM_NONE) {
-        out[col] = dw1[c][i];
-        out[H + col] = db1[c][i];
-      }
-      if (a.pre != DLMI_ROW_NORM_NONE) {
-        out[2 * H + col] = dw2[c][i];
-        out[3 * static_cast<size_t>(H) + col] = db2[c][i];
-      }
-      if (!a.want_gate_direct) out[4 * static_cast<size_t>(H) + col] = dg[c][i];
+      if (col < H) out[static_cast<size_t>(plane) * H + col] = v[c][i];
     }
+  };
+  leave(a.plane[0], dw1);
+  if constexpr (BIAS) leave(a.plane[1], db1);
+  leave(a.plane[2], dw2);
+  if constexpr (BIAS) leave(a.plane[3], db2);
+  if constexpr (GATE == kBnGateShared) {
+    if (r0 < r1) {
+      float f[C][N];
+      shared_gate(r1 - 1, f);
+      BN_EACH dg[c][i] *= bn_gate_slope(a.act, f[c][i]);
+    }
+    leave(a.plane[4], dg);
+  }
 }
 
 struct BnReduce {
   float const *partial;
-  float *out[4];      // the parameters' gradients (may be null)
-  void *dgate;        // [runs][H] (may be null)
-  unsigned workgroups, slices, runs;
+  int plane[5], planes;
+  float *out[4];      // the parameters' gradients
+  void *dgate;        // [runs][H]
+  unsigned workgroups, slices;
   int H, accumulate;
 };
 
-// 64 columns of one plane: 16 threads per column add every 16th row, then a tree.  Planes 0-3 the parameters' gradients
-// over all workgroups, planes 4 and up a run's slices of the gate's.
+// 64 columns of one plane: 16 threads per column add every 16th row, then a tree.  blockIdx.y: a plane of the parameters'
+// gradients (over all workgroups), from `params` on a run's slices of the gate's.
 template <class T>
-__global__ __launch_bounds__(1024) void k_block_norm_reduce(BnReduce a) {
+__global__ __launch_bounds__(1024) void k_block_norm_reduce(BnReduce a, unsigned params) {
   __shared__ float lds[16][64];
-  unsigned const plane = blockIdx.y < 4 ? blockIdx.y : 4;
-  if (plane < 4 ? a.out[plane] == nullptr : a.dgate == nullptr) return;
-  unsigned const from = plane < 4 ? 0 : (blockIdx.y - 4) * a.slices, n = plane < 4 ? a.workgroups : a.slices;
+  bool const gate = blockIdx.y >= params;
+  int which = 4;
+  if (!gate)
+    for (which = 0; a.plane[which] != static_cast<int>(blockIdx.y); ++which) {
+    }
+  int const plane = a.plane[which];
+  unsigned const from = gate ? (blockIdx.y - params) * a.slices : 0, n = gate ? a.slices : a.workgroups;
   int const col = static_cast<int>(blockIdx.x * 64 + (threadIdx.x & 63));
   unsigned const part = threadIdx.x >> 6;
   float s = 0.0f;
-  if (col < a.H)
-    for (unsigned w = part; w < n; w += 16) s += a.partial[(static_cast<size_t>(from + w) * 5 + plane) * a.H + col];
+  if (col < a.H) {
+    float const *const p = a.partial + static_cast<size_t>(plane) * a.H + col;
+    size_t const step = static_cast<size_t>(a.planes) * a.H;
+#pragma unroll 8
+    for (unsigned w = part; w < n; w += 16) s += p[(from + w) * step];
+  }
   lds[part][threadIdx.x & 63] = s;
   __syncthreads();
   for (unsigned o = 8; o > 0; o >>= 1) {
@@ -393,18 +521,30 @@ __global__ __launch_bounds__(1024) void k_block_norm_reduce(BnReduce a) {
   }
   if (part != 0 || col >= a.H) return;
   s = lds[0][threadIdx.x & 63];
-  if (plane < 4)
-    a.out[plane][col] = a.accumulate ? a.out[plane][col] + s : s;
+  if (!gate)
+    a.out[which][col] = a.accumulate ? a.out[which][col] + s : s;
   else
-    static_cast<T *>(a.dgate)[static_cast<size_t>(blockIdx.y - 4) * a.H + col] = static_cast<T>(s);
+    static_cast<T *>(a.dgate)[static_cast<size_t>(blockIdx.y - params) * a.H + col] = static_cast<T>(s);
+}
+
+template <class T, int NT, int C, int GATE>
+static void bn_launch_bwd(dlmi_ctx *ctx, BnArgs const &a, unsigned blocks) {
+  if (a.b_post != nullptr || a.plane[1] >= 0 || a.plane[3] >= 0)
+    hipLaunchKernelGGL((k_block_norm_bwd<T, NT, C, GATE, true>), dim3(blocks), dim3(NT), 0, ctx->stream, a);
+  else
+    hipLaunchKernelGGL((k_block_norm_bwd<T, NT, C, GATE, false>), dim3(blocks), dim3(NT), 0, ctx->stream, a);
 }
 
 template <class T, int NT, int C>
 static void bn_launch(dlmi_ctx *ctx, bool back, BnArgs const &a, unsigned blocks) {
-  if (back)
-    hipLaunchKernelGGL((k_block_norm_bwd<T, NT, C>), dim3(blocks), dim3(NT), 0, ctx->stream, a);
-  else
+  if (!back)
     hipLaunchKernelGGL((k_block_norm_fwd<T, NT, C>), dim3(blocks), dim3(NT), 0, ctx->stream, a);
+  else if (a.gate_rows == 0)
+    bn_launch_bwd<T, NT, C, kBnNoGate>(ctx, a, blocks);
+  else if (a.gate_rows == 1)
+    bn_launch_bwd<T, NT, C, kBnGateEach>(ctx, a, blocks);
+  else
+    bn_launch_bwd<T, NT, C, kBnGateShared>(ctx, a, blocks);
 }
 
 // Threads of a row: 8 columns each, up to 1024 threads; wider rows 16 columns each.
@@ -525,27 +665,32 @@ int dlmi_block_norm_bwd(dlmi_ctx *ctx, dlmi_dtype type, dlmi_block_norm_desc con
   a.dx = dx;
   a.du = du;
   a.dgate = dgate;
-  bool const sums = dw_post != nullptr || db_post != nullptr || dw_pre != nullptr || db_pre != nullptr;
-  // as many workgroups as fill the device with 32 wavefronts per CU, but at least 4 rows each where there are sums: a
-  // workgroup leaves up to 5 rows of partial sums
-  size_t most = static_cast<size_t>(ctx->num_cu) * (2048 / bn_threads(a.H));
+  float *const params[4] = {dw_post, db_post, dw_pre, db_pre};
+  for (int k = 0; k < 4; ++k) a.plane[k] = params[k] != nullptr ? a.planes++ : -1;
+  unsigned const sums = static_cast<unsigned>(a.planes);
+  // as many workgroups as run at once (16 wavefronts per CU), but at least 4 rows each where there are sums: a workgroup
+  // leaves a row of partial sums per plane
+  size_t const nt = static_cast<size_t>(bn_threads(a.H));
+  size_t const most = static_cast<size_t>(ctx->num_cu) * (nt < 1024 ? 1024 / nt : 1);
   size_t want = dlmi_ceil_div(B, most);
-  if ((sums || desc->gate_rows > 1) && want < 4) want = 4;
+  if ((sums != 0 || desc->gate_rows > 1) && want < 4) want = 4;
   size_t const gr = desc->gate_rows != 0 ? desc->gate_rows : 1;
-  size_t runs = dlmi_ceil_div(B, gr), blocks;
+  size_t const runs = dlmi_ceil_div(B, gr);
+  size_t blocks;
   a.slices = 1;
-  a.want_gate_direct = gr <= want ? 1 : 0;
-  if (a.want_gate_direct) {
+  a.direct = gr <= want ? 1 : 0;
+  if (a.direct) {
     a.rows_per_wg = want / gr * gr;
     blocks = dlmi_ceil_div(B, a.rows_per_wg);
   } else {
+    // (runs that are cut into slices are longer than `want` rows, so there are fewer of them than workgroups)
     a.slices = static_cast<unsigned>(dlmi_ceil_div(gr < B ? gr : B, want));
     a.rows_per_wg = want;
     blocks = runs * a.slices;
   }
-  // (runs that are cut into slices are longer than `want` rows, so there are fewer of them than workgroups)
-  if (sums || (!a.want_gate_direct && dgate != nullptr)) {
-    int const rc = dlmi_scratch_reserve(ctx, blocks * 5 * H * sizeof(float));
+  a.plane[4] = !a.direct && dgate != nullptr ? a.planes++ : -1;
+  if (a.planes != 0) {
+    int const rc = dlmi_scratch_reserve(ctx, blocks * a.planes * H * sizeof(float));
     if (rc != DLMI_OK) return rc;
     a.partial = reinterpret_cast<float *>(dlmi_scratch_data(ctx));
   }
@@ -555,24 +700,22 @@ int dlmi_block_norm_bwd(dlmi_ctx *ctx, dlmi_dtype type, dlmi_block_norm_desc con
     bn_dispatch<__bf16>(ctx, true, a, static_cast<unsigned>(blocks));
   DLMI_LAUNCH_CHECK(ctx, "k_block_norm_bwd");
   if (a.partial == nullptr) return DLMI_OK;
+  // (without dh nothing was added up for the norm before the next block: the kernel left zeros)
   BnReduce r = {};
   r.partial = a.partial;
-  r.out[0] = dw_post;
-  r.out[1] = db_post;
-  // without dh nothing was added up for the norm before the next block: the kernel left zeros
-  r.out[2] = dw_pre;
-  r.out[3] = db_pre;
-  r.dgate = a.want_gate_direct ? nullptr : dgate;
+  for (int k = 0; k < 5; ++k) r.plane[k] = a.plane[k];
+  for (int k = 0; k < 4; ++k) r.out[k] = params[k];
+  r.planes = a.planes;
+  r.dgate = dgate;
   r.workgroups = static_cast<unsigned>(blocks);
   r.slices = a.slices;
-  r.runs = static_cast<unsigned>(runs);
   r.H = a.H;
   r.accumulate = accumulate;
-  dim3 const grid(static_cast<unsigned>(dlmi_ceil_div(H, 64)), 4 + (r.dgate != nullptr ? r.runs : 0));
+  dim3 const grid(static_cast<unsigned>(dlmi_ceil_div(H, 64)), sums + (a.plane[4] >= 0 ? static_cast<unsigned>(runs) : 0u));
   if (type == DLMI_F32)
-    hipLaunchKernelGGL(k_block_norm_reduce<float>, grid, dim3(1024), 0, ctx->stream, r);
+    hipLaunchKernelGGL(k_block_norm_reduce<float>, grid, dim3(1024), 0, ctx->stream, r, sums);
   else
-    hipLaunchKernelGGL(k_block_norm_reduce<__bf16>, grid, dim3(1024), 0, ctx->stream, r);
+    hipLaunchKernelGGL(k_block_norm_reduce<__bf16>, grid, dim3(1024), 0, ctx->stream, r, sums);
   DLMI_LAUNCH_CHECK(ctx, "k_block_norm_reduce");
   return DLMI_OK;
 }
