@@ -101,7 +101,20 @@ def load_library():
     lib = ctypes.CDLL(LIB_PATH)
     lib.dlmi_last_error.restype = ctypes.c_char_p
     lib.dlmi_last_error.argtypes = [vp]
+    # the calls of a training or serving step's inner loop: with their argument types declared, ctypes takes plain integers
+    # (addresses as data_ptr() gives them), which halves what a call costs on the host
+    lib.dlmi_vocab_ce_fwd.argtypes = [vp, c_int, c_sz, c_sz, c_sz] + [vp] * 6
+    lib.dlmi_vocab_ce_bwd.argtypes = [vp, c_int, c_sz, c_sz, c_sz] + [vp] * 6 + [c_f] + [vp] * 3 + [c_int]
+    lib.dlmi_block_norm_fwd.argtypes = [vp, c_int, vp, c_sz, c_sz] + [vp] * 9
+    lib.dlmi_block_norm_bwd.argtypes = [vp, c_int, vp, c_sz, c_sz] + [vp] * 15 + [c_int]
+    lib.dlmi_orthogonalize.argtypes = [vp, c_int, c_sz, c_sz, vp, vp, vp]
+    lib.dlmi_opt_muon.argtypes = [vp, c_sz, vp, c_f, c_int, c_f, vp]
     return lib
+
+
+def _a(t):
+    """A tensor's address (None: null) for the calls whose argument types are declared."""
+    return None if t is None else t.data_ptr()
 
 
 def _p(t):
@@ -125,6 +138,7 @@ class Dlmi:
             raise DlmiError("dlmi_ctx_create failed with %d" % rc)
         self.ctx = ctx
         self._stream = stream
+        self._types = {torch.float32: DTYPE["F32"], torch.bfloat16: DTYPE["BF16"]}
 
     def close(self):
         if getattr(self, "ctx", None):
@@ -150,7 +164,7 @@ class Dlmi:
 
     def _chk_is(self, t, what, dtype, *shape):
         """One tensor of the calls that take more than fp32: its type, shape, device and layout."""
-        if t is None:
+        if t is None or (t.dtype is dtype and t.shape == shape and t.device == self.device and t.is_contiguous()):
             return
         assert t.dtype == dtype, "%s must be %s, is %s" % (what, dtype, t.dtype)
         assert tuple(t.shape) == shape, "%s must be %s, is %s" % (what, shape, tuple(t.shape))
@@ -159,9 +173,8 @@ class Dlmi:
 
     def _type(self, t):
         """dlmi_dtype of a tensor of `type`."""
-        types = {self.torch.float32: DTYPE["F32"], self.torch.bfloat16: DTYPE["BF16"]}
-        assert t.dtype in types, "float32 or bfloat16 tensors, not %s" % t.dtype
-        return c_int(types[t.dtype])
+        assert t.dtype in self._types, "float32 or bfloat16 tensors, not %s" % t.dtype
+        return self._types[t.dtype]
 
     def _out(self, dtype, *shape):
         """An output that belongs to the context's stream, whichever stream is current."""
@@ -393,7 +406,7 @@ class Dlmi:
         o = out if out is not None else self._out(G.dtype, rows, cols)
         self._chk_is(o, "out", G.dtype, rows, cols)
         ns = NewtonSchulz(*[float(c) for c in coefficients], int(steps), float(eps))
-        self._ck(self.lib.dlmi_orthogonalize(self.ctx, kind, c_sz(rows), c_sz(cols), _p(G), _p(o), ctypes.byref(ns)))
+        self._ck(self.lib.dlmi_orthogonalize(self.ctx, kind, rows, cols, _a(G), _a(o), ctypes.byref(ns)))
         return o
 
     def opt_muon(self, problems, lr, momentum=0.95, wd=0.0, nesterov=True, steps=5, coefficients=(3.4445, -4.7750, 2.0315),
@@ -407,11 +420,10 @@ class Dlmi:
             for t, what in ((p, "p"), (g, "g"), (m, "m")):
                 self._chk_is(t, what, self.torch.float32, *p.shape)
             a.rows, a.cols = p.shape
-            a.params, a.grads, a.momentum = _p(p), _p(g), _p(m)
+            a.params, a.grads, a.momentum = _a(p), _a(g), _a(m)
             a.lr = float(q[3]) if len(q) > 3 else float(lr)
         ns = NewtonSchulz(*[float(c) for c in coefficients], int(steps), float(eps))
-        self._ck(self.lib.dlmi_opt_muon(self.ctx, c_sz(len(problems)), arr, c_f(momentum), c_int(1 if nesterov else 0), c_f(wd),
-                                        ctypes.byref(ns)))
+        self._ck(self.lib.dlmi_opt_muon(self.ctx, len(problems), arr, momentum, 1 if nesterov else 0, wd, ctypes.byref(ns)))
 
     def opt_adabound(self, p, g, m1, m2, vhat, mask, lr_t, beta1, beta2, eps, wd, rate_lower, rate_upper, nthreads=0):
         self._chk(p, g, m1, m2, vhat, mask)
@@ -595,11 +607,12 @@ class Dlmi:
         """Cross entropy of softmax(X W^T + bias) at int32 labels, the logits not kept (dlmi_vocab_ce_fwd); a label outside
         [0, V) leaves its row out.  Returns (loss, lse), float32 [B]."""
         kind = self._type(X)
+        if loss is None and lse is None:
+            loss, lse = self._out(self.torch.float32, 2, X.shape[0]).unbind(0)
         loss = loss if loss is not None else self._out(self.torch.float32, X.shape[0])
         lse = lse if lse is not None else self._out(self.torch.float32, X.shape[0])
         B, K, V = self._chk_vocab_ce(X, W, labels, bias, dict(loss=loss, lse=lse))
-        self._ck(self.lib.dlmi_vocab_ce_fwd(self.ctx, kind, c_sz(B), c_sz(K), c_sz(V), _p(X), _p(W), _p(bias), _p(labels),
-                                            _p(loss), _p(lse)))
+        self._ck(self.lib.dlmi_vocab_ce_fwd(self.ctx, kind, B, K, V, _a(X), _a(W), _a(bias), _a(labels), _a(loss), _a(lse)))
         return loss, lse
 
     def vocab_ce_bwd(self, X, W, labels, lse, bias=None, dloss=None, scale=1.0, dX=None, dW=None, db=None, accumulate=False):
@@ -615,9 +628,8 @@ class Dlmi:
         self._chk_is(dX, "dX", X.dtype, B, K)
         self._chk_is(dW, "dW", X.dtype, V, K)
         self._chk_is(db, "db", self.torch.float32, V)
-        self._ck(self.lib.dlmi_vocab_ce_bwd(self.ctx, kind, c_sz(B), c_sz(K), c_sz(V), _p(X), _p(W), _p(bias), _p(labels),
-                                            _p(lse), _p(dloss), c_f(scale), _p(dX), _p(dW), _p(db),
-                                            c_int(1 if accumulate else 0)))
+        self._ck(self.lib.dlmi_vocab_ce_bwd(self.ctx, kind, B, K, V, _a(X), _a(W), _a(bias), _a(labels), _a(lse), _a(dloss),
+                                            scale, _a(dX), _a(dW), _a(db), 1 if accumulate else 0))
         return dX, dW, db
 
     # ------------------------------------------------------------ residual blocks with row norms
@@ -626,50 +638,50 @@ class Dlmi:
                         eps_pre=1e-5, residual_scale=1.0, branch_scale=1.0):
         return BlockNormDesc(post, pre, gate_act, gate_rows, eps_post, eps_pre, residual_scale, branch_scale)
 
-    def _chk_block_norm(self, desc, like, rows, gate, params):
-        B, H = like.shape
-        for what, t in rows.items():
-            self._chk_is(t, what, like.dtype, B, H)
-        if gate is not None and desc.gate_rows:
-            self._chk_is(gate, "gate", like.dtype, -(-B // desc.gate_rows), H)
-        for what, t in params.items():
-            self._chk_is(t, what, self.torch.float32, H)
-        return B, H
-
     def block_norm_fwd(self, desc, x, u, gate=None, w_post=None, b_post=None, w_pre=None, b_pre=None, y=None, h=None):
         """y = residual_scale x + branch_scale f(gate) post(u), h = pre(y) (dlmi_block_norm_fwd).  Returns (y, h)."""
-        assert u.dim() == 2
-        kind = self._type(u)
-        y = y if y is not None else self._out(u.dtype, *u.shape)
-        h = h if h is not None else self._out(u.dtype, *u.shape)
-        B, H = self._chk_block_norm(desc, u, dict(x=x, u=u, y=y, h=h), gate,
-                                    dict(w_post=w_post, b_post=b_post, w_pre=w_pre, b_pre=b_pre))
-        self._ck(self.lib.dlmi_block_norm_fwd(self.ctx, kind, ctypes.byref(desc), c_sz(B), c_sz(H), _p(x), _p(u), _p(gate),
-                                              _p(w_post), _p(b_post), _p(w_pre), _p(b_pre), _p(y), _p(h)))
+        B, H = u.shape
+        kind, dtype = self._type(u), u.dtype
+        y = y if y is not None else self._out(dtype, B, H)
+        h = h if h is not None else self._out(dtype, B, H)
+        for t, what in ((u, "u"), (x, "x"), (y, "y"), (h, "h")):
+            self._chk_is(t, what, dtype, B, H)
+        if gate is not None and desc.gate_rows:
+            self._chk_is(gate, "gate", dtype, -(-B // desc.gate_rows), H)
+        for t, what in ((w_post, "w_post"), (b_post, "b_post"), (w_pre, "w_pre"), (b_pre, "b_pre")):
+            self._chk_is(t, what, self.torch.float32, H)
+        self._ck(self.lib.dlmi_block_norm_fwd(self.ctx, kind, ctypes.byref(desc), B, H, _a(x), _a(u), _a(gate), _a(w_post),
+                                              _a(b_post), _a(w_pre), _a(b_pre), _a(y), _a(h)))
         return y, h
 
     def block_norm_bwd(self, desc, u, y, dy, dh, gate=None, w_post=None, b_post=None, w_pre=None, b_pre=None, dx=None, du=None,
                        dgate=None, grads=None, accumulate=False):
         """Its gradient (dlmi_block_norm_bwd).  Returns dict(dx, du, dgate, dw_post, db_post, dw_pre, db_pre), None for what
         is not there; grads: a dict of fp32 tensors for the last four (needed to accumulate), made where missing."""
-        assert u.dim() == 2
-        kind = self._type(u)
-        H = u.shape[1]
-        o = dict(dx=dx if dx is not None else self._out(u.dtype, *u.shape),
-                 du=du if du is not None else self._out(u.dtype, *u.shape),
-                 dgate=dgate if dgate is not None or gate is None else self._out(gate.dtype, *gate.shape))
-        for k, p in (("dw_post", w_post), ("db_post", b_post), ("dw_pre", w_pre), ("db_pre", b_pre)):
-            o[k] = (grads or {}).get(k)
-            if o[k] is None and p is not None:
-                assert not accumulate, "accumulating needs the gradients so far"
-                o[k] = self._out(self.torch.float32, H)
-        self._chk_block_norm(desc, u, dict(u=u, y=y, dy=dy, dh=dh, dx=o["dx"], du=o["du"]), gate,
-                             dict(w_post=w_post, b_post=b_post, w_pre=w_pre, b_pre=b_pre, dw_post=o["dw_post"],
-                                  db_post=o["db_post"], dw_pre=o["dw_pre"], db_pre=o["db_pre"]))
-        if o["dgate"] is not None and gate is not None:
-            self._chk_is(o["dgate"], "dgate", gate.dtype, *gate.shape)
+        B, H = u.shape
+        kind, dtype = self._type(u), u.dtype
+        dx = dx if dx is not None else self._out(dtype, B, H)
+        du = du if du is not None else self._out(dtype, B, H)
+        dgate = dgate if dgate is not None or gate is None else self._out(dtype, *gate.shape)
+        o = dict(dx=dx, du=du, dgate=dgate)
+        params = dict(dw_post=w_post, db_post=b_post, dw_pre=w_pre, db_pre=b_pre)
+        given = grads or {}
+        missing = [k for k, p in params.items() if p is not None and given.get(k) is None]
+        if missing:
+            assert not accumulate, "accumulating needs the gradients so far"
+            made = dict(zip(missing, self._out(self.torch.float32, len(missing), H).unbind(0)))
+        for k, p in params.items():
+            o[k] = made[k] if k in missing else given.get(k)
+            self._chk_is(p, k[1:], self.torch.float32, H)
+            self._chk_is(o[k], k, self.torch.float32, H)
+        for t, what in ((u, "u"), (y, "y"), (dy, "dy"), (dh, "dh"), (dx, "dx"), (du, "du")):
+            self._chk_is(t, what, dtype, B, H)
+        if gate is not None and desc.gate_rows:
+            rows = -(-B // desc.gate_rows)
+            self._chk_is(gate, "gate", dtype, rows, H)
+            self._chk_is(dgate, "dgate", dtype, rows, H)
         self._ck(self.lib.dlmi_block_norm_bwd(
-            self.ctx, kind, ctypes.byref(desc), c_sz(u.shape[0]), c_sz(H), _p(u), _p(y), _p(gate), _p(w_post), _p(b_post),
-            _p(w_pre), _p(dy), _p(dh), _p(o["dx"]), _p(o["du"]), _p(o["dgate"]), _p(o["dw_post"]), _p(o["db_post"]),
-            _p(o["dw_pre"]), _p(o["db_pre"]), c_int(1 if accumulate else 0)))
+            self.ctx, kind, ctypes.byref(desc), B, H, _a(u), _a(y), _a(gate), _a(w_post), _a(b_post), _a(w_pre), _a(dy), _a(dh),
+            _a(dx), _a(du), _a(dgate), _a(o["dw_post"]), _a(o["db_post"]), _a(o["dw_pre"]), _a(o["db_pre"]),
+            1 if accumulate else 0))
         return o

@@ -24,43 +24,85 @@ constexpr int kBnMaxWidth = DLMI_BLOCK_NORM_MAX_WIDTH;
 
 typedef float f32x4v __attribute__((ext_vector_type(4)));
 
-template <class T>
-constexpr int kBnVec = 16 / static_cast<int>(sizeof(T));  // elements of a 16-byte access
-
-template <class T>
+// N consecutive columns in one access, at any alignment (the hardware takes unaligned ones).
+template <class T, int N>
 struct __attribute__((packed, aligned(sizeof(T)))) BnVec {
-  T v[kBnVec<T>];
+  T v[N];
 };
 
-// 16 bytes at a time whatever the alignment of the row (the hardware takes unaligned 16-byte accesses).
-template <class T, int N>
-__device__ __forceinline__ void bn_load(T const *row, int col, int H, float (&o)[N]) {
-  if (col + N <= H) {
-    BnVec<T> const v = *reinterpret_cast<BnVec<T> const *>(row + col);
+// A thread's pieces of a row: C of them, N columns each, NT * N apart.  A piece that hangs over the row's end is moved back
+// to end with it, and its first `shift` columns, which belong to the thread before, are left alone: all loads are whole and
+// without conditions, which the compiler would wait behind (rows prefetched behind branches: 154 us against 129 us at
+// [8192 x 4096] FP32 forward).  H >= N.
+template <int N, int NT, int C>
+struct BnPlace {
+  int pos[C], shift[C];
+  bool tail;  // this wavefront has such a piece
+  __device__ __forceinline__ explicit BnPlace(int H) {
+    bool t = false;
 #pragma unroll
-    for (int i = 0; i < N; ++i) o[i] = static_cast<float>(v.v[i]);
-  } else {
+    for (int c = 0; c < C; ++c) {
+      int const col = (c * NT + static_cast<int>(threadIdx.x)) * N;
+      pos[c] = col < H - N ? col : H - N;
+      shift[c] = col - pos[c];
+      t = t || shift[c] != 0;
+    }
+    tail = __any(t);
+  }
+};
+
+template <class T, int N, int C>
+struct BnRaw {
+  BnVec<T, N> v[C];
+};
+
+template <class T, int N, int NT, int C>
+__device__ __forceinline__ void bn_fetch(BnRaw<T, N, C> &o, T const *row, BnPlace<N, NT, C> const &at) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) o[i] = col + i < H ? static_cast<float>(row[col + i]) : 0.0f;
+  for (int c = 0; c < C; ++c) o.v[c] = *reinterpret_cast<BnVec<T, N> const *>(row + at.pos[c]);
+}
+template <class T, int N, int NT, int C>
+__device__ __forceinline__ void bn_widen(float (&o)[C][N], BnRaw<T, N, C> const &r, BnPlace<N, NT, C> const &at) {
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[c][i] = static_cast<float>(r.v[c].v[i]);
+  if (at.tail) {
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int i = 0; i < N; ++i) o[c][i] = i >= at.shift[c] ? o[c][i] : 0.0f;
   }
 }
-template <class T, int N>
-__device__ __forceinline__ void bn_store(T *row, int col, int H, float const (&o)[N]) {
-  if (col + N <= H) {
-    BnVec<T> v;
+template <class T, int N, int NT, int C>
+__device__ __forceinline__ void bn_store(T *row, float const (&o)[C][N], BnPlace<N, NT, C> const &at) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v.v[i] = static_cast<T>(o[i]);
-    *reinterpret_cast<BnVec<T> *>(row + col) = v;
-  } else {
+  for (int c = 0; c < C; ++c) {
+    BnVec<T, N> v;
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (col + i < H) row[col + i] = static_cast<T>(o[i]);
+    for (int i = 0; i < N; ++i) v.v[i] = static_cast<T>(o[c][i]);
+    if (at.shift[c] == 0) {
+      *reinterpret_cast<BnVec<T, N> *>(row + at.pos[c]) = v;
+    } else {
+#pragma unroll
+      for (int i = 1; i < N; ++i)
+        if (i >= at.shift[c]) row[at.pos[c] + i] = v.v[i];
+    }
   }
 }
-template <int N>
-__device__ __forceinline__ void bn_param(float const *p, float dflt, int col, int H, float (&o)[N]) {
+template <int N, int NT, int C>
+__device__ __forceinline__ void bn_param(float const *p, float dflt, float (&o)[C][N], BnPlace<N, NT, C> const &at) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) o[i] = p != nullptr && col + i < H ? p[col + i] : dflt;
+  for (int c = 0; c < C; ++c)
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[c][i] = dflt;
+  if (p == nullptr) return;
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    BnVec<float, N> const v = *reinterpret_cast<BnVec<float, N> const *>(p + at.pos[c]);
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[c][i] = v.v[i];
+  }
 }
 
 // Sum over each 16 lanes, the same in all of them (DPP).
@@ -139,64 +181,31 @@ struct BnArgs {
   float rs, bs, eps_post, eps_pre;
 };
 
-// A row's 16-byte pieces of one thread, as they lie in memory.
-template <class T, int C>
-struct BnRaw {
-  BnVec<T> v[C];
-};
-
-template <class T, int NT, int C>
-__device__ __forceinline__ void bn_fetch(BnRaw<T, C> &o, T const *row, int H) {
-  constexpr int N = kBnVec<T>;
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    int const col = (c * NT + threadIdx.x) * N;
-    if (col + N <= H) {
-      o.v[c] = *reinterpret_cast<BnVec<T> const *>(row + col);
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) o.v[c].v[i] = col + i < H ? row[col + i] : static_cast<T>(0.0f);
-    }
-  }
-}
-template <class T, int C>
-__device__ __forceinline__ void bn_widen(float (&o)[C][kBnVec<T>], BnRaw<T, C> const &r) {
-#pragma unroll
-  for (int c = 0; c < C; ++c)
-#pragma unroll
-    for (int i = 0; i < kBnVec<T>; ++i) o[c][i] = static_cast<float>(r.v[c].v[i]);
-}
-
 #define BN_EACH                     \
   _Pragma("unroll") for (int c = 0; c < C; ++c) _Pragma("unroll") for (int i = 0; i < N; ++i)
-#define BN_IN ((c * NT + static_cast<int>(threadIdx.x)) * N + i < H)
+#define BN_IN (i >= at_.shift[c])
 
-template <class T, int NT, int C>
+template <class T, int N, int NT, int C>
 __global__ __launch_bounds__(NT) void k_block_norm_fwd(BnArgs a) {
-  constexpr int N = kBnVec<T>;
   __shared__ float lds[2][16][4];
   int flip = 0;
   int const H = a.H;
   float const inv_h = 1.0f / static_cast<float>(H);
-  BnRaw<T, C> ru, rx, rg;
+  BnPlace<N, NT, C> const at_(H);
+  BnRaw<T, N, C> ru, rx, rg;
   auto const fetch = [&](size_t r) {
     size_t const at = r * static_cast<size_t>(H);
-    bn_fetch<T, NT, C>(ru, static_cast<T const *>(a.u) + at, H);
-    bn_fetch<T, NT, C>(rx, static_cast<T const *>(a.x) + at, H);
-    if (a.gate_rows != 0)
-      bn_fetch<T, NT, C>(rg, static_cast<T const *>(a.gate) + (a.gate_rows == 1 ? r : r / a.gate_rows) * static_cast<size_t>(H), H);
+    bn_fetch(ru, static_cast<T const *>(a.u) + at, at_);
+    bn_fetch(rx, static_cast<T const *>(a.x) + at, at_);
+    if (a.gate_rows != 0) bn_fetch(rg, static_cast<T const *>(a.gate) + (a.gate_rows == 1 ? r : r / a.gate_rows) * static_cast<size_t>(H), at_);
   };
   if (blockIdx.x < a.B) fetch(blockIdx.x);
   float w1[C][N], b1[C][N], w2[C][N], b2[C][N];
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    int const col = (c * NT + threadIdx.x) * N;
-    bn_param(a.w_post, 1.0f, col, H, w1[c]);
-    bn_param(a.b_post, 0.0f, col, H, b1[c]);
-    bn_param(a.w_pre, 1.0f, col, H, w2[c]);
-    bn_param(a.b_pre, 0.0f, col, H, b2[c]);
-  }
-  // the columns beyond the row are zero; what centring makes of them stays out of the sums
+  bn_param(a.w_post, 1.0f, w1, at_);
+  bn_param(a.b_post, 0.0f, b1, at_);
+  bn_param(a.w_pre, 1.0f, w2, at_);
+  bn_param(a.b_pre, 0.0f, b2, at_);
+  // the columns that are another thread's are zero; what centring makes of them stays out of the sums
   auto const norm = [&](float (&v)[C][N], int how, float eps) {
     if (how == DLMI_ROW_NORM_NONE) return;
     if (how == DLMI_ROW_NORM_LAYER) {
@@ -215,9 +224,9 @@ __global__ __launch_bounds__(NT) void k_block_norm_fwd(BnArgs a) {
   for (size_t r = blockIdx.x; r < a.B; r += gridDim.x) {
     size_t const at = r * static_cast<size_t>(H);
     float u[C][N], x[C][N], g[C][N];
-    bn_widen(u, ru);
-    bn_widen(x, rx);
-    if (a.gate_rows != 0) bn_widen(g, rg);
+    bn_widen(u, ru, at_);
+    bn_widen(x, rx, at_);
+    if (a.gate_rows != 0) bn_widen(g, rg, at_);
     // the next row is on its way while this one is worked on (y may be x and h may be u: this row's only)
     if (r + gridDim.x < a.B) fetch(r + gridDim.x);
     norm(u, a.post, a.eps_post);
@@ -226,13 +235,11 @@ __global__ __launch_bounds__(NT) void k_block_norm_fwd(BnArgs a) {
       if (a.gate_rows != 0) n *= bn_gate(a.act, g[c][i]);
       x[c][i] = a.rs * x[c][i] + a.bs * n;
     }
-#pragma unroll
-    for (int c = 0; c < C; ++c) bn_store(static_cast<T *>(a.y) + at, (c * NT + threadIdx.x) * N, H, x[c]);
+    bn_store(static_cast<T *>(a.y) + at, x, at_);
     BN_EACH x[c][i] = BN_IN ? x[c][i] : 0.0f;
     norm(x, a.pre, a.eps_pre);
     BN_EACH x[c][i] = x[c][i] * w2[c][i] + b2[c][i];
-#pragma unroll
-    for (int c = 0; c < C; ++c) bn_store(static_cast<T *>(a.h) + at, (c * NT + threadIdx.x) * N, H, x[c]);
+    bn_store(static_cast<T *>(a.h) + at, x, at_);
   }
 }
 
@@ -243,36 +250,35 @@ enum { kBnNoGate = 0, kBnGateEach = 1, kBnGateShared = 2 };
 // A thread keeps its columns' sums and the row at hand and the next in registers; the weights (and a shared gate's f) it
 // reads again every row from LDS, which only it uses: with them in registers too, two workgroups of 8 wavefronts did not
 // fit a CU without spilling ([16384 x 4096] bf16, shared gate: 511 us then).
-template <class T, int NT, int C, int GATE, bool BIAS>
-__global__ __launch_bounds__(NT, NT <= 512 && C * kBnVec<T> <= 8 ? 4 : 1) void k_block_norm_bwd(BnArgs a) {
-  constexpr int N = kBnVec<T>, Q = C * N / 4;
-  constexpr bool kLds = C * N <= 8;  // wider rows read the weights from memory
+template <class T, int N, int NT, int C, int GATE, bool BIAS>
+__global__ __launch_bounds__(NT, NT <= 512 && C * N <= 8 ? 4 : 1) void k_block_norm_bwd(BnArgs a) {
+  constexpr int Q = N >= 4 ? C * N / 4 : 1;
+  constexpr bool kLds = N >= 4 && C * N <= 8;  // wider rows (and those of a few columns) read the weights from memory
   __shared__ float lds[2][16][4];
   __shared__ f32x4v kept[kLds ? 2 + (BIAS ? 1 : 0) + (GATE == kBnGateShared ? 1 : 0) : 1][kLds ? Q : 1][kLds ? NT : 1];
   constexpr int kW1 = 0, kW2 = 1, kF = 2, kB1 = GATE == kBnGateShared ? 3 : 2;
   int flip = 0;
   int const H = a.H;
   float const inv_h = 1.0f / static_cast<float>(H);
+  BnPlace<N, NT, C> const at_(H);
   auto const keep = [&](int k, float const (&v)[C][N]) {
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
-      int const c = q / (N / 4), i = q % (N / 4) * 4;
-      kept[k][q][threadIdx.x] = f32x4v{v[c][i], v[c][i + 1], v[c][i + 2], v[c][i + 3]};
+      f32x4v x;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = v[(q * 4 + j) / N][(q * 4 + j) % N];
+      kept[k][q][threadIdx.x] = x;
     }
   };
   auto const back = [&](int k, float (&v)[C][N]) {
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
-      int const c = q / (N / 4), i = q % (N / 4) * 4;
       f32x4v const x = kept[k][q][threadIdx.x];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[c][i + j] = x[j];
+      for (int j = 0; j < 4; ++j) v[(q * 4 + j) / N][(q * 4 + j) % N] = x[j];
     }
   };
-  auto const params = [&](float const *p, float dflt, float (&v)[C][N]) {
-#pragma unroll
-    for (int c = 0; c < C; ++c) bn_param(p, dflt, (c * NT + threadIdx.x) * N, H, v[c]);
-  };
+  auto const params = [&](float const *p, float dflt, float (&v)[C][N]) { bn_param(p, dflt, v, at_); };
   size_t r0, r1;
   if (a.direct) {
     r0 = blockIdx.x * a.rows_per_wg;
@@ -285,14 +291,14 @@ __global__ __launch_bounds__(NT, NT <= 512 && C * kBnVec<T> <= 8 ? 4 : 1) void k
   }
   if (r1 > a.B) r1 = a.B;
   bool const live_y = a.dh != nullptr && a.pre != DLMI_ROW_NORM_NONE;
-  BnRaw<T, C> ru, ry, rt, re, rg;
+  BnRaw<T, N, C> ru, ry, rt, re, rg;
   auto const fetch = [&](size_t r) {
     size_t const at = r * static_cast<size_t>(H);
-    bn_fetch<T, NT, C>(ru, static_cast<T const *>(a.u) + at, H);
-    if (live_y) bn_fetch<T, NT, C>(ry, static_cast<T const *>(a.y) + at, H);
-    if (a.dy != nullptr) bn_fetch<T, NT, C>(rt, static_cast<T const *>(a.dy) + at, H);
-    if (a.dh != nullptr) bn_fetch<T, NT, C>(re, static_cast<T const *>(a.dh) + at, H);
-    if constexpr (GATE == kBnGateEach) bn_fetch<T, NT, C>(rg, static_cast<T const *>(a.gate) + at, H);
+    bn_fetch(ru, static_cast<T const *>(a.u) + at, at_);
+    if (live_y) bn_fetch(ry, static_cast<T const *>(a.y) + at, at_);
+    if (a.dy != nullptr) bn_fetch(rt, static_cast<T const *>(a.dy) + at, at_);
+    if (a.dh != nullptr) bn_fetch(re, static_cast<T const *>(a.dh) + at, at_);
+    if constexpr (GATE == kBnGateEach) bn_fetch(rg, static_cast<T const *>(a.gate) + at, at_);
   };
   if (r0 < r1) fetch(r0);
   if constexpr (kLds) {
@@ -320,8 +326,8 @@ __global__ __launch_bounds__(NT, NT <= 512 && C * kBnVec<T> <= 8 ? 4 : 1) void k
       params(a.b_post, 0.0f, v);
   };
   auto const gate_row = [&](size_t r, float (&v)[C][N]) {
-    bn_fetch<T, NT, C>(rg, static_cast<T const *>(a.gate) + r / a.gate_rows * static_cast<size_t>(H), H);
-    bn_widen(v, rg);
+    bn_fetch(rg, static_cast<T const *>(a.gate) + r / a.gate_rows * static_cast<size_t>(H), at_);
+    bn_widen(v, rg, at_);
     BN_EACH v[c][i] = bn_gate(a.act, v[c][i]);
   };
   auto const shared_gate = [&](size_t r, float (&v)[C][N]) {
@@ -335,17 +341,17 @@ __global__ __launch_bounds__(NT, NT <= 512 && C * kBnVec<T> <= 8 ? 4 : 1) void k
   for (size_t r = r0; r < r1; ++r) {
     size_t const at = r * static_cast<size_t>(H);
     float u[C][N], y[C][N], t[C][N], e[C][N];
-    bn_widen(u, ru);
-    if (live_y) bn_widen(y, ry);
+    bn_widen(u, ru, at_);
+    if (live_y) bn_widen(y, ry, at_);
     if (a.dy != nullptr)
-      bn_widen(t, rt);
+      bn_widen(t, rt, at_);
     else
       BN_EACH t[c][i] = 0.0f;
     if (a.dh != nullptr)
-      bn_widen(e, re);
+      bn_widen(e, re, at_);
     else
       BN_EACH e[c][i] = 0.0f;
-    BnRaw<T, C> rgr;
+    BnRaw<T, N, C> rgr;
     if constexpr (GATE == kBnGateEach) rgr = rg;
     if constexpr (GATE == kBnGateShared && kLds) {
       if (r == r0 || r % a.gate_rows == 0) {
@@ -405,7 +411,7 @@ __global__ __launch_bounds__(NT, NT <= 512 && C * kBnVec<T> <= 8 ? 4 : 1) void k
     float f[C][N], b1[C][N];
     weight(kW1, w);
     if constexpr (GATE == kBnGateEach) {
-      bn_widen(f, rgr);
+      bn_widen(f, rgr, at_);
       BN_EACH f[c][i] = bn_gate(a.act, f[c][i]);
     }
     if constexpr (GATE == kBnGateShared) shared_gate(r, f);
@@ -431,20 +437,17 @@ __global__ __launch_bounds__(NT, NT <= 512 && C * kBnVec<T> <= 8 ? 4 : 1) void k
       t[c][i] *= a.rs;
       u[c][i] = uh;
     }
-#pragma unroll
-    for (int c = 0; c < C; ++c) bn_store(static_cast<T *>(a.dx) + at, (c * NT + threadIdx.x) * N, H, t[c]);
+bn_store(static_cast<T *>(a.dx) + at, t, at_);
     if (a.post != DLMI_ROW_NORM_NONE) {
       bn_sums<NT>(p, lds, flip);
       weight(kW1, w);
       float const c1 = a.post == DLMI_ROW_NORM_LAYER ? p[0] * inv_h : 0.0f, c2 = p[1] * inv_h;
       BN_EACH e[c][i] = ru_ * (e[c][i] * w[c][i] - c1 - u[c][i] * c2);
     }
-#pragma unroll
-    for (int c = 0; c < C; ++c) bn_store(static_cast<T *>(a.du) + at, (c * NT + threadIdx.x) * N, H, e[c]);
+bn_store(static_cast<T *>(a.du) + at, e, at_);
     if constexpr (GATE == kBnGateEach) {
       if (a.dgate != nullptr) {
-#pragma unroll
-        for (int c = 0; c < C; ++c) bn_store(static_cast<T *>(a.dgate) + at, (c * NT + threadIdx.x) * N, H, dg[c]);
+bn_store(static_cast<T *>(a.dgate) + at, dg, at_);
       }
     }
     if constexpr (GATE == kBnGateShared) {
@@ -453,8 +456,7 @@ __global__ __launch_bounds__(NT, NT <= 512 && C * kBnVec<T> <= 8 ? 4 : 1) void k
         BN_EACH dg[c][i] *= bn_gate_slope(a.act, f[c][i]);
         if (a.dgate != nullptr) {
           T *const out = static_cast<T *>(a.dgate) + r / a.gate_rows * static_cast<size_t>(H);
-#pragma unroll
-          for (int c = 0; c < C; ++c) bn_store(out, (c * NT + threadIdx.x) * N, H, dg[c]);
+bn_store(out, dg, at_);
         }
         BN_EACH dg[c][i] = 0.0f;
       }
@@ -464,10 +466,7 @@ __global__ __launch_bounds__(NT, NT <= 512 && C * kBnVec<T> <= 8 ? 4 : 1) void k
   float *const out = a.partial + static_cast<size_t>(blockIdx.x) * a.planes * H;
   auto const leave = [&](int plane, float const (&v)[C][N]) {
     if (plane < 0) return;
-    BN_EACH {
-      int const col = (c * NT + threadIdx.x) * N + i;
-      if (col < H) out[static_cast<size_t>(plane) * H + col] = v[c][i];
-    }
+    bn_store(out + static_cast<size_t>(plane) * H, v, at_);
   };
   leave(a.plane[0], dw1);
   if constexpr (BIAS) leave(a.plane[1], db1);
@@ -527,45 +526,63 @@ __global__ __launch_bounds__(1024) void k_block_norm_reduce(BnReduce a, unsigned
     static_cast<T *>(a.dgate)[static_cast<size_t>(blockIdx.y - params) * a.H + col] = static_cast<T>(s);
 }
 
-template <class T, int NT, int C, int GATE>
+template <class T, int N, int NT, int C, int GATE>
 static void bn_launch_bwd(dlmi_ctx *ctx, BnArgs const &a, unsigned blocks) {
   if (a.b_post != nullptr || a.plane[1] >= 0 || a.plane[3] >= 0)
-    hipLaunchKernelGGL((k_block_norm_bwd<T, NT, C, GATE, true>), dim3(blocks), dim3(NT), 0, ctx->stream, a);
+    hipLaunchKernelGGL((k_block_norm_bwd<T, N, NT, C, GATE, true>), dim3(blocks), dim3(NT), 0, ctx->stream, a);
   else
-    hipLaunchKernelGGL((k_block_norm_bwd<T, NT, C, GATE, false>), dim3(blocks), dim3(NT), 0, ctx->stream, a);
+    hipLaunchKernelGGL((k_block_norm_bwd<T, N, NT, C, GATE, false>), dim3(blocks), dim3(NT), 0, ctx->stream, a);
 }
 
-template <class T, int NT, int C>
-static void bn_launch(dlmi_ctx *ctx, bool back, BnArgs const &a, unsigned blocks) {
-  if (!back)
-    hipLaunchKernelGGL((k_block_norm_fwd<T, NT, C>), dim3(blocks), dim3(NT), 0, ctx->stream, a);
+template <class T, int N, int NT, int C, bool BACK>
+static void bn_launch(dlmi_ctx *ctx, BnArgs const &a, unsigned blocks) {
+  if constexpr (!BACK)
+    hipLaunchKernelGGL((k_block_norm_fwd<T, N, NT, C>), dim3(blocks), dim3(NT), 0, ctx->stream, a);
   else if (a.gate_rows == 0)
-    bn_launch_bwd<T, NT, C, kBnNoGate>(ctx, a, blocks);
+    bn_launch_bwd<T, N, NT, C, kBnNoGate>(ctx, a, blocks);
   else if (a.gate_rows == 1)
-    bn_launch_bwd<T, NT, C, kBnGateEach>(ctx, a, blocks);
+    bn_launch_bwd<T, N, NT, C, kBnGateEach>(ctx, a, blocks);
   else
-    bn_launch_bwd<T, NT, C, kBnGateShared>(ctx, a, blocks);
+    bn_launch_bwd<T, N, NT, C, kBnGateShared>(ctx, a, blocks);
 }
 
-// Threads of a row: 8 columns each, up to 1024 threads; wider rows 16 columns each.
-static int bn_threads(int H) {
+// Threads of a row: `each` columns each, up to 1024 threads.
+static int bn_threads(int H, int each) {
   int nt = 64;
-  while (nt < 1024 && nt * 8 < H) nt *= 2;
+  while (nt < 1024 && nt * each < H) nt *= 2;
   return nt;
 }
+// Columns of a thread: 8, but 4 in the fp32 backward, whose rows at hand and next take twice the registers of bf16's (with 8
+// they spilled).  Rows wider than 1024 threads of these take two or four times as many.
+static int bn_each(dlmi_dtype type, bool back) { return back && type == DLMI_F32 ? 4 : 8; }
 
-template <class T>
-static void bn_dispatch(dlmi_ctx *ctx, bool back, BnArgs const &a, unsigned blocks) {
-  constexpr int C = 8 / kBnVec<T>;
-  switch (bn_threads(a.H)) {
-    case 64: return bn_launch<T, 64, C>(ctx, back, a, blocks);
-    case 128: return bn_launch<T, 128, C>(ctx, back, a, blocks);
-    case 256: return bn_launch<T, 256, C>(ctx, back, a, blocks);
-    case 512: return bn_launch<T, 512, C>(ctx, back, a, blocks);
-    default:
-      if (a.H <= 8192) return bn_launch<T, 1024, C>(ctx, back, a, blocks);
-      return bn_launch<T, 1024, 2 * C>(ctx, back, a, blocks);
+template <class T, int C, bool BACK>
+static void bn_dispatch_each(dlmi_ctx *ctx, BnArgs const &a, unsigned blocks) {
+  constexpr int N = 16 / static_cast<int>(sizeof(T));  // 16-byte accesses
+  if (a.H < N) return bn_launch<T, 1, 64, 1, BACK>(ctx, a, blocks);
+  switch (bn_threads(a.H, C * N)) {
+    case 64: return bn_launch<T, N, 64, C, BACK>(ctx, a, blocks);
+    case 128: return bn_launch<T, N, 128, C, BACK>(ctx, a, blocks);
+    case 256: return bn_launch<T, N, 256, C, BACK>(ctx, a, blocks);
+    case 512: return bn_launch<T, N, 512, C, BACK>(ctx, a, blocks);
+    default: break;
   }
+  if (a.H <= 1024 * C * N) return bn_launch<T, N, 1024, C, BACK>(ctx, a, blocks);
+  if constexpr (C * N < 8) {
+    if (a.H <= 8192) return bn_launch<T, N, 1024, 8 / N, BACK>(ctx, a, blocks);
+  }
+  return bn_launch<T, N, 1024, 16 / N, BACK>(ctx, a, blocks);
+}
+
+static void bn_dispatch(dlmi_ctx *ctx, dlmi_dtype type, bool back, BnArgs const &a, unsigned blocks) {
+  if (type == DLMI_BF16 && back)
+    bn_dispatch_each<__bf16, 1, true>(ctx, a, blocks);
+  else if (type == DLMI_BF16)
+    bn_dispatch_each<__bf16, 1, false>(ctx, a, blocks);
+  else if (back)
+    bn_dispatch_each<float, 1, true>(ctx, a, blocks);
+  else
+    bn_dispatch_each<float, 2, false>(ctx, a, blocks);
 }
 
 static char const *bn_check(dlmi_block_norm_desc const *d, size_t B, size_t H, void const *gate, float const *w_post,
@@ -626,12 +643,9 @@ int dlmi_block_norm_fwd(dlmi_ctx *ctx, dlmi_dtype type, dlmi_block_norm_desc con
   a.b_pre = b_pre;
   a.y = y;
   a.h = h;
-  size_t blocks = static_cast<size_t>(ctx->num_cu) * (2048 / bn_threads(a.H));
+  size_t blocks = static_cast<size_t>(ctx->num_cu) * (2048 / bn_threads(a.H, bn_each(type, false)));
   if (blocks > B) blocks = B;
-  if (type == DLMI_F32)
-    bn_dispatch<float>(ctx, false, a, static_cast<unsigned>(blocks));
-  else
-    bn_dispatch<__bf16>(ctx, false, a, static_cast<unsigned>(blocks));
+  bn_dispatch(ctx, type, false, a, static_cast<unsigned>(blocks));
   DLMI_LAUNCH_CHECK(ctx, "k_block_norm_fwd");
   return DLMI_OK;
 }
@@ -670,7 +684,7 @@ int dlmi_block_norm_bwd(dlmi_ctx *ctx, dlmi_dtype type, dlmi_block_norm_desc con
   unsigned const sums = static_cast<unsigned>(a.planes);
   // as many workgroups as run at once (16 wavefronts per CU), but at least 4 rows each where there are sums: a workgroup
   // leaves a row of partial sums per plane
-  size_t const nt = static_cast<size_t>(bn_threads(a.H));
+  size_t const nt = static_cast<size_t>(bn_threads(a.H, bn_each(type, true)));
   size_t const most = static_cast<size_t>(ctx->num_cu) * (nt < 1024 ? 1024 / nt : 1);
   size_t want = dlmi_ceil_div(B, most);
   if ((sums != 0 || desc->gate_rows > 1) && want < 4) want = 4;
@@ -694,10 +708,7 @@ int dlmi_block_norm_bwd(dlmi_ctx *ctx, dlmi_dtype type, dlmi_block_norm_desc con
     if (rc != DLMI_OK) return rc;
     a.partial = reinterpret_cast<float *>(dlmi_scratch_data(ctx));
   }
-  if (type == DLMI_F32)
-    bn_dispatch<float>(ctx, true, a, static_cast<unsigned>(blocks));
-  else
-    bn_dispatch<__bf16>(ctx, true, a, static_cast<unsigned>(blocks));
+  bn_dispatch(ctx, type, true, a, static_cast<unsigned>(blocks));
   DLMI_LAUNCH_CHECK(ctx, "k_block_norm_bwd");
   if (a.partial == nullptr) return DLMI_OK;
   // (without dh nothing was added up for the norm before the next block: the kernel left zeros)
