@@ -212,19 +212,21 @@ struct CeLogits {
   size_t v0, vn;                     // first class of the piece, classes in it
 };
 
-// z of one 32 x 32 block; classes beyond the piece are -infinity.
-template <int T>
-__device__ __forceinline__ f32x16 ce_block_logits(CeArgs const &a, CeLogits const &g, f32x16 v, size_t c0, float ux, float uw, int lane) {
+// The biases of a lane's 16 classes of a 32-class block from c0 on; -infinity beyond the piece, which makes the logit that.
+// (Every load is made, of the last class at most: loads behind conditions of their own would each be waited for.)
+__device__ __forceinline__ f32x16 ce_biases(CeArgs const &a, CeLogits const &g, size_t c0, int lane) {
+  f32x16 v = {};
+  size_t const c1 = c0 + 4 * (lane >> 5);
+  if (a.bias != nullptr) {
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    size_t const c = c0 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
-    float z = v[r] * ux * uw;
-    if (c < g.vn) {
-      if (a.bias != nullptr) z += a.bias[g.v0 + c];
-    } else {
-      z = -INFINITY;
+    for (int r = 0; r < 16; ++r) {
+      size_t const c = c1 + 8 * (r >> 2) + (r & 3);
+      v[r] = a.bias[g.v0 + (c < g.vn ? c : g.vn - 1)];
     }
-    v[r] = z;
+  }
+  if (c0 + 32 > g.vn) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) v[r] = c1 + 8 * (r >> 2) + (r & 3) < g.vn ? v[r] : -INFINITY;
   }
   return v;
 }
@@ -242,18 +244,27 @@ __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_stats(CeArgs a, Ce
   int const lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   float const uw = g.unscale_w[0];
   size_t const c0 = static_cast<size_t>(ti) * T + (wave >> 1) * (T / 2);
+  size_t const b0 = static_cast<size_t>(tj) * T + (wave & 1) * (T / 2) + (lane & 31);
+  float ux[H::kNB];
+#pragma unroll
+  for (int n = 0; n < H::kNB; ++n) ux[n] = g.unscale_x[b0 + n * 32 < a.B ? b0 + n * 32 : a.B - 1];
+#pragma unroll
+  for (int m = 0; m < H::kMB; ++m) {
+    f32x16 const bias = ce_biases(a, g, c0 + m * 32, lane);
+#pragma unroll
+    for (int n = 0; n < H::kNB; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc.v[m][n][r] = acc.v[m][n][r] * ux[n] * uw + bias[r];
+  }
 #pragma unroll
   for (int n = 0; n < H::kNB; ++n) {
-    size_t const b = static_cast<size_t>(tj) * T + (wave & 1) * (T / 2) + n * 32 + (lane & 31);
+    size_t const b = b0 + n * 32;
     bool const in = b < a.B;
-    float const ux = in ? g.unscale_x[b] : 0.0f;
     float top = -INFINITY;
 #pragma unroll
-    for (int m = 0; m < H::kMB; ++m) {
-      acc.v[m][n] = ce_block_logits<T>(a, g, acc.v[m][n], c0 + m * 32, ux, uw, lane);
+    for (int m = 0; m < H::kMB; ++m)
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, acc.v[m][n][r]);
-    }
     float sum = 0.0f;
     float const base = top > -INFINITY ? top : 0.0f;
 #pragma unroll
@@ -514,7 +525,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_ce_direct(CeArgs a, float2 *part
   }
   // The first wavefront alone writes what other workgroups read, past the caches (device scope), waits until that is done
   // and takes a ticket; who draws the last one reads it all, past the caches as well.  A release and acquire instead would
-  // write back and empty the L2 for every workgroup: 17.6 us against 13.4 us for 4 rows, 512 features, 10007 classes.
+  // write back and empty the L2 for every workgroup.
   if (wave == 0) {
     if (lane < NB * RB && static_cast<size_t>(lane) < a.B)
       __hip_atomic_store(reinterpret_cast<unsigned long long *>(part + static_cast<size_t>(blockIdx.x) * a.B + lane),
@@ -537,7 +548,11 @@ __global__ __launch_bounds__(NW * 64, 2) void k_ce_direct(CeArgs a, float2 *part
   int const slices = NW * 64 / wide, b = static_cast<int>(threadIdx.x) & (wide - 1), slice = static_cast<int>(threadIdx.x) / wide;
   float2 *const tree = reinterpret_cast<float2 *>(&red[0][0][0][0]);
   float2 p = make_float2(-INFINITY, 0.0f);
+  int label = -1;
+  float chosen = 0.0f;
   if (static_cast<size_t>(b) < a.B) {
+    label = a.labels[b];
+    if (label >= 0 && static_cast<size_t>(label) < a.V) chosen = __hip_atomic_load(&target[b], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     auto const at = [&](unsigned q) {
       unsigned long long const o =
           __hip_atomic_load(reinterpret_cast<unsigned long long *>(part + static_cast<size_t>(q) * a.B + b), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -565,8 +580,41 @@ __global__ __launch_bounds__(NW * 64, 2) void k_ce_direct(CeArgs a, float2 *part
   if (slice != 0 || static_cast<size_t>(b) >= a.B) return;
   float const lse = p.x + logf(p.y);
   a.lse[b] = lse;
-  int const l = a.labels[b];
-  a.loss[b] = l >= 0 && static_cast<size_t>(l) < a.V ? lse - __hip_atomic_load(&target[b], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0f;
+  a.loss[b] = label >= 0 && static_cast<size_t>(label) < a.V ? lse - chosen : 0.0f;
+}
+
+// The sums over the 32 lanes of a half wavefront of its 16 values each, scattered: lanes halve what they hold with a partner
+// (16, 8 and 4 lanes away, then in mirrored fours) until one value is left, which the neighbour shares.  Value
+// ce_scatter_row(lane) ends up in the lane.
+template <int CTRL>
+__device__ __forceinline__ float ce_dpp(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false));
+}
+__device__ __forceinline__ int ce_scatter_row(int lane) { return (lane >> 4 & 1) * 8 + (lane >> 3 & 1) * 4 + (lane >> 2 & 1) * 2 + (lane >> 1 & 1); }
+__device__ __forceinline__ float ce_scatter_sum(f32x16 const &v, int lane) {
+  float a[8], b[4], c[2];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    unsigned const lo = __float_as_uint(v[i]), hi = __float_as_uint(v[i + 8]);
+    // rows of 16 lanes: the even one keeps the low values of both, the odd one the high
+    auto const x = __builtin_amdgcn_permlane16_swap(lo, hi, false, false);
+    a[i] = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+  }
+  bool const up8 = lane & 8, up4 = lane & 4, up2 = lane & 2;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float const keep = up8 ? a[i + 4] : a[i], give = up8 ? a[i] : a[i + 4];
+    b[i] = keep + ce_dpp<0x128>(give);  // lane ^ 8: rotated by 8 in 16
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    float const keep = up4 ? b[i + 2] : b[i], give = up4 ? b[i] : b[i + 2];
+    // lane ^ 4: mirrored in 8 (lane ^ 7), then in 4 (lane ^ 3)
+    c[i] = keep + ce_dpp<0x1B>(ce_dpp<0x141>(give));
+  }
+  float const keep = up2 ? c[1] : c[0], give = up2 ? c[0] : c[1];
+  float const d = keep + ce_dpp<0x4E>(give);  // lane ^ 2
+  return d + ce_dpp<0xB1>(d);                 // lane ^ 1
 }
 
 // dL of a tile, packed for dX (rows of the batch, k = classes) and for dW (rows are classes, k = rows of the batch);
@@ -586,51 +634,48 @@ __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_grad(CeArgs a, CeL
   size_t const c0 = static_cast<size_t>(ti) * T + (wave >> 1) * (T / 2);
   size_t const b0 = static_cast<size_t>(tj) * T + (wave & 1) * (T / 2);
   size_t const rb = static_cast<size_t>(kblocks_v) * NP * kFragBytes, rv = static_cast<size_t>(kblocks_b) * NP * kFragBytes;
-  float dsum[H::kMB];
-#pragma unroll
-  for (int m = 0; m < H::kMB; ++m) dsum[m] = 0.0f;
+  // of this lane's rows of the batch: unscale, lse, weight, and the label's class from c0 on (-1: none here)
+  float ux[H::kNB], lse[H::kNB], weight[H::kNB];
+  int at[H::kNB];
+  bool live[H::kNB];
 #pragma unroll
   for (int n = 0; n < H::kNB; ++n) {
-    size_t const b = b0 + n * 32 + (lane & 31);
-    bool const in = b < a.B;
-    float const ux = in ? g.unscale_x[b] : 0.0f;
-    int const label = in ? a.labels[b] : -1;
-    bool const live = label >= 0 && static_cast<size_t>(label) < a.V;
-    float const lse = live ? a.lse_in[b] : 0.0f;
-    long long const at = static_cast<long long>(label) - static_cast<long long>(g.v0 + c0);
+    size_t const b = b0 + n * 32 + (lane & 31), in = b < a.B ? b : a.B - 1;
+    int const label = a.labels[in];
+    ux[n] = g.unscale_x[in];
+    lse[n] = a.lse_in[in];
+    weight[n] = DB && a.dloss != nullptr ? a.dloss[in] : 1.0f;
+    live[n] = b < a.B && label >= 0 && static_cast<size_t>(label) < a.V;
+    long long const c = static_cast<long long>(label) - static_cast<long long>(g.v0 + c0);
+    at[n] = live[n] && c >= 0 && c < T / 2 ? static_cast<int>(c) : -1;
+  }
 #pragma unroll
-    for (int m = 0; m < H::kMB; ++m) {
-      f32x16 z = ce_block_logits<T>(a, g, acc.v[m][n], c0 + m * 32, ux, uw, lane);
+  for (int m = 0; m < H::kMB; ++m) {
+    f32x16 const bias = ce_biases(a, g, c0 + m * 32, lane);
+    f32x16 sum = {};
+    bool const whole = c0 + m * 32 + 32 <= g.vn;
+#pragma unroll
+    for (int n = 0; n < H::kNB; ++n) {
+      f32x16 z = acc.v[m][n];
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        float p = __expf(z[r] - lse);
-        if (at == m * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3)) p -= 1.0f;
-        // (a class beyond the piece: z is -infinity, but a row's lse may be too)
-        z[r] = live && c0 + m * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3) < g.vn ? p * kCeDl : 0.0f;
+        int const c = m * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+        float p = __expf(z[r] * ux[n] * uw + bias[r] - lse[n]);
+        p -= at[n] == c ? 1.0f : 0.0f;
+        // (a class beyond the piece: its logit is -infinity, but a row's lse may be too)
+        z[r] = live[n] && (whole || c0 + c < g.vn) ? p : 0.0f;
+        if constexpr (DB) sum[r] += live[n] ? weight[n] * z[r] : 0.0f;
       }
       size_t const ib = c0 / 32 + m, jb = b0 / 32 + n;
-      HalfBlock<NP> const blk = half_split<NP>(z);
+      HalfBlock<NP> const blk = half_split<NP>(z * kCeDl);
       half_store<NP>(dlb + jb * rb + ib * 2 * NP * kFragBytes, blk, lane);
-      HalfBlock<NP> const flip = half_flip<NP>(blk, id0, id1);
-      half_store<NP>(dlv + ib * rv + jb * 2 * NP * kFragBytes, flip, lane);
-      if constexpr (DB) {
-        // the transposed block in fp32 (22 bits): a lane has a class, 16 rows of the batch
-        HalfBlock<2> const two = half_split<2>(z);
-        f32x16 const t = half_transposed(two.pl[0], id0, id1) + half_transposed(two.pl[1], id0, id1);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          size_t const bb = b0 + n * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
-          float const w = bb < a.B ? ce_row_weight(a, bb) : 0.0f;
-          dsum[m] += bb < a.B ? w * t[r] : 0.0f;
-        }
-      }
+      half_store<NP>(dlv + ib * rv + jb * 2 * NP * kFragBytes, half_flip<NP>(blk, id0, id1), lane);
     }
-  }
-  if constexpr (DB) {
-#pragma unroll
-    for (int m = 0; m < H::kMB; ++m) {
-      float const s = dsum[m] + __shfl_xor(dsum[m], 32);
-      if (lane < 32) dbpart[(tj * 2 + (wave & 1)) * dbpart_stride + c0 + m * 32 + lane] = s * (1.0f / kCeDl);
+    if constexpr (DB) {
+      float const s = ce_scatter_sum(sum, lane);
+      int const r = ce_scatter_row(lane);
+      if ((lane & 1) == 0)
+        dbpart[(tj * 2 + (wave & 1)) * dbpart_stride + c0 + m * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3)] = s;
     }
   }
 }
