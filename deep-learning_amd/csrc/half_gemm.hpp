@@ -115,6 +115,39 @@ __device__ __forceinline__ void half_stage_wait() {
   asm volatile("" ::: "memory");
 }
 
+// The order of a k block's instructions: the next block's LDS reads and the next stages' loads spread between the matrix
+// instructions.  Left to itself the compiler puts them behind most of these, and the loads right before the next wait: 246
+// us against 221 us for 8192 x 8192 x 2048 in one plane (1242 TFLOP/s), 623 against 603 us in two (1368 TFLOP/s), 50 against
+// 45 us for 2048^3 in two planes with 128 x 128 tiles.  One plane of a 256 x 256 tile has few matrix instructions per read
+// and does best with all reads first (221 against 224 us); everything else with reads and loads spread alike.
+template <class T, bool LOADS>
+__device__ __forceinline__ void half_schedule() {
+  constexpr int kMfma = 0x008, kLoad = 0x020, kRead = 0x100;
+  constexpr int NM = T::kMB * T::kNB * (T::kPlanes == 2 ? 3 : 1), NR = (T::kMB + T::kNB) * T::kPlanes;
+  if constexpr (T::kPlanes == 1 && T::kMB == 4) {
+    __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+      __builtin_amdgcn_sched_group_barrier(kRead, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+    }
+    if constexpr (LOADS) {
+#pragma unroll
+      for (int i = 0; i < T::kLoads; ++i) {
+        __builtin_amdgcn_sched_group_barrier(kLoad, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+      if (LOADS && i < T::kLoads) __builtin_amdgcn_sched_group_barrier(kLoad, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(kRead, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(kMfma, NM / NR, 0);
+    }
+  }
+}
+
 // The K loop of one workgroup (256 threads, wavefronts 2 x 2) over `stages` >= 1 stages.  P, Q: the first fragment of the
 // tile's first row block at the first k block; row_stride_*: bytes from one row block to the next.
 template <int BM, int BN, int NP>
@@ -159,6 +192,7 @@ __device__ __forceinline__ void half_gemm(HalfAcc<HalfTile<BM, BN, NP>> &acc, ch
     for (int u = 0; u < 4; ++u) {
 #pragma unroll
       for (int ks = 0; ks < T::KS; ++ks) {
+        __builtin_amdgcn_sched_barrier(0);
         if (ks + 1 < T::KS) {
           half_frags_read<T>(nxt, bufs[u], ks + 1, wm, wn, lane);
         } else {
@@ -168,6 +202,11 @@ __device__ __forceinline__ void half_gemm(HalfAcc<HalfTile<BM, BN, NP>> &acc, ch
         }
         half_mfma<T>(acc, cur);
         cur = nxt;
+        if (ks + 1 == T::KS)
+          half_schedule<T, true>();
+        else
+          half_schedule<T, false>();
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
   }

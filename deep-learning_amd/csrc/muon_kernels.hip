@@ -168,6 +168,11 @@ struct MuonOut {
   float wd;
 };
 
+template <int MODE>
+__device__ __forceinline__ float muon_new(float w, float x, float lr, float wd) {
+  return MODE == kMuonStep ? w - (lr * x + wd * w) : x;
+}
+
 // A tile of X' = a X + Bm X; XT = X^T packed (row j, k = i).  MORE: written packed both ways; OUT, STEP: the last of the
 // iteration, written to the caller's matrix.
 template <int T, int MODE, class O>
@@ -197,18 +202,27 @@ __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_muon_update(char cons
       } else {
         v *= 1.0f / kMuonScale;
         O *const p = static_cast<O *>(b.p[mat]);
-        unsigned const j = jb * 32 + (lane & 31);
+        size_t const j = jb * 32 + (lane & 31), i0 = ib * 32 + 4 * (lane >> 5);
+        size_t const si = o.flipped ? 1 : o.cols, sj = o.flipped ? o.cols : 1;
+        unsigned const rows = o.flipped ? o.cols : o.rows, cols = o.flipped ? o.rows : o.cols;  // of X
+        float const lr = MODE == kMuonStep ? b.lr[mat] : 0.0f;
+        // (a block inside the matrix has no conditions between its loads, which would each be waited for)
+        if (ib * 32 + 32 <= rows && jb * 32 + 32 <= cols) {
+          O *const q = p + i0 * si + j * sj;
+          f32x16 w = {};
+          if constexpr (MODE == kMuonStep) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          unsigned const i = ib * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
-          unsigned const row = o.flipped ? j : i, col = o.flipped ? i : j;
-          if (row < o.rows && col < o.cols) {
-            size_t const at = static_cast<size_t>(row) * o.cols + col;
-            if constexpr (MODE == kMuonStep) {
-              float const w = static_cast<float>(p[at]);
-              p[at] = static_cast<O>(w - (b.lr[mat] * v[r] + o.wd * w));
-            } else {
-              p[at] = static_cast<O>(v[r]);
+            for (int r = 0; r < 16; ++r) w[r] = static_cast<float>(q[(8 * (r >> 2) + (r & 3)) * si]);
+          }
+#pragma unroll
+          for (int r = 0; r < 16; ++r) q[(8 * (r >> 2) + (r & 3)) * si] = static_cast<O>(muon_new<MODE>(w[r], v[r], lr, o.wd));
+        } else {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            size_t const i = i0 + 8 * (r >> 2) + (r & 3);
+            if (i < rows && j < cols) {
+              O *const q = p + i * si + j * sj;
+              *q = static_cast<O>(muon_new<MODE>(MODE == kMuonStep ? static_cast<float>(*q) : 0.0f, v[r], lr, o.wd));
             }
           }
         }

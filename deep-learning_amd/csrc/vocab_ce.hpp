@@ -43,7 +43,7 @@ int ce_backward(dlmi_ctx *ctx, CeArgs const &a);
 #ifdef DLMI_CE_IMPLEMENTATION
 
 constexpr int kCeBlock = 256;
-constexpr unsigned kCeMaxParts = 256;     // partial maxima of a piece of W
+constexpr unsigned kCeMaxParts = 1024;     // partial maxima of a piece of W
 constexpr float kCeDl = 32768.0f;         // dL is held times this
 
 template <class T>
@@ -125,7 +125,12 @@ __global__ __launch_bounds__(kCeBlock) void k_ce_pack(CeArgs a, T const *src, si
   int const lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   float scale = 1.0f;
   if (parts != nullptr) {
-    float m = threadIdx.x < nparts ? parts[threadIdx.x] : 0.0f;
+    float m = 0.0f;
+#pragma unroll
+    for (unsigned q = 0; q < kCeMaxParts / kCeBlock; ++q) {
+      unsigned const at = q * kCeBlock + threadIdx.x;
+      m = fmaxf(m, at < nparts ? parts[at] : 0.0f);
+    }
     m = ce_wave_max(m);
     if (lane == 0) lds[wave] = m;
     __syncthreads();
@@ -689,6 +694,33 @@ static __global__ __launch_bounds__(kCeBlock) void k_ce_db(float const *part, si
   db[c] = accumulate ? db[c] + s : s;
 }
 
+// A 32 x 32 block of a product into row-major out [rows][cols] at (i0, j0), times `factor`, added to what is there or not.
+// (A block inside has no conditions between its loads, which would each be waited for.)
+template <class O>
+__device__ __forceinline__ void ce_block_out(f32x16 const &v, float factor, O *out, size_t i0, size_t j0, size_t rows, size_t cols, bool add,
+                                             int lane) {
+  size_t const j = j0 + (lane & 31), i = i0 + 4 * (lane >> 5);
+  if (i0 + 32 <= rows && j0 + 32 <= cols) {
+    O *const p = out + i * cols + j;
+    f32x16 w = {};
+    if (add) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) w[r] = static_cast<float>(p[(8 * (r >> 2) + (r & 3)) * cols]);
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) p[(8 * (r >> 2) + (r & 3)) * cols] = static_cast<O>(w[r] + v[r] * factor);
+  } else {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      size_t const at = i + 8 * (r >> 2) + (r & 3);
+      if (at < rows && j < cols) {
+        O *const p = out + at * cols + j;
+        *p = static_cast<O>((add ? static_cast<float>(*p) : 0.0f) + v[r] * factor);
+      }
+    }
+  }
+}
+
 // dW of a piece: classes i (P = dL packed by classes), features j (Q = dloss X packed by features), times `scale`.
 template <int T, int NP, class O>
 __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_dw(char const *P, char const *Q, unsigned ni, unsigned nj, unsigned kblocks,
@@ -701,23 +733,13 @@ __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_dw(char const *P, 
   HalfAcc<H> acc;
   half_gemm<T, T, NP>(acc, P + ti * (T / 32) * rs, Q + tj * (T / 32) * rs, rs, rs, stages);
   int const lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  float const us = unscale[0];
+  float const factor = unscale[0] * (scale * (1.0f / kCeDl));
 #pragma unroll
   for (int m = 0; m < H::kMB; ++m)
 #pragma unroll
-    for (int n = 0; n < H::kNB; ++n) {
-      size_t const j = static_cast<size_t>(tj) * T + (wave & 1) * (T / 2) + n * 32 + (lane & 31);
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        size_t const i = static_cast<size_t>(ti) * T + (wave >> 1) * (T / 2) + m * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
-        if (i < rows && j < cols) {
-          O *const p = out + i * cols + j;
-          float v = acc.v[m][n][r] * (1.0f / kCeDl) * us * scale;
-          if (accumulate) v += static_cast<float>(*p);
-          *p = static_cast<O>(v);
-        }
-      }
-    }
+    for (int n = 0; n < H::kNB; ++n)
+      ce_block_out(acc.v[m][n], factor, out, static_cast<size_t>(ti) * T + (wave >> 1) * (T / 2) + m * 32,
+                   static_cast<size_t>(tj) * T + (wave & 1) * (T / 2) + n * 32, rows, cols, accumulate != 0, lane);
 }
 
 // A slice of a piece's share of dX: rows of the batch i (P = dL packed by rows), features j (Q = W packed by features), summed
@@ -737,39 +759,36 @@ __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_dx(char const *P, 
   HalfAcc<H> acc;
   half_gemm<T, T, NP>(acc, P + ti * (T / 32) * rs + skip, Q + tj * (T / 32) * rs + skip, rs, rs, count);
   int const lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  float const us = unscale[0];
+  float const factor = unscale[0] * (1.0f / kCeDl);
   out += slice * rows * cols;
 #pragma unroll
   for (int m = 0; m < H::kMB; ++m)
 #pragma unroll
-    for (int n = 0; n < H::kNB; ++n) {
-      size_t const j = static_cast<size_t>(tj) * T + (wave & 1) * (T / 2) + n * 32 + (lane & 31);
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        size_t const i = static_cast<size_t>(ti) * T + (wave >> 1) * (T / 2) + m * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
-        if (i < rows && j < cols) {
-          float const v = acc.v[m][n][r] * (1.0f / kCeDl) * us;
-          float *const p = out + i * cols + j;
-          *p = first ? v : *p + v;
-        }
-      }
-    }
+    for (int n = 0; n < H::kNB; ++n)
+      ce_block_out(acc.v[m][n], factor, out, static_cast<size_t>(ti) * T + (wave >> 1) * (T / 2) + m * 32,
+                   static_cast<size_t>(tj) * T + (wave & 1) * (T / 2) + n * 32, rows, cols, first == 0, lane);
 }
 
-// dX = scale dloss sum over slices, rows left out zero.
+// dX = scale dloss sum over slices, rows left out zero.  A workgroup per row and 1024 features.
 template <class O>
 __global__ __launch_bounds__(kCeBlock) void k_ce_dx_finish(CeArgs a, float const *acc, unsigned slices, O *dX) {
+  size_t const b = blockIdx.x, k0 = static_cast<size_t>(blockIdx.y) * (kCeBlock * 4) + threadIdx.x;
+  int const l = a.labels[b];
+  bool const live = l >= 0 && static_cast<size_t>(l) < a.V;
+  float const g = ce_row_weight(a, b) * a.scale;
   size_t const n = a.B * a.K;
-  for (size_t i = static_cast<size_t>(blockIdx.x) * kCeBlock + threadIdx.x; i < n; i += static_cast<size_t>(gridDim.x) * kCeBlock) {
-    size_t const b = i / a.K;
-    int const l = a.labels[b];
-    float s = 0.0f;
-    if (l >= 0 && static_cast<size_t>(l) < a.V) {
-      for (unsigned q = 0; q < slices; ++q) s += acc[q * n + i];
-      s *= ce_row_weight(a, b) * a.scale;
-    }
-    dX[i] = static_cast<O>(s);
+  float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  size_t at[4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) at[t] = b * a.K + (k0 + t * kCeBlock < a.K ? k0 + t * kCeBlock : a.K - 1);
+  if (live) {
+    for (unsigned q = 0; q < slices; ++q)
+#pragma unroll
+      for (int t = 0; t < 4; ++t) s[t] += acc[q * n + at[t]];
   }
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+    if (k0 + t * kCeBlock < a.K) dX[at[t]] = static_cast<O>(live ? s[t] * g : 0.0f);
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------
@@ -947,9 +966,8 @@ struct CeRun {
       }
     }
     if (rc != DLMI_OK || a.dX == nullptr) return rc;
-    size_t const blocks = dlmi_ceil_div(a.B * a.K, kCeBlock * 4), cap = static_cast<size_t>(ctx->num_cu) * 16;
-    hipLaunchKernelGGL(k_ce_dx_finish<E>, dim3(static_cast<unsigned>(blocks < cap ? blocks : cap)), dim3(kCeBlock), 0, ctx->stream, a,
-                       floats(p.dxacc), p.slices, static_cast<E *>(a.dX));
+    dim3 const grid(static_cast<unsigned>(a.B), static_cast<unsigned>(dlmi_ceil_div(a.K, kCeBlock * 4)));
+    hipLaunchKernelGGL(k_ce_dx_finish<E>, grid, dim3(kCeBlock), 0, ctx->stream, a, floats(p.dxacc), p.slices, static_cast<E *>(a.dX));
     DLMI_LAUNCH_CHECK(ctx, "k_ce_dx_finish");
     return DLMI_OK;
   }
