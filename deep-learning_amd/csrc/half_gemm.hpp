@@ -31,14 +31,22 @@ constexpr int kFragBytes = 1024;
 // Bytes of a packed matrix of `rows` x `k` (both already padded: rows to 32, k to 16).
 inline size_t packed_bytes(size_t rows, size_t k, int planes) { return rows * k * 2 * planes; }
 
-// One step of the K loop reads one stage of LDS: KS k blocks of all planes of the BM + BN rows.
+// Workgroup number -> number in an order in which the workgroups of one XCD (numbers equal modulo 8) are consecutive.
+__device__ __forceinline__ unsigned xcd_consecutive(unsigned id, unsigned n) {
+  unsigned const q = n >> 3, r = n & 7, x = id & 7;
+  return x * q + (x < r ? x : r) + (id >> 3);
+}
+
+// One step of the K loop reads one stage of LDS: KS k blocks of all planes of the BM + BN rows, four stages in all.  64 x 64
+// tiles take twice the k blocks of the others per stage: their stages are short, and three of them ahead is less than a load
+// takes.
 template <int BM, int BN, int NP>
 struct HalfTile {
   static constexpr int kPlanes = NP;
-  static constexpr int KS = 2 / NP;                          // k blocks per stage
-  static constexpr int kBufs = 4;                            // stages in LDS
+  static constexpr int kDepth = BM + BN <= 128 ? 4 : 2;      // fragments of a row block in a stage
+  static constexpr int KS = kDepth / NP;                     // k blocks per stage
   static constexpr int kMB = BM / 64, kNB = BN / 64;         // 32 x 32 blocks of a wavefront, 2 x 2 wavefronts
-  static constexpr int kFragsA = BM / 32 * 2, kFragsB = BN / 32 * 2;  // fragments of a stage (KS * NP == 2)
+  static constexpr int kFragsA = BM / 32 * kDepth, kFragsB = BN / 32 * kDepth;  // fragments of a stage
   static constexpr int kStageBytes = (kFragsA + kFragsB) * kFragBytes;
   static constexpr int kLoads = (kFragsA + kFragsB) / 4;     // direct loads of a wavefront per stage
 };
@@ -52,18 +60,18 @@ template <int BM, int BN, int NP>
 __device__ __forceinline__ void half_stage_load(char *lds, char const *P, char const *Q, size_t row_stride_p,
                                                 size_t row_stride_q, int wave, int lane) {
   using T = HalfTile<BM, BN, NP>;
-  // fragment f of an operand: row block f >> 1, the (f & 1)-th KiB of its KS k blocks x NP planes
+  // fragment f of an operand: row block f / kDepth, the (f % kDepth)-th KiB of its KS k blocks x NP planes
 #pragma unroll
   for (int u = 0; u < T::kFragsA / 4; ++u) {
     int const f = u * 4 + wave;
-    char const *src = P + static_cast<size_t>(f >> 1) * row_stride_p + (f & 1) * kFragBytes + lane * 16;
+    char const *src = P + static_cast<size_t>(f / T::kDepth) * row_stride_p + (f % T::kDepth) * kFragBytes + lane * 16;
     __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void const *)src,
                                      (__attribute__((address_space(3))) void *)(lds + f * kFragBytes), 16, 0, 0);
   }
 #pragma unroll
   for (int u = 0; u < T::kFragsB / 4; ++u) {
     int const f = u * 4 + wave;
-    char const *src = Q + static_cast<size_t>(f >> 1) * row_stride_q + (f & 1) * kFragBytes + lane * 16;
+    char const *src = Q + static_cast<size_t>(f / T::kDepth) * row_stride_q + (f % T::kDepth) * kFragBytes + lane * 16;
     __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void const *)src,
                                      (__attribute__((address_space(3))) void *)(lds + (T::kFragsA + f) * kFragBytes), 16,
                                      0, 0);
@@ -82,11 +90,11 @@ __device__ __forceinline__ void half_frags_read(HalfFrags<T> &f, char const *lds
   for (int pl = 0; pl < T::kPlanes; ++pl) {
 #pragma unroll
     for (int m = 0; m < T::kMB; ++m)
-      f.p[pl][m] = *reinterpret_cast<half8 const *>(lds + (((wm * T::kMB + m) * 2 + ks * T::kPlanes + pl) * kFragBytes + lane * 16));
+      f.p[pl][m] = *reinterpret_cast<half8 const *>(lds + (((wm * T::kMB + m) * T::kDepth + ks * T::kPlanes + pl) * kFragBytes + lane * 16));
 #pragma unroll
     for (int n = 0; n < T::kNB; ++n)
       f.q[pl][n] = *reinterpret_cast<half8 const *>(
-          lds + ((T::kFragsA + (wn * T::kNB + n) * 2 + ks * T::kPlanes + pl) * kFragBytes + lane * 16));
+          lds + ((T::kFragsA + (wn * T::kNB + n) * T::kDepth + ks * T::kPlanes + pl) * kFragBytes + lane * 16));
   }
 }
 
@@ -168,7 +176,7 @@ __device__ __forceinline__ void half_gemm(HalfAcc<HalfTile<BM, BN, NP>> &acc, ch
     for (int n = 0; n < T::kNB; ++n) acc.v[m][n] = f32x16{};
 
   auto const load = [&](char *buf, int t) {
-    half_stage_load<BM, BN, NP>(buf, P + static_cast<size_t>(t) * 2 * kFragBytes, Q + static_cast<size_t>(t) * 2 * kFragBytes,
+    half_stage_load<BM, BN, NP>(buf, P + static_cast<size_t>(t) * T::kDepth * kFragBytes, Q + static_cast<size_t>(t) * T::kDepth * kFragBytes,
                                 row_stride_p, row_stride_q, wave, lane);
   };
   // the first three stages are requested before the first is waited for
@@ -233,6 +241,95 @@ __device__ __forceinline__ void half_gemm(HalfAcc<HalfTile<BM, BN, NP>> &acc, ch
       }
     }
   }
+}
+
+// ---- the last tiles shared out -------------------------------------------------------------------------------------
+// Of a number of tiles that is no multiple of the G workgroups that run at once, the last ones (fewer than G) would leave
+// most of the device idle.  Their K loops are one list of pieces, kShareStages stages each, cut into G equal ranges; a
+// workgroup leaves the sums of each part of a tile in its range in memory, and a second launch adds a tile's parts in the
+// order of k and runs its epilogue, a wavefront per 32 x 32 block.
+constexpr unsigned kShareStages = 4;
+
+struct HalfShares {
+  unsigned whole, tiles;    // tiles that have a workgroup each; all tiles
+  unsigned stages;          // of a tile
+  unsigned grid;            // workgroups of the shared tiles: every one of them has a piece
+  unsigned pieces;          // of a shared tile
+  unsigned long long total; // pieces of all shared tiles
+  float *parts;             // [grid][2][BM * BN]: the first tile of a range, and the last
+  // the workgroup that holds a piece, and the tile of a workgroup's first piece
+  __host__ __device__ unsigned owner(unsigned long long piece) const { return static_cast<unsigned>(((piece + 1) * grid - 1) / total); }
+  __host__ __device__ unsigned first(unsigned w) const { return static_cast<unsigned>(w * total / grid / pieces); }
+};
+
+// (Fewer shared tiles than workgroups: a range is shorter than a tile and touches at most two.)
+inline HalfShares half_shares(unsigned tiles, unsigned stages, unsigned G, float *parts) {
+  HalfShares s = {};
+  s.tiles = tiles;
+  s.whole = tiles - tiles % G;
+  s.stages = stages;
+  s.pieces = (stages + kShareStages - 1) / kShareStages;
+  s.total = static_cast<unsigned long long>(tiles - s.whole) * s.pieces;
+  s.grid = s.total < G ? static_cast<unsigned>(s.total) : G;
+  s.parts = parts;
+  return s;
+}
+
+// A wavefront's blocks of a part, register pairs of a block's 64 lanes side by side.
+template <class T>
+__device__ __forceinline__ void half_part_store(float *part, HalfAcc<T> const &acc) {
+  f32x4 *const p = reinterpret_cast<f32x4 *>(part) + (threadIdx.x >> 6) * (T::kMB * T::kNB * 4 * 64) + (threadIdx.x & 63);
+#pragma unroll
+  for (int m = 0; m < T::kMB; ++m)
+#pragma unroll
+    for (int n = 0; n < T::kNB; ++n)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        f32x16 const &v = acc.v[m][n];
+        p[((m * T::kNB + n) * 4 + q) * 64] = f32x4{v[q * 4], v[q * 4 + 1], v[q * 4 + 2], v[q * 4 + 3]};
+      }
+}
+
+// The parts of the shared tiles.  operands(tile, P, Q): a tile's operands at its first stage.
+template <int BM, int BN, int NP, class Operands>
+__device__ __forceinline__ void half_gemm_parts(HalfShares const &s, size_t row_stride_p, size_t row_stride_q, Operands &&operands) {
+  using T = HalfTile<BM, BN, NP>;
+  unsigned const g = xcd_consecutive(blockIdx.x, gridDim.x);
+  unsigned long long u = g * s.total / s.grid;
+  unsigned long long const u1 = (g + 1ull) * s.total / s.grid;
+  unsigned const first = static_cast<unsigned>(u / s.pieces);
+  while (u < u1) {
+    unsigned const shared = static_cast<unsigned>(u / s.pieces);
+    unsigned long long const begin = static_cast<unsigned long long>(shared) * s.pieces, end = begin + s.pieces < u1 ? begin + s.pieces : u1;
+    unsigned const from = static_cast<unsigned>(u - begin) * kShareStages, to = static_cast<unsigned>(end - begin) * kShareStages;
+    char const *P, *Q;
+    operands(s.whole + shared, P, Q);
+    HalfAcc<T> acc;
+    __syncthreads();  // the stages of the part before have been read
+    half_gemm<BM, BN, NP>(acc, P + static_cast<size_t>(from) * T::kDepth * kFragBytes, Q + static_cast<size_t>(from) * T::kDepth * kFragBytes,
+                          row_stride_p, row_stride_q, static_cast<int>((to < s.stages ? to : s.stages) - from));
+    half_part_store(s.parts + (static_cast<size_t>(g) * 2 + (shared == first ? 0 : 1)) * (BM * BN), acc);
+    u = end;
+  }
+}
+
+// Block `block` (wavefront, m, n) of shared tile `shared`, its parts added in the order of k.
+template <class T>
+__device__ __forceinline__ f32x16 half_part_sum(HalfShares const &s, unsigned shared, unsigned block, int tile_floats) {
+  unsigned long long const begin = static_cast<unsigned long long>(shared) * s.pieces;
+  unsigned const w0 = s.owner(begin), w1 = s.owner(begin + s.pieces - 1);
+  f32x16 v = {};
+  for (unsigned w = w0; w <= w1; ++w) {
+    float const *const part = s.parts + (static_cast<size_t>(w) * 2 + (shared == s.first(w) ? 0 : 1)) * tile_floats;
+    f32x4 const *const p = reinterpret_cast<f32x4 const *>(part) + block * (4 * 64) + (threadIdx.x & 63);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      f32x4 const x = p[q * 64];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) v[q * 4 + t] += x[t];
+    }
+  }
+  return v;
 }
 
 // ---- a 32 x 32 block of C in registers (lane l: column j = l & 31, rows i = 8 (r >> 2) + 4 (l >> 5) + (r & 3)) -------------
@@ -343,12 +440,6 @@ __device__ __forceinline__ HalfBlock<NP> half_flip(HalfBlock<NP> const &b, half8
     r.pl[p] = o.pl[0];
   }
   return r;
-}
-
-// Workgroup number -> number in an order in which the workgroups of one XCD (numbers equal modulo 8) are consecutive.
-__device__ __forceinline__ unsigned xcd_consecutive(unsigned id, unsigned n) {
-  unsigned const q = n >> 3, r = n & 7, x = id & 7;
-  return x * q + (x < r ? x : r) + (id >> 3);
 }
 
 }  // namespace dlmi

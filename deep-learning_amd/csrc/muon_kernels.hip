@@ -12,8 +12,8 @@
 // Precision.  The polynomial multiplies what lies in weak directions by up to a^steps (485 for 5 steps of 3.4445), the
 // rounding of the operands among it.  With one f16 plane a random matrix ends 1.3e-3 off and a matrix of rank 32 plus 1 %
 // noise 2.7e-2; with two planes (22 bits) 1.8e-6 and 1.2e-5, as far as a computation in fp32 (1.1e-5 and 1.9e-5).  So X,
-// A and b A + c A A keep two planes throughout, whatever the type of the result.  Singular values stay below about 1.3
-// and the polynomial in A below 3, so all three matrices are held times 2^12: far from the ends of f16's range.
+// A and a I + b A + c A A keep two planes throughout, whatever the type of the result.  Singular values stay below about 1.3
+// and the polynomial in A between -3 and 4, so all three matrices are held times 2^12: far from the ends of f16's range.
 //
 // X is kept both ways round (rows i, k = j for X X^T; rows j, k = i for the product by X), each written by the product
 // that makes it: a block of C in registers is a fragment of the transposed matrix as it stands, and two matrix
@@ -47,21 +47,45 @@ __device__ __forceinline__ double muon_block_sum(double s, double *lds) {
   return s;
 }
 
-// The momentum, and partial[matrix][block] = sum of u^2 (double: the norm of a tiny gradient does not underflow).
+// The momentum, and partial[matrix][block] = sum of u^2 (double: the norm of a tiny gradient does not underflow).  Four
+// elements of a thread at a time: their loads are on their way together.
 template <class T, bool STEP>
 __global__ __launch_bounds__(kMuonBlock) void k_muon_moment(MuonBatch b, size_t n, float momentum, int nesterov, double *partial) {
   __shared__ double lds[kMuonBlock / 64];
+  struct __attribute__((packed, aligned(sizeof(T)))) V {
+    T v[4];
+  };
+  struct __attribute__((packed, aligned(4))) F {
+    float v[4];
+  };
   T const *const g = static_cast<T const *>(b.g[blockIdx.y]);
   float *const m = b.m[blockIdx.y];
-  double s = 0.0;
-  for (size_t i = static_cast<size_t>(blockIdx.x) * kMuonBlock + threadIdx.x; i < n; i += static_cast<size_t>(gridDim.x) * kMuonBlock) {
-    float u = static_cast<float>(g[i]);
+  auto const one = [&](float x, float &mv) {
     if constexpr (STEP) {
-      float const v = momentum * m[i] + u;
-      m[i] = v;
-      u = nesterov ? u + momentum * v : v;
+      mv = momentum * mv + x;
+      x = nesterov ? x + momentum * mv : mv;
     }
-    s += static_cast<double>(u) * u;
+    return static_cast<double>(x) * x;
+  };
+  size_t const quads = n / 4, stride = static_cast<size_t>(gridDim.x) * kMuonBlock;
+  size_t const at = static_cast<size_t>(blockIdx.x) * kMuonBlock + threadIdx.x;
+  double s = 0.0;
+#pragma unroll 2
+  for (size_t i = at; i < quads; i += stride) {
+    V const x = *reinterpret_cast<V const *>(g + i * 4);
+    F w = {};
+    if constexpr (STEP) w = *reinterpret_cast<F const *>(m + i * 4);
+    double q = 0.0;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) q += one(static_cast<float>(x.v[t]), w.v[t]);
+    if constexpr (STEP) *reinterpret_cast<F *>(m + i * 4) = w;
+    s += q;
+  }
+  if (at < n - quads * 4) {
+    float w = 0.0f;
+    if constexpr (STEP) w = m[quads * 4 + at];
+    s += one(static_cast<float>(g[quads * 4 + at]), w);
+    if constexpr (STEP) m[quads * 4 + at] = w;
   }
   s = muon_block_sum(s, lds);
   if (threadIdx.x == 0) partial[static_cast<size_t>(blockIdx.y) * gridDim.x + blockIdx.x] = s;
@@ -83,22 +107,26 @@ __global__ __launch_bounds__(kMuonBlock) void k_muon_pack(MuonBatch b, unsigned 
   T *const g = static_cast<T *>(b.g[mat]);
   float const *const m = b.m[mat];
   unsigned const r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
-  unsigned const tc = threadIdx.x & 63;
+  // every load is made, of the last row and column at most: loads behind conditions of their own would each be waited for
+  unsigned const tc = threadIdx.x & 63, c = c0 + tc, cl = c < C ? c : C - 1;
+  float gv[16], mv[16];
 #pragma unroll
   for (int q = 0; q < 16; ++q) {
-    unsigned const tr = q * 4 + (threadIdx.x >> 6);
-    unsigned const r = r0 + tr, c = c0 + tc;
-    float u = 0.0f;
-    if (r < R && c < C) {
-      size_t const at = static_cast<size_t>(r) * C + c;
-      u = static_cast<float>(g[at]);
-      if constexpr (STEP) {
-        float const v = m[at];
-        u = nesterov ? u + momentum * v : v;
-        g[at] = static_cast<T>(0.0f);
-      }
+    unsigned const r = r0 + q * 4 + (threadIdx.x >> 6);
+    size_t const at = static_cast<size_t>(r < R ? r : R - 1) * C + cl;
+    gv[q] = static_cast<float>(g[at]);
+    mv[q] = STEP ? m[at] : 0.0f;
+  }
+#pragma unroll
+  for (int q = 0; q < 16; ++q) {
+    unsigned const tr = q * 4 + (threadIdx.x >> 6), r = r0 + tr;
+    bool const in = r < R && c < C;
+    float u = gv[q];
+    if constexpr (STEP) {
+      u = nesterov ? u + momentum * mv[q] : mv[q];
+      if (in) g[static_cast<size_t>(r) * C + c] = static_cast<T>(0.0f);
     }
-    tile[tr][tc] = static_cast<float>(u * inv);
+    tile[tr][tc] = in ? static_cast<float>(u * inv) : 0.0f;
   }
   __syncthreads();
   int const lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -126,38 +154,92 @@ __global__ __launch_bounds__(kMuonBlock) void k_muon_pack(MuonBatch b, unsigned 
 }
 
 // A tile of a symmetric product C = P P^T (P: [mp, k] packed), only the tiles on and below the diagonal; written packed
-// with its mirror image.  POLY: C = b P + c P P^T (P symmetric itself).  Products of two values held times 2^12.
-template <int T, bool POLY>
-__global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_muon_symmetric(char const *P, char *C, size_t stride_p, size_t stride_c,
-                                                                         unsigned tiles, unsigned kblocks, unsigned kblocks_c,
-                                                                         float cb, float cc) {
-  using H = HalfTile<T, T, 2>;
-  unsigned const tri = tiles * (tiles + 1) / 2;
-  unsigned const id = xcd_consecutive(blockIdx.x, gridDim.x);
-  unsigned const mat = id / tri, t = id - mat * tri;
-  unsigned ti = static_cast<unsigned>((sqrtf(8.0f * static_cast<float>(t) + 1.0f) - 1.0f) * 0.5f);
+// with its mirror image.  POLY: C = a I + b P + c P P^T (P symmetric itself).  Products of two values held times 2^12.
+struct MuonSymmetric {
+  char const *P;
+  char *C;
+  size_t stride_p, stride_c;
+  unsigned tiles, kblocks, kblocks_c;  // of a side; k blocks of P and of C
+  float ca, cb, cc;
+};
+
+__device__ __forceinline__ void muon_triangle(unsigned t, unsigned &ti, unsigned &tj) {
+  ti = static_cast<unsigned>((sqrtf(8.0f * static_cast<float>(t) + 1.0f) - 1.0f) * 0.5f);
   while (ti * (ti + 1) / 2 > t) --ti;
   while ((ti + 1) * (ti + 2) / 2 <= t) ++ti;
-  unsigned const tj = t - ti * (ti + 1) / 2;
-  char const *const p = P + mat * stride_p;
-  size_t const rs = static_cast<size_t>(kblocks) * 2 * kFragBytes;
+  tj = t - ti * (ti + 1) / 2;
+}
+
+template <bool POLY>
+__device__ __forceinline__ void muon_symmetric_block(MuonSymmetric const &a, unsigned mat, unsigned ib, unsigned jb, bool mirror, f32x16 v,
+                                                     half8 id0, half8 id1, int lane) {
+  char const *const p = a.P + mat * a.stride_p;
+  char *const c = a.C + mat * a.stride_c;
+  size_t const rs = static_cast<size_t>(a.kblocks) * 2 * kFragBytes, rc = static_cast<size_t>(a.kblocks_c) * 2 * kFragBytes;
+  v *= a.cc / kMuonScale;
+  if constexpr (POLY) {
+    v += a.cb * half_load<2>(p + jb * rs + ib * 4 * kFragBytes, lane);
+    if (ib == jb) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) v[r] += 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3) == (lane & 31) ? a.ca * kMuonScale : 0.0f;
+    }
+  }
+  HalfBlock<2> const blk = half_split<2>(v);
+  half_store<2>(c + jb * rc + ib * 4 * kFragBytes, blk, lane);
+  if (mirror) half_store<2>(c + ib * rc + jb * 4 * kFragBytes, half_flip<2>(blk, id0, id1), lane);
+}
+
+struct MuonTile {
+  unsigned mat, ti, tj;
+};
+__device__ __forceinline__ MuonTile muon_tile(MuonSymmetric const &a, unsigned tile) {
+  unsigned const tri = a.tiles * (a.tiles + 1) / 2;
+  MuonTile t;
+  t.mat = tile / tri;
+  muon_triangle(tile - t.mat * tri, t.ti, t.tj);
+  return t;
+}
+
+template <int T, bool POLY>
+__global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_muon_symmetric(MuonSymmetric a, unsigned stages) {
+  using H = HalfTile<T, T, 2>;
+  MuonTile const t = muon_tile(a, xcd_consecutive(blockIdx.x, gridDim.x));
+  size_t const rs = static_cast<size_t>(a.kblocks) * 2 * kFragBytes;
+  char const *const p = a.P + t.mat * a.stride_p;
   HalfAcc<H> acc;
-  half_gemm<T, T, 2>(acc, p + ti * (T / 32) * rs, p + tj * (T / 32) * rs, rs, rs, kblocks);
+  half_gemm<T, T, 2>(acc, p + t.ti * (T / 32) * rs, p + t.tj * (T / 32) * rs, rs, rs, stages);
   int const lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   half8 const id0 = half_identity(0, lane), id1 = half_identity(1, lane);
-  char *const c = C + mat * stride_c;
-  size_t const rc = static_cast<size_t>(kblocks_c) * 2 * kFragBytes;
 #pragma unroll
   for (int m = 0; m < H::kMB; ++m)
 #pragma unroll
-    for (int n = 0; n < H::kNB; ++n) {
-      unsigned const ib = ti * (T / 32) + (wave >> 1) * H::kMB + m, jb = tj * (T / 32) + (wave & 1) * H::kNB + n;
-      f32x16 v = acc.v[m][n] * (cc / kMuonScale);
-      if constexpr (POLY) v += cb * half_load<2>(p + jb * rs + ib * 4 * kFragBytes, lane);
-      HalfBlock<2> const blk = half_split<2>(v);
-      half_store<2>(c + jb * rc + ib * 4 * kFragBytes, blk, lane);
-      if (ti != tj) half_store<2>(c + ib * rc + jb * 4 * kFragBytes, half_flip<2>(blk, id0, id1), lane);
-    }
+    for (int n = 0; n < H::kNB; ++n)
+      muon_symmetric_block<POLY>(a, t.mat, t.ti * (T / 32) + (wave >> 1) * H::kMB + m, t.tj * (T / 32) + (wave & 1) * H::kNB + n, t.ti != t.tj,
+                                 acc.v[m][n], id0, id1, lane);
+}
+
+template <int T>
+__global__ __launch_bounds__(256, 1) void k_muon_symmetric_parts(MuonSymmetric a, HalfShares shares) {
+  size_t const rs = static_cast<size_t>(a.kblocks) * 2 * kFragBytes;
+  half_gemm_parts<T, T, 2>(shares, rs, rs, [&](unsigned tile, char const *&p, char const *&q) {
+    MuonTile const t = muon_tile(a, tile);
+    p = a.P + t.mat * a.stride_p + t.ti * (T / 32) * rs;
+    q = a.P + t.mat * a.stride_p + t.tj * (T / 32) * rs;
+  });
+}
+
+// The blocks of the shared tiles, a wavefront each.
+template <int T, bool POLY>
+__global__ __launch_bounds__(256) void k_muon_symmetric_join(MuonSymmetric a, HalfShares shares) {
+  using H = HalfTile<T, T, 2>;
+  constexpr unsigned kBlocks = (T / 32) * (T / 32), kWave = H::kMB * H::kNB;
+  int const lane = threadIdx.x & 63;
+  unsigned const id = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), shared = id / kBlocks, block = id % kBlocks;
+  f32x16 const v = half_part_sum<H>(shares, shared, block, T * T);
+  MuonTile const t = muon_tile(a, shares.whole + shared);
+  unsigned const wave = block / kWave, m = block % kWave / H::kNB, n = block % H::kNB;
+  muon_symmetric_block<POLY>(a, t.mat, t.ti * (T / 32) + (wave >> 1) * H::kMB + m, t.tj * (T / 32) + (wave & 1) * H::kNB + n, t.ti != t.tj, v,
+                             half_identity(0, lane), half_identity(1, lane), lane);
 }
 
 enum { kMuonMore = 0, kMuonOut = 1, kMuonStep = 2 };
@@ -173,71 +255,114 @@ __device__ __forceinline__ float muon_new(float w, float x, float lr, float wd) 
   return MODE == kMuonStep ? w - (lr * x + wd * w) : x;
 }
 
-// A tile of X' = a X + Bm X; XT = X^T packed (row j, k = i).  MORE: written packed both ways; OUT, STEP: the last of the
+// A tile of X' = Bm X, Bm = a I + b A + c A A (a X inside the product: read beside it in the epilogue it is 4 bytes more per
+// element, while the matrix pipe waits); XT = X^T packed (row j, k = i).  MORE: written packed both ways; OUT, STEP: the last of the
 // iteration, written to the caller's matrix.
+struct MuonUpdate {
+  char const *Bm, *XT;
+  char *XTn, *XP;
+  size_t stride_b, stride_x;
+  unsigned mt, nt, kbm, kbn;  // tiles and k blocks of the short and of the long side
+  MuonOut o;
+};
+
+template <int MODE, class O>
+__device__ __forceinline__ void muon_update_block(MuonUpdate const &a, MuonBatch const &b, unsigned mat, unsigned ib, unsigned jb, f32x16 v,
+                                                  half8 id0, half8 id1, int lane) {
+  size_t const rs = static_cast<size_t>(a.kbm) * 2 * kFragBytes, rn = static_cast<size_t>(a.kbn) * 2 * kFragBytes;
+  v *= 1.0f / kMuonScale;
+  if constexpr (MODE == kMuonMore) {
+    HalfBlock<2> const blk = half_split<2>(v);
+    half_store<2>(a.XTn + mat * a.stride_x + jb * rs + ib * 4 * kFragBytes, blk, lane);
+    half_store<2>(a.XP + mat * a.stride_x + ib * rn + jb * 4 * kFragBytes, half_flip<2>(blk, id0, id1), lane);
+  } else {
+    MuonOut const &o = a.o;
+    v *= 1.0f / kMuonScale;
+    O *const p = static_cast<O *>(b.p[mat]);
+    size_t const j = jb * 32 + (lane & 31), i0 = ib * 32 + 4 * (lane >> 5);
+    size_t const si = o.flipped ? 1 : o.cols, sj = o.flipped ? o.cols : 1;
+    unsigned const rows = o.flipped ? o.cols : o.rows, cols = o.flipped ? o.rows : o.cols;  // of X
+    float const lr = MODE == kMuonStep ? b.lr[mat] : 0.0f;
+    // (a block inside the matrix has no conditions between its loads, which would each be waited for)
+    if (ib * 32 + 32 <= rows && jb * 32 + 32 <= cols) {
+      O *const q = p + i0 * si + j * sj;
+      f32x16 w = {};
+      if constexpr (MODE == kMuonStep) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) w[r] = static_cast<float>(q[(8 * (r >> 2) + (r & 3)) * si]);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) q[(8 * (r >> 2) + (r & 3)) * si] = static_cast<O>(muon_new<MODE>(w[r], v[r], lr, o.wd));
+    } else {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        size_t const i = i0 + 8 * (r >> 2) + (r & 3);
+        if (i < rows && j < cols) {
+          O *const q = p + i * si + j * sj;
+          *q = static_cast<O>(muon_new<MODE>(MODE == kMuonStep ? static_cast<float>(*q) : 0.0f, v[r], lr, o.wd));
+        }
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ MuonTile muon_tile(MuonUpdate const &a, unsigned tile) {
+  MuonTile t;
+  t.mat = tile / (a.mt * a.nt);
+  unsigned const r = tile - t.mat * (a.mt * a.nt);
+  t.tj = r / a.mt;
+  t.ti = r - t.tj * a.mt;
+  return t;
+}
+
 template <int T, int MODE, class O>
-__global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_muon_update(char const *Bm, char const *XT, char *XTn, char *XP,
-                                                                      size_t stride_b, size_t stride_x, unsigned mt, unsigned nt,
-                                                                      unsigned kbm, unsigned kbn, float ca, MuonBatch b, MuonOut o) {
+__global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_muon_update(MuonUpdate a, MuonBatch b, unsigned stages) {
   using H = HalfTile<T, T, 2>;
-  unsigned const id = xcd_consecutive(blockIdx.x, gridDim.x);
-  unsigned const mat = id / (mt * nt), t = id - mat * (mt * nt);
-  unsigned const ti = t % mt, tj = t / mt;
-  size_t const rs = static_cast<size_t>(kbm) * 2 * kFragBytes, rn = static_cast<size_t>(kbn) * 2 * kFragBytes;
-  char const *const xt = XT + mat * stride_x;
+  MuonTile const t = muon_tile(a, xcd_consecutive(blockIdx.x, gridDim.x));
+  size_t const rs = static_cast<size_t>(a.kbm) * 2 * kFragBytes;
   HalfAcc<H> acc;
-  half_gemm<T, T, 2>(acc, Bm + mat * stride_b + ti * (T / 32) * rs, xt + tj * (T / 32) * rs, rs, rs, kbm);
+  half_gemm<T, T, 2>(acc, a.Bm + t.mat * a.stride_b + t.ti * (T / 32) * rs, a.XT + t.mat * a.stride_x + t.tj * (T / 32) * rs, rs, rs, stages);
   int const lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   half8 const id0 = half_identity(0, lane), id1 = half_identity(1, lane);
 #pragma unroll
   for (int m = 0; m < H::kMB; ++m)
 #pragma unroll
-    for (int n = 0; n < H::kNB; ++n) {
-      unsigned const ib = ti * (T / 32) + (wave >> 1) * H::kMB + m, jb = tj * (T / 32) + (wave & 1) * H::kNB + n;
-      f32x16 v = acc.v[m][n] * (1.0f / kMuonScale) + ca * half_load<2>(xt + jb * rs + ib * 4 * kFragBytes, lane);
-      if constexpr (MODE == kMuonMore) {
-        HalfBlock<2> const blk = half_split<2>(v);
-        half_store<2>(XTn + mat * stride_x + jb * rs + ib * 4 * kFragBytes, blk, lane);
-        half_store<2>(XP + mat * stride_x + ib * rn + jb * 4 * kFragBytes, half_flip<2>(blk, id0, id1), lane);
-      } else {
-        v *= 1.0f / kMuonScale;
-        O *const p = static_cast<O *>(b.p[mat]);
-        size_t const j = jb * 32 + (lane & 31), i0 = ib * 32 + 4 * (lane >> 5);
-        size_t const si = o.flipped ? 1 : o.cols, sj = o.flipped ? o.cols : 1;
-        unsigned const rows = o.flipped ? o.cols : o.rows, cols = o.flipped ? o.rows : o.cols;  // of X
-        float const lr = MODE == kMuonStep ? b.lr[mat] : 0.0f;
-        // (a block inside the matrix has no conditions between its loads, which would each be waited for)
-        if (ib * 32 + 32 <= rows && jb * 32 + 32 <= cols) {
-          O *const q = p + i0 * si + j * sj;
-          f32x16 w = {};
-          if constexpr (MODE == kMuonStep) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) w[r] = static_cast<float>(q[(8 * (r >> 2) + (r & 3)) * si]);
-          }
-#pragma unroll
-          for (int r = 0; r < 16; ++r) q[(8 * (r >> 2) + (r & 3)) * si] = static_cast<O>(muon_new<MODE>(w[r], v[r], lr, o.wd));
-        } else {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            size_t const i = i0 + 8 * (r >> 2) + (r & 3);
-            if (i < rows && j < cols) {
-              O *const q = p + i * si + j * sj;
-              *q = static_cast<O>(muon_new<MODE>(MODE == kMuonStep ? static_cast<float>(*q) : 0.0f, v[r], lr, o.wd));
-            }
-          }
-        }
-      }
-    }
+    for (int n = 0; n < H::kNB; ++n)
+      muon_update_block<MODE, O>(a, b, t.mat, t.ti * (T / 32) + (wave >> 1) * H::kMB + m, t.tj * (T / 32) + (wave & 1) * H::kNB + n,
+                                 acc.v[m][n], id0, id1, lane);
 }
 
-// The iteration's bounds for singular values in [0, 1]: largest magnitude of X X^T and of b A + c A A on the way.
+template <int T>
+__global__ __launch_bounds__(256, 1) void k_muon_update_parts(MuonUpdate a, HalfShares shares) {
+  size_t const rs = static_cast<size_t>(a.kbm) * 2 * kFragBytes;
+  half_gemm_parts<T, T, 2>(shares, rs, rs, [&](unsigned tile, char const *&p, char const *&q) {
+    MuonTile const t = muon_tile(a, tile);
+    p = a.Bm + t.mat * a.stride_b + t.ti * (T / 32) * rs;
+    q = a.XT + t.mat * a.stride_x + t.tj * (T / 32) * rs;
+  });
+}
+
+template <int T, int MODE, class O>
+__global__ __launch_bounds__(256) void k_muon_update_join(MuonUpdate a, MuonBatch b, HalfShares shares) {
+  using H = HalfTile<T, T, 2>;
+  constexpr unsigned kBlocks = (T / 32) * (T / 32), kWave = H::kMB * H::kNB;
+  int const lane = threadIdx.x & 63;
+  unsigned const id = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), shared = id / kBlocks, block = id % kBlocks;
+  f32x16 const v = half_part_sum<H>(shares, shared, block, T * T);
+  MuonTile const t = muon_tile(a, shares.whole + shared);
+  unsigned const wave = block / kWave, m = block % kWave / H::kNB, n = block % H::kNB;
+  muon_update_block<MODE, O>(a, b, t.mat, t.ti * (T / 32) + (wave >> 1) * H::kMB + m, t.tj * (T / 32) + (wave & 1) * H::kNB + n, v,
+                             half_identity(0, lane), half_identity(1, lane), lane);
+}
+
+// The iteration's bounds for singular values in [0, 1]: largest magnitude of X X^T and of a I + b A + c A A on the way.
 static double muon_reach(float const *coefs, int steps) {
   double most = 1.0;
   for (int i = 0; i <= 2048; ++i) {
     double s = i / 2048.0;
     for (int k = 0; k < steps; ++k) {
-      double const q = s * s, poly = coefs[1] * q + coefs[2] * q * q;
-      s = coefs[0] * s + poly * s;
+      double const q = s * s, poly = coefs[0] + coefs[1] * q + coefs[2] * q * q;
+      s *= poly;
       if (!(std::fabs(poly) <= 1e6) || !(std::fabs(s) <= 1e6)) return 1e6;
       if (std::fabs(poly) > most) most = std::fabs(poly);
       if (s * s > most) most = s * s;
@@ -251,6 +376,9 @@ struct MuonPlan {
   size_t mp, np, bytes_x, bytes_a, per_matrix;
   int tile;
   unsigned nparts;
+  unsigned workgroups;         // that run at once
+  size_t parts;                // bytes of the parts of shared tiles
+  size_t bytes(size_t count) const { return per_matrix * count + parts; }
 };
 
 static MuonPlan muon_plan(dlmi_ctx const *ctx, size_t rows, size_t cols, size_t count) {
@@ -272,33 +400,78 @@ static MuonPlan muon_plan(dlmi_ctx const *ctx, size_t rows, size_t cols, size_t 
   pl.nparts = static_cast<unsigned>(dlmi_ceil_div(rows * cols, kMuonBlock * 8));
   if (pl.nparts > 256) pl.nparts = 256;
   pl.per_matrix = 3 * pl.bytes_x + 2 * pl.bytes_a + dlmi_ceil_div(pl.nparts * sizeof(double), 1024) * 1024;
+  // a workgroup of 256 x 256 tiles per CU; their last tiles may be shared out, two parts a workgroup
+  pl.workgroups = static_cast<unsigned>(ctx->num_cu);
+  pl.parts = pl.tile == 256 ? static_cast<size_t>(pl.workgroups) * 2 * 256 * 256 * sizeof(float) : 0;
   return pl;
 }
 
-template <int T, class O>
+// Whether sharing out the last tiles pays: a round of 256 x 256 tiles that is at most three quarters full is worth the
+// two launches and the parts' way through memory; smaller tiles leave less idle than that costs.
+static HalfShares muon_shares(MuonPlan const &pl, unsigned tiles, unsigned stages, float *parts) {
+  unsigned const over = tiles % pl.workgroups;
+  bool const share = pl.tile == 256 && over != 0 && over * 4 <= pl.workgroups * 3;
+  return half_shares(tiles, stages, share ? pl.workgroups : tiles, parts);
+}
+
+template <int T, bool POLY>
+static int muon_symmetric(dlmi_ctx *ctx, MuonSymmetric const &a, HalfShares const &shares) {
+  if (shares.whole != 0) {
+    hipLaunchKernelGGL((k_muon_symmetric<T, POLY>), dim3(shares.whole), dim3(256), 0, ctx->stream, a, shares.stages);
+    DLMI_LAUNCH_CHECK(ctx, "k_muon_symmetric");
+  }
+  if constexpr (T == 256) {
+    if (shares.total == 0) return DLMI_OK;
+    hipLaunchKernelGGL(k_muon_symmetric_parts<T>, dim3(shares.grid), dim3(256), 0, ctx->stream, a, shares);
+    DLMI_LAUNCH_CHECK(ctx, "k_muon_symmetric_parts");
+    unsigned const blocks = (shares.tiles - shares.whole) * (T / 32) * (T / 32) / 4;
+    hipLaunchKernelGGL((k_muon_symmetric_join<T, POLY>), dim3(blocks), dim3(256), 0, ctx->stream, a, shares);
+    DLMI_LAUNCH_CHECK(ctx, "k_muon_symmetric_join");
+  }
+  return DLMI_OK;
+}
+
+template <int T, int MODE, class O>
+static int muon_update(dlmi_ctx *ctx, MuonUpdate const &a, MuonBatch const &b, HalfShares const &shares) {
+  if (shares.whole != 0) {
+    hipLaunchKernelGGL((k_muon_update<T, MODE, O>), dim3(shares.whole), dim3(256), 0, ctx->stream, a, b, shares.stages);
+    DLMI_LAUNCH_CHECK(ctx, "k_muon_update");
+  }
+  if constexpr (T == 256) {
+    if (shares.total == 0) return DLMI_OK;
+    hipLaunchKernelGGL(k_muon_update_parts<T>, dim3(shares.grid), dim3(256), 0, ctx->stream, a, shares);
+    DLMI_LAUNCH_CHECK(ctx, "k_muon_update_parts");
+    unsigned const blocks = (shares.tiles - shares.whole) * (T / 32) * (T / 32) / 4;
+    hipLaunchKernelGGL((k_muon_update_join<T, MODE, O>), dim3(blocks), dim3(256), 0, ctx->stream, a, b, shares);
+    DLMI_LAUNCH_CHECK(ctx, "k_muon_update_join");
+  }
+  return DLMI_OK;
+}
+
+template <int T, class O, bool STEP>
 static int muon_iterate(dlmi_ctx *ctx, MuonBatch const &b, MuonPlan const &pl, unsigned count, float const *coefs, int steps,
-                        MuonOut const &o, int last_mode, char *XP, char *XT, char *XTn, char *A, char *Bm) {
+                        MuonOut const &o, char *XP, char *XT, char *XTn, char *A, char *Bm, float *parts) {
   unsigned const mt = static_cast<unsigned>(pl.mp / T), nt = static_cast<unsigned>(pl.np / T);
   unsigned const kbm = static_cast<unsigned>(pl.mp / 16), kbn = static_cast<unsigned>(pl.np / 16);
-  dim3 const tri(mt * (mt + 1) / 2 * count), all(mt * nt * count);
+  constexpr unsigned KS = HalfTile<T, T, 2>::KS;
+  unsigned const tri = mt * (mt + 1) / 2 * count, all = mt * nt * count;
+  HalfShares const gram = muon_shares(pl, tri, kbn / KS, parts), square = muon_shares(pl, tri, kbm / KS, parts),
+                   product = muon_shares(pl, all, kbm / KS, parts);
+  MuonSymmetric const g{XP, A, pl.bytes_x, pl.bytes_a, mt, kbn, kbm, 0.0f, 0.0f, 1.0f};
+  MuonSymmetric const q{A, Bm, pl.bytes_a, pl.bytes_a, mt, kbm, kbm, coefs[0], coefs[1], coefs[2]};
+  MuonUpdate u{Bm, XT, XTn, XP, pl.bytes_a, pl.bytes_x, mt, nt, kbm, kbn, o};
   for (int s = 0; s < steps; ++s) {
-    hipLaunchKernelGGL((k_muon_symmetric<T, false>), tri, dim3(256), 0, ctx->stream, XP, A, pl.bytes_x, pl.bytes_a, mt, kbn, kbm, 0.0f,
-                       1.0f);
-    DLMI_LAUNCH_CHECK(ctx, "k_muon_symmetric");
-    hipLaunchKernelGGL((k_muon_symmetric<T, true>), tri, dim3(256), 0, ctx->stream, A, Bm, pl.bytes_a, pl.bytes_a, mt, kbm, kbm,
-                       coefs[1], coefs[2]);
-    DLMI_LAUNCH_CHECK(ctx, "k_muon_symmetric");
+    int rc = muon_symmetric<T, false>(ctx, g, gram);
+    if (rc == DLMI_OK) rc = muon_symmetric<T, true>(ctx, q, square);
+    if (rc != DLMI_OK) return rc;
     if (s + 1 < steps)
-      hipLaunchKernelGGL((k_muon_update<T, kMuonMore, O>), all, dim3(256), 0, ctx->stream, Bm, XT, XTn, XP, pl.bytes_a, pl.bytes_x, mt, nt,
-                         kbm, kbn, coefs[0], b, o);
-    else if (last_mode == kMuonStep)
-      hipLaunchKernelGGL((k_muon_update<T, kMuonStep, O>), all, dim3(256), 0, ctx->stream, Bm, XT, XTn, XP, pl.bytes_a, pl.bytes_x, mt, nt,
-                         kbm, kbn, coefs[0], b, o);
+      rc = muon_update<T, kMuonMore, O>(ctx, u, b, product);
     else
-      hipLaunchKernelGGL((k_muon_update<T, kMuonOut, O>), all, dim3(256), 0, ctx->stream, Bm, XT, XTn, XP, pl.bytes_a, pl.bytes_x, mt, nt,
-                         kbm, kbn, coefs[0], b, o);
-    DLMI_LAUNCH_CHECK(ctx, "k_muon_update");
-    std::swap(XT, XTn);
+      rc = muon_update<T, STEP ? kMuonStep : kMuonOut, O>(ctx, u, b, product);
+    if (rc != DLMI_OK) return rc;
+    char *const x = const_cast<char *>(u.XT);
+    u.XT = u.XTn;
+    u.XTn = x;
   }
   return DLMI_OK;
 }
@@ -309,7 +482,8 @@ static int muon_batch(dlmi_ctx *ctx, MuonBatch const &b, size_t rows, size_t col
                       int nesterov, float wd, int steps, float const *coefs, float eps) {
   char *const XP = dlmi_scratch_data(ctx), *const XT = XP + count * pl.bytes_x, *const XTn = XT + count * pl.bytes_x;
   char *const A = XTn + count * pl.bytes_x, *const Bm = A + count * pl.bytes_a;
-  double *const partial = reinterpret_cast<double *>(Bm + count * pl.bytes_a);
+  float *const parts = reinterpret_cast<float *>(Bm + count * pl.bytes_a);
+  double *const partial = reinterpret_cast<double *>(reinterpret_cast<char *>(parts) + pl.parts);
   size_t const n = rows * cols;
   hipLaunchKernelGGL((k_muon_moment<T, STEP>), dim3(pl.nparts, count), dim3(kMuonBlock), 0, ctx->stream, b, n, momentum, nesterov, partial);
   DLMI_LAUNCH_CHECK(ctx, "k_muon_moment");
@@ -320,10 +494,9 @@ static int muon_batch(dlmi_ctx *ctx, MuonBatch const &b, size_t rows, size_t col
                      pl.bytes_x);
   DLMI_LAUNCH_CHECK(ctx, "k_muon_pack");
   MuonOut const o{static_cast<unsigned>(rows), static_cast<unsigned>(cols), pl.flipped, wd};
-  int const mode = STEP ? kMuonStep : kMuonOut;
-  if (pl.tile == 256) return muon_iterate<256, T>(ctx, b, pl, count, coefs, steps, o, mode, XP, XT, XTn, A, Bm);
-  if (pl.tile == 128) return muon_iterate<128, T>(ctx, b, pl, count, coefs, steps, o, mode, XP, XT, XTn, A, Bm);
-  return muon_iterate<64, T>(ctx, b, pl, count, coefs, steps, o, mode, XP, XT, XTn, A, Bm);
+  if (pl.tile == 256) return muon_iterate<256, T, STEP>(ctx, b, pl, count, coefs, steps, o, XP, XT, XTn, A, Bm, parts);
+  if (pl.tile == 128) return muon_iterate<128, T, STEP>(ctx, b, pl, count, coefs, steps, o, XP, XT, XTn, A, Bm, parts);
+  return muon_iterate<64, T, STEP>(ctx, b, pl, count, coefs, steps, o, XP, XT, XTn, A, Bm, parts);
 }
 
 static char const *muon_check(dlmi_newton_schulz const *ns) {
@@ -365,7 +538,7 @@ int dlmi_orthogonalize(dlmi_ctx *ctx, dlmi_dtype type, size_t rows, size_t cols,
   b.g[0] = const_cast<void *>(G);
   float const c[3] = {ns->a, ns->b, ns->c};
   MuonPlan const pl = muon_plan(ctx, rows, cols, 1);
-  int const rc = dlmi_scratch_reserve(ctx, pl.per_matrix);
+  int const rc = dlmi_scratch_reserve(ctx, pl.bytes(1));
   if (rc != DLMI_OK) return rc;
   if (type == DLMI_F32) return muon_batch<float, false>(ctx, b, rows, cols, 1, pl, 0.0f, 0, 0.0f, ns->steps, c, ns->eps);
   return muon_batch<__bf16, false>(ctx, b, rows, cols, 1, pl, 0.0f, 0, 0.0f, ns->steps, c, ns->eps);
@@ -429,7 +602,7 @@ int dlmi_opt_muon(dlmi_ctx *ctx, size_t n, dlmi_muon_problem const *problems, fl
         l.b.m[k] = q.momentum;
         l.b.lr[k] = q.lr;
       }
-      if (l.pl.per_matrix * l.count > scratch) scratch = l.pl.per_matrix * l.count;
+      if (l.pl.bytes(l.count) > scratch) scratch = l.pl.bytes(l.count);
       at += l.count;
       launches.push_back(l);
     }

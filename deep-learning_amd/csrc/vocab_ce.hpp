@@ -755,7 +755,7 @@ __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_dx(char const *P, 
   unsigned const s0 = slice * per_slice;
   if (s0 >= stages) return;  // a shorter last piece (the first has work for every slice)
   unsigned const count = stages - s0 < per_slice ? stages - s0 : per_slice;
-  size_t const rs = static_cast<size_t>(kblocks) * NP * kFragBytes, skip = static_cast<size_t>(s0) * 2 * kFragBytes;
+  size_t const rs = static_cast<size_t>(kblocks) * NP * kFragBytes, skip = static_cast<size_t>(s0) * H::kDepth * kFragBytes;
   HalfAcc<H> acc;
   half_gemm<T, T, NP>(acc, P + ti * (T / 32) * rs + skip, Q + tj * (T / 32) * rs + skip, rs, rs, count);
   int const lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -838,7 +838,7 @@ CePlan ce_plan(dlmi_ctx const *ctx, size_t B, size_t K, size_t V, bool back) {
     p.wt = take(packed_bytes(p.Kp, p.Vc, NP));
     p.dlb = take(packed_bytes(p.Bp, p.Vc, NP));
     p.dlv = take(packed_bytes(p.Vc, p.Bp, NP));
-    size_t const dxt = p.Bp / T * (p.Kp / T), stages = p.Vc / 16 * NP / 2;
+    size_t const dxt = p.Bp / T * (p.Kp / T), stages = dlmi_ceil_div(p.Vc, T == 64 ? 64 / NP : 32 / NP);
     size_t s = static_cast<size_t>(ctx->num_cu) * (T >= 256 ? 1 : 2) / dxt;
     if (s < 1) s = 1;
     if (s > 16) s = 16;
@@ -859,6 +859,8 @@ struct CeRun {
   CePlan p;
   char *s;
 
+  // stages of the K loop over k values (padded rows of zeros follow them to a whole stage)
+  static unsigned ce_stages(int T, size_t k) { return static_cast<unsigned>(dlmi_ceil_div(k, (T == 64 ? 64 : 32) / NP)); }
   float *floats(size_t at) const { return reinterpret_cast<float *>(s + at); }
 
   int pack_rows() const {
@@ -905,7 +907,7 @@ struct CeRun {
     g.ni = static_cast<unsigned>(vp / p.T);
     g.nj = static_cast<unsigned>(p.Bp / p.T);
     g.kblocks = static_cast<unsigned>(p.Kp / 16);
-    g.stages = static_cast<unsigned>(dlmi_ceil_div(a.K, 32 / NP));
+    g.stages = ce_stages(p.T, a.K);
     g.v0 = v0;
     g.vn = vn;
     return g;
@@ -954,13 +956,13 @@ struct CeRun {
         DLMI_LAUNCH_CHECK(ctx, "k_ce_db");
       }
       if (a.dX != nullptr) {
-        hipLaunchKernelGGL((k_ce_dx<T, NP>), dim3(nb * nk * p.slices), dim3(256), 0, ctx->stream, s + p.dlb, s + p.wt, nb, nk, kv, kv * NP / 2,
+        hipLaunchKernelGGL((k_ce_dx<T, NP>), dim3(nb * nk * p.slices), dim3(256), 0, ctx->stream, s + p.dlb, s + p.wt, nb, nk, kv, ce_stages(T, vp),
                            p.per_slice, floats(p.unscale), floats(p.dxacc), a.B, a.K, v0 == 0 ? 1 : 0);
         DLMI_LAUNCH_CHECK(ctx, "k_ce_dx");
       }
       if (a.dW != nullptr) {
         hipLaunchKernelGGL((k_ce_dw<T, NP, E>), dim3(g.ni * nk), dim3(256), 0, ctx->stream, s + p.dlv, s + p.xg, g.ni, nk, kb,
-                           static_cast<unsigned>(dlmi_ceil_div(a.B, 32 / NP)), floats(p.unscale) + 1, a.scale, static_cast<E *>(a.dW) + v0 * a.K, vn, a.K,
+                           ce_stages(T, a.B), floats(p.unscale) + 1, a.scale, static_cast<E *>(a.dW) + v0 * a.K, vn, a.K,
                            a.accumulate);
         DLMI_LAUNCH_CHECK(ctx, "k_ce_dw");
       }
