@@ -40,7 +40,8 @@ __device__ __forceinline__ unsigned xcd_consecutive(unsigned id, unsigned n) {
 // One step of the K loop reads one stage of LDS: KS k blocks of all planes of the BM + BN rows, four stages in all.  64 x 64
 // tiles take twice the k blocks of the others per stage: their stages are short, and three of them ahead is less than a load
 // takes.
-template <int BM, int BN, int NP>
+// NP: planes that are multiplied; MP: planes that lie in memory (of two, the first alone may be read).
+template <int BM, int BN, int NP, int MP = NP>
 struct HalfTile {
   static constexpr int kPlanes = NP;
   static constexpr int kDepth = BM + BN <= 128 ? 4 : 2;      // fragments of a row block in a stage
@@ -49,6 +50,9 @@ struct HalfTile {
   static constexpr int kFragsA = BM / 32 * kDepth, kFragsB = BN / 32 * kDepth;  // fragments of a stage
   static constexpr int kStageBytes = (kFragsA + kFragsB) * kFragBytes;
   static constexpr int kLoads = (kFragsA + kFragsB) / 4;     // direct loads of a wavefront per stage
+  static constexpr int kStep = KS * MP * kFragBytes;         // bytes from a row block's stage to its next
+  // where fragment f of an operand's stage lies in its row block: plane f % NP of k block f / NP
+  static __host__ __device__ constexpr int at(int f) { return (f % kDepth / NP * MP + f % NP) * kFragBytes; }
 };
 
 template <class T>
@@ -56,22 +60,21 @@ struct HalfAcc {
   f32x16 v[T::kMB][T::kNB];
 };
 
-template <int BM, int BN, int NP>
+template <class T>
 __device__ __forceinline__ void half_stage_load(char *lds, char const *P, char const *Q, size_t row_stride_p,
                                                 size_t row_stride_q, int wave, int lane) {
-  using T = HalfTile<BM, BN, NP>;
-  // fragment f of an operand: row block f / kDepth, the (f % kDepth)-th KiB of its KS k blocks x NP planes
+  // fragment f of an operand: of row block f / kDepth
 #pragma unroll
   for (int u = 0; u < T::kFragsA / 4; ++u) {
     int const f = u * 4 + wave;
-    char const *src = P + static_cast<size_t>(f / T::kDepth) * row_stride_p + (f % T::kDepth) * kFragBytes + lane * 16;
+    char const *src = P + static_cast<size_t>(f / T::kDepth) * row_stride_p + T::at(f) + lane * 16;
     __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void const *)src,
                                      (__attribute__((address_space(3))) void *)(lds + f * kFragBytes), 16, 0, 0);
   }
 #pragma unroll
   for (int u = 0; u < T::kFragsB / 4; ++u) {
     int const f = u * 4 + wave;
-    char const *src = Q + static_cast<size_t>(f / T::kDepth) * row_stride_q + (f % T::kDepth) * kFragBytes + lane * 16;
+    char const *src = Q + static_cast<size_t>(f / T::kDepth) * row_stride_q + T::at(f) + lane * 16;
     __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void const *)src,
                                      (__attribute__((address_space(3))) void *)(lds + (T::kFragsA + f) * kFragBytes), 16,
                                      0, 0);
@@ -158,10 +161,8 @@ __device__ __forceinline__ void half_schedule() {
 
 // The K loop of one workgroup (256 threads, wavefronts 2 x 2) over `stages` >= 1 stages.  P, Q: the first fragment of the
 // tile's first row block at the first k block; row_stride_*: bytes from one row block to the next.
-template <int BM, int BN, int NP>
-__device__ __forceinline__ void half_gemm(HalfAcc<HalfTile<BM, BN, NP>> &acc, char const *P, char const *Q,
-                                          size_t row_stride_p, size_t row_stride_q, int stages) {
-  using T = HalfTile<BM, BN, NP>;
+template <class T>
+__device__ __forceinline__ void half_gemm(HalfAcc<T> &acc, char const *P, char const *Q, size_t row_stride_p, size_t row_stride_q, int stages) {
   __shared__ __attribute__((aligned(1024))) char buf0[T::kStageBytes];
   __shared__ __attribute__((aligned(1024))) char buf1[T::kStageBytes];
   __shared__ __attribute__((aligned(1024))) char buf2[T::kStageBytes];
@@ -176,8 +177,7 @@ __device__ __forceinline__ void half_gemm(HalfAcc<HalfTile<BM, BN, NP>> &acc, ch
     for (int n = 0; n < T::kNB; ++n) acc.v[m][n] = f32x16{};
 
   auto const load = [&](char *buf, int t) {
-    half_stage_load<BM, BN, NP>(buf, P + static_cast<size_t>(t) * T::kDepth * kFragBytes, Q + static_cast<size_t>(t) * T::kDepth * kFragBytes,
-                                row_stride_p, row_stride_q, wave, lane);
+    half_stage_load<T>(buf, P + static_cast<size_t>(t) * T::kStep, Q + static_cast<size_t>(t) * T::kStep, row_stride_p, row_stride_q, wave, lane);
   };
   // the first three stages are requested before the first is waited for
   load(bufs[0], 0);
@@ -291,9 +291,9 @@ __device__ __forceinline__ void half_part_store(float *part, HalfAcc<T> const &a
 }
 
 // The parts of the shared tiles.  operands(tile, P, Q): a tile's operands at its first stage.
-template <int BM, int BN, int NP, class Operands>
+template <class T, class Operands>
 __device__ __forceinline__ void half_gemm_parts(HalfShares const &s, size_t row_stride_p, size_t row_stride_q, Operands &&operands) {
-  using T = HalfTile<BM, BN, NP>;
+  constexpr int kTile = 4 * T::kMB * T::kNB * 1024;
   unsigned const g = xcd_consecutive(blockIdx.x, gridDim.x);
   unsigned long long u = g * s.total / s.grid;
   unsigned long long const u1 = (g + 1ull) * s.total / s.grid;
@@ -306,9 +306,9 @@ __device__ __forceinline__ void half_gemm_parts(HalfShares const &s, size_t row_
     operands(s.whole + shared, P, Q);
     HalfAcc<T> acc;
     __syncthreads();  // the stages of the part before have been read
-    half_gemm<BM, BN, NP>(acc, P + static_cast<size_t>(from) * T::kDepth * kFragBytes, Q + static_cast<size_t>(from) * T::kDepth * kFragBytes,
-                          row_stride_p, row_stride_q, static_cast<int>((to < s.stages ? to : s.stages) - from));
-    half_part_store(s.parts + (static_cast<size_t>(g) * 2 + (shared == first ? 0 : 1)) * (BM * BN), acc);
+    half_gemm<T>(acc, P + static_cast<size_t>(from) * T::kStep, Q + static_cast<size_t>(from) * T::kStep, row_stride_p, row_stride_q,
+                 static_cast<int>((to < s.stages ? to : s.stages) - from));
+    half_part_store(s.parts + (static_cast<size_t>(g) * 2 + (shared == first ? 0 : 1)) * kTile, acc);
     u = end;
   }
 }

@@ -12,7 +12,9 @@
 // Precision.  The polynomial multiplies what lies in weak directions by up to a^steps (485 for 5 steps of 3.4445), the
 // rounding of the operands among it.  With one f16 plane a random matrix ends 1.3e-3 off and a matrix of rank 32 plus 1 %
 // noise 2.7e-2; with two planes (22 bits) 1.8e-6 and 1.2e-5, as far as a computation in fp32 (1.1e-5 and 1.9e-5).  So X,
-// A and a I + b A + c A A keep two planes throughout, whatever the type of the result.  Singular values stay below about 1.3
+// A and a I + b A + c A A keep two planes; only the last step of a bf16 result multiplies the first plane alone (11 bits: 4.5e-4
+// on random matrices, 1.0e-3 on the rank 32 one, under the 1.7e-3 of rounding the result to 8 bits; two such steps would be
+// at 7.5e-4 and 2.5e-3).  Singular values stay below about 1.3
 // and the polynomial in A between -3 and 4, so all three matrices are held times 2^12: far from the ends of f16's range.
 //
 // X is kept both ways round (rows i, k = j for X X^T; rows j, k = i for the product by X), each written by the product
@@ -200,14 +202,14 @@ __device__ __forceinline__ MuonTile muon_tile(MuonSymmetric const &a, unsigned t
   return t;
 }
 
-template <int T, bool POLY>
+template <int T, int NP, bool POLY>
 __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_muon_symmetric(MuonSymmetric a, unsigned stages) {
-  using H = HalfTile<T, T, 2>;
+  using H = HalfTile<T, T, NP, 2>;
   MuonTile const t = muon_tile(a, xcd_consecutive(blockIdx.x, gridDim.x));
   size_t const rs = static_cast<size_t>(a.kblocks) * 2 * kFragBytes;
   char const *const p = a.P + t.mat * a.stride_p;
   HalfAcc<H> acc;
-  half_gemm<T, T, 2>(acc, p + t.ti * (T / 32) * rs, p + t.tj * (T / 32) * rs, rs, rs, stages);
+  half_gemm<H>(acc, p + t.ti * (T / 32) * rs, p + t.tj * (T / 32) * rs, rs, rs, stages);
   int const lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   half8 const id0 = half_identity(0, lane), id1 = half_identity(1, lane);
 #pragma unroll
@@ -218,10 +220,10 @@ __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_muon_symmetric(MuonSy
                                  acc.v[m][n], id0, id1, lane);
 }
 
-template <int T>
+template <int T, int NP>
 __global__ __launch_bounds__(256, 1) void k_muon_symmetric_parts(MuonSymmetric a, HalfShares shares) {
   size_t const rs = static_cast<size_t>(a.kblocks) * 2 * kFragBytes;
-  half_gemm_parts<T, T, 2>(shares, rs, rs, [&](unsigned tile, char const *&p, char const *&q) {
+  half_gemm_parts<HalfTile<T, T, NP, 2>>(shares, rs, rs, [&](unsigned tile, char const *&p, char const *&q) {
     MuonTile const t = muon_tile(a, tile);
     p = a.P + t.mat * a.stride_p + t.ti * (T / 32) * rs;
     q = a.P + t.mat * a.stride_p + t.tj * (T / 32) * rs;
@@ -229,9 +231,9 @@ __global__ __launch_bounds__(256, 1) void k_muon_symmetric_parts(MuonSymmetric a
 }
 
 // The blocks of the shared tiles, a wavefront each.
-template <int T, bool POLY>
+template <int T, int NP, bool POLY>
 __global__ __launch_bounds__(256) void k_muon_symmetric_join(MuonSymmetric a, HalfShares shares) {
-  using H = HalfTile<T, T, 2>;
+  using H = HalfTile<T, T, NP, 2>;
   constexpr unsigned kBlocks = (T / 32) * (T / 32), kWave = H::kMB * H::kNB;
   int const lane = threadIdx.x & 63;
   unsigned const id = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), shared = id / kBlocks, block = id % kBlocks;
@@ -315,13 +317,13 @@ __device__ __forceinline__ MuonTile muon_tile(MuonUpdate const &a, unsigned tile
   return t;
 }
 
-template <int T, int MODE, class O>
+template <int T, int NP, int MODE, class O>
 __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_muon_update(MuonUpdate a, MuonBatch b, unsigned stages) {
-  using H = HalfTile<T, T, 2>;
+  using H = HalfTile<T, T, NP, 2>;
   MuonTile const t = muon_tile(a, xcd_consecutive(blockIdx.x, gridDim.x));
   size_t const rs = static_cast<size_t>(a.kbm) * 2 * kFragBytes;
   HalfAcc<H> acc;
-  half_gemm<T, T, 2>(acc, a.Bm + t.mat * a.stride_b + t.ti * (T / 32) * rs, a.XT + t.mat * a.stride_x + t.tj * (T / 32) * rs, rs, rs, stages);
+  half_gemm<H>(acc, a.Bm + t.mat * a.stride_b + t.ti * (T / 32) * rs, a.XT + t.mat * a.stride_x + t.tj * (T / 32) * rs, rs, rs, stages);
   int const lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   half8 const id0 = half_identity(0, lane), id1 = half_identity(1, lane);
 #pragma unroll
@@ -332,19 +334,19 @@ __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_muon_update(MuonUpdat
                                  acc.v[m][n], id0, id1, lane);
 }
 
-template <int T>
+template <int T, int NP>
 __global__ __launch_bounds__(256, 1) void k_muon_update_parts(MuonUpdate a, HalfShares shares) {
   size_t const rs = static_cast<size_t>(a.kbm) * 2 * kFragBytes;
-  half_gemm_parts<T, T, 2>(shares, rs, rs, [&](unsigned tile, char const *&p, char const *&q) {
+  half_gemm_parts<HalfTile<T, T, NP, 2>>(shares, rs, rs, [&](unsigned tile, char const *&p, char const *&q) {
     MuonTile const t = muon_tile(a, tile);
     p = a.Bm + t.mat * a.stride_b + t.ti * (T / 32) * rs;
     q = a.XT + t.mat * a.stride_x + t.tj * (T / 32) * rs;
   });
 }
 
-template <int T, int MODE, class O>
+template <int T, int NP, int MODE, class O>
 __global__ __launch_bounds__(256) void k_muon_update_join(MuonUpdate a, MuonBatch b, HalfShares shares) {
-  using H = HalfTile<T, T, 2>;
+  using H = HalfTile<T, T, NP, 2>;
   constexpr unsigned kBlocks = (T / 32) * (T / 32), kWave = H::kMB * H::kNB;
   int const lane = threadIdx.x & 63;
   unsigned const id = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), shared = id / kBlocks, block = id % kBlocks;
@@ -414,38 +416,50 @@ static HalfShares muon_shares(MuonPlan const &pl, unsigned tiles, unsigned stage
   return half_shares(tiles, stages, share ? pl.workgroups : tiles, parts);
 }
 
-template <int T, bool POLY>
+template <int T, int NP, bool POLY>
 static int muon_symmetric(dlmi_ctx *ctx, MuonSymmetric const &a, HalfShares const &shares) {
   if (shares.whole != 0) {
-    hipLaunchKernelGGL((k_muon_symmetric<T, POLY>), dim3(shares.whole), dim3(256), 0, ctx->stream, a, shares.stages);
+    hipLaunchKernelGGL((k_muon_symmetric<T, NP, POLY>), dim3(shares.whole), dim3(256), 0, ctx->stream, a, shares.stages);
     DLMI_LAUNCH_CHECK(ctx, "k_muon_symmetric");
   }
   if constexpr (T == 256) {
     if (shares.total == 0) return DLMI_OK;
-    hipLaunchKernelGGL(k_muon_symmetric_parts<T>, dim3(shares.grid), dim3(256), 0, ctx->stream, a, shares);
+    hipLaunchKernelGGL((k_muon_symmetric_parts<T, NP>), dim3(shares.grid), dim3(256), 0, ctx->stream, a, shares);
     DLMI_LAUNCH_CHECK(ctx, "k_muon_symmetric_parts");
     unsigned const blocks = (shares.tiles - shares.whole) * (T / 32) * (T / 32) / 4;
-    hipLaunchKernelGGL((k_muon_symmetric_join<T, POLY>), dim3(blocks), dim3(256), 0, ctx->stream, a, shares);
+    hipLaunchKernelGGL((k_muon_symmetric_join<T, NP, POLY>), dim3(blocks), dim3(256), 0, ctx->stream, a, shares);
     DLMI_LAUNCH_CHECK(ctx, "k_muon_symmetric_join");
   }
   return DLMI_OK;
 }
 
-template <int T, int MODE, class O>
+template <int T, int NP, int MODE, class O>
 static int muon_update(dlmi_ctx *ctx, MuonUpdate const &a, MuonBatch const &b, HalfShares const &shares) {
   if (shares.whole != 0) {
-    hipLaunchKernelGGL((k_muon_update<T, MODE, O>), dim3(shares.whole), dim3(256), 0, ctx->stream, a, b, shares.stages);
+    hipLaunchKernelGGL((k_muon_update<T, NP, MODE, O>), dim3(shares.whole), dim3(256), 0, ctx->stream, a, b, shares.stages);
     DLMI_LAUNCH_CHECK(ctx, "k_muon_update");
   }
   if constexpr (T == 256) {
     if (shares.total == 0) return DLMI_OK;
-    hipLaunchKernelGGL(k_muon_update_parts<T>, dim3(shares.grid), dim3(256), 0, ctx->stream, a, shares);
+    hipLaunchKernelGGL((k_muon_update_parts<T, NP>), dim3(shares.grid), dim3(256), 0, ctx->stream, a, shares);
     DLMI_LAUNCH_CHECK(ctx, "k_muon_update_parts");
     unsigned const blocks = (shares.tiles - shares.whole) * (T / 32) * (T / 32) / 4;
-    hipLaunchKernelGGL((k_muon_update_join<T, MODE, O>), dim3(blocks), dim3(256), 0, ctx->stream, a, b, shares);
+    hipLaunchKernelGGL((k_muon_update_join<T, NP, MODE, O>), dim3(blocks), dim3(256), 0, ctx->stream, a, b, shares);
     DLMI_LAUNCH_CHECK(ctx, "k_muon_update_join");
   }
   return DLMI_OK;
+}
+
+// A step of the iteration, NP planes multiplied.
+template <int T, int NP, int MODE, class O>
+static int muon_one(dlmi_ctx *ctx, MuonPlan const &pl, MuonBatch const &b, MuonSymmetric const &g, MuonSymmetric const &q, MuonUpdate const &u,
+                    unsigned count, float *parts) {
+  constexpr unsigned KS = HalfTile<T, T, NP, 2>::KS;
+  unsigned const tri = u.mt * (u.mt + 1) / 2 * count;
+  int rc = muon_symmetric<T, NP, false>(ctx, g, muon_shares(pl, tri, u.kbn / KS, parts));
+  if (rc == DLMI_OK) rc = muon_symmetric<T, NP, true>(ctx, q, muon_shares(pl, tri, u.kbm / KS, parts));
+  if (rc == DLMI_OK) rc = muon_update<T, NP, MODE, O>(ctx, u, b, muon_shares(pl, u.mt * u.nt * count, u.kbm / KS, parts));
+  return rc;
 }
 
 template <int T, class O, bool STEP>
@@ -453,27 +467,17 @@ static int muon_iterate(dlmi_ctx *ctx, MuonBatch const &b, MuonPlan const &pl, u
                         MuonOut const &o, char *XP, char *XT, char *XTn, char *A, char *Bm, float *parts) {
   unsigned const mt = static_cast<unsigned>(pl.mp / T), nt = static_cast<unsigned>(pl.np / T);
   unsigned const kbm = static_cast<unsigned>(pl.mp / 16), kbn = static_cast<unsigned>(pl.np / 16);
-  constexpr unsigned KS = HalfTile<T, T, 2>::KS;
-  unsigned const tri = mt * (mt + 1) / 2 * count, all = mt * nt * count;
-  HalfShares const gram = muon_shares(pl, tri, kbn / KS, parts), square = muon_shares(pl, tri, kbm / KS, parts),
-                   product = muon_shares(pl, all, kbm / KS, parts);
   MuonSymmetric const g{XP, A, pl.bytes_x, pl.bytes_a, mt, kbn, kbm, 0.0f, 0.0f, 1.0f};
   MuonSymmetric const q{A, Bm, pl.bytes_a, pl.bytes_a, mt, kbm, kbm, coefs[0], coefs[1], coefs[2]};
   MuonUpdate u{Bm, XT, XTn, XP, pl.bytes_a, pl.bytes_x, mt, nt, kbm, kbn, o};
-  for (int s = 0; s < steps; ++s) {
-    int rc = muon_symmetric<T, false>(ctx, g, gram);
-    if (rc == DLMI_OK) rc = muon_symmetric<T, true>(ctx, q, square);
-    if (rc != DLMI_OK) return rc;
-    if (s + 1 < steps)
-      rc = muon_update<T, kMuonMore, O>(ctx, u, b, product);
-    else
-      rc = muon_update<T, STEP ? kMuonStep : kMuonOut, O>(ctx, u, b, product);
+  for (int s = 0; s + 1 < steps; ++s) {
+    int const rc = muon_one<T, 2, kMuonMore, O>(ctx, pl, b, g, q, u, count, parts);
     if (rc != DLMI_OK) return rc;
     char *const x = const_cast<char *>(u.XT);
     u.XT = u.XTn;
     u.XTn = x;
   }
-  return DLMI_OK;
+  return muon_one<T, sizeof(O) == 2 ? 1 : 2, STEP ? kMuonStep : kMuonOut, O>(ctx, pl, b, g, q, u, count, parts);
 }
 
 // `count` matrices of one shape, at most kMuonMax of them; the scratch has been reserved.

@@ -245,7 +245,7 @@ __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_stats(CeArgs a, Ce
   ce_tile(xcd_consecutive(blockIdx.x, gridDim.x), g.ni, g.nj, ti, tj);
   size_t const rs = static_cast<size_t>(g.kblocks) * NP * kFragBytes;
   HalfAcc<H> acc;
-  half_gemm<T, T, NP>(acc, g.P + ti * (T / 32) * rs, g.Q + tj * (T / 32) * rs, rs, rs, g.stages);
+  half_gemm<H>(acc, g.P + ti * (T / 32) * rs, g.Q + tj * (T / 32) * rs, rs, rs, g.stages);
   int const lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   float const uw = g.unscale_w[0];
   size_t const c0 = static_cast<size_t>(ti) * T + (wave >> 1) * (T / 2);
@@ -632,7 +632,7 @@ __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_grad(CeArgs a, CeL
   ce_tile(xcd_consecutive(blockIdx.x, gridDim.x), g.ni, g.nj, ti, tj);
   size_t const rs = static_cast<size_t>(g.kblocks) * NP * kFragBytes;
   HalfAcc<H> acc;
-  half_gemm<T, T, NP>(acc, g.P + ti * (T / 32) * rs, g.Q + tj * (T / 32) * rs, rs, rs, g.stages);
+  half_gemm<H>(acc, g.P + ti * (T / 32) * rs, g.Q + tj * (T / 32) * rs, rs, rs, g.stages);
   int const lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   half8 const id0 = half_identity(0, lane), id1 = half_identity(1, lane);
   float const uw = g.unscale_w[0];
@@ -731,7 +731,7 @@ __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_dw(char const *P, 
   ce_tile(xcd_consecutive(blockIdx.x, gridDim.x), ni, nj, ti, tj);
   size_t const rs = static_cast<size_t>(kblocks) * NP * kFragBytes;
   HalfAcc<H> acc;
-  half_gemm<T, T, NP>(acc, P + ti * (T / 32) * rs, Q + tj * (T / 32) * rs, rs, rs, stages);
+  half_gemm<H>(acc, P + ti * (T / 32) * rs, Q + tj * (T / 32) * rs, rs, rs, stages);
   int const lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   float const factor = unscale[0] * (scale * (1.0f / kCeDl));
 #pragma unroll
@@ -755,9 +755,9 @@ __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_dx(char const *P, 
   unsigned const s0 = slice * per_slice;
   if (s0 >= stages) return;  // a shorter last piece (the first has work for every slice)
   unsigned const count = stages - s0 < per_slice ? stages - s0 : per_slice;
-  size_t const rs = static_cast<size_t>(kblocks) * NP * kFragBytes, skip = static_cast<size_t>(s0) * H::kDepth * kFragBytes;
+  size_t const rs = static_cast<size_t>(kblocks) * NP * kFragBytes, skip = static_cast<size_t>(s0) * H::kStep;
   HalfAcc<H> acc;
-  half_gemm<T, T, NP>(acc, P + ti * (T / 32) * rs + skip, Q + tj * (T / 32) * rs + skip, rs, rs, count);
+  half_gemm<H>(acc, P + ti * (T / 32) * rs + skip, Q + tj * (T / 32) * rs + skip, rs, rs, count);
   int const lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   float const factor = unscale[0] * (1.0f / kCeDl);
   out += slice * rows * cols;
