@@ -364,7 +364,9 @@ struct HalfBlock {
   HalfPair pl[NP];
 };
 
-// Rounds the block to its planes (each to nearest even; the second holds what the first lost).
+// Rounds the block to its planes (each to nearest even; the second holds what the first lost).  The empty asm makes the
+// value one of fp32 before it is rounded: the compiler may otherwise fold a product before it into one of the two uses of
+// `hi` (a multiplication that rounds to f16 at once), and a value near a tie then loses a whole step of its first plane.
 template <int NP>
 __device__ __forceinline__ HalfBlock<NP> half_split(f32x16 const &v) {
   half4 h[4], l[4];
@@ -372,7 +374,8 @@ __device__ __forceinline__ HalfBlock<NP> half_split(f32x16 const &v) {
   for (int q = 0; q < 4; ++q)
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      float const x = v[q * 4 + t];
+      float x = v[q * 4 + t];
+      if constexpr (NP == 2) asm("" : "+v"(x));
       _Float16 const hi = static_cast<_Float16>(x);
       h[q][t] = hi;
       if constexpr (NP == 2) l[q][t] = static_cast<_Float16>(x - static_cast<float>(hi));

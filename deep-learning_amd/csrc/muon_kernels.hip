@@ -143,7 +143,8 @@ __global__ __launch_bounds__(kMuonBlock) void k_muon_pack(MuonBatch b, unsigned 
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
       int const row = rb * 32 + (lane & 31), k = kb * 16 + (lane >> 5) * 8 + t;
-      float const x = flip ? tile[k][row] : tile[row][k];
+      float x = flip ? tile[k][row] : tile[row][k];
+      asm("" : "+v"(x));  // (one value for both planes)
       _Float16 const h = static_cast<_Float16>(x);
       hi[t] = h;
       lo[t] = static_cast<_Float16>(x - static_cast<float>(h));

@@ -10,12 +10,14 @@
 // Bound by the 16-bit matrix pipe: 2 B K V operations forward, 6 B K V backward, times three for the two planes of an fp32
 // input (half_gemm.hpp); by reading W where there are few rows.
 //
-// Operands are packed as f16 planes of powers-of-two multiples: a row of X by its own largest magnitude (a padding row
-// full of garbage spoils nobody's scale), a piece of W by its own.  bf16 values have 8 bits and one plane holds them
-// exactly; fp32 values take two planes.  dL is in [-1, 1] and held times 2^15, rounded to 11 bits (bf16; the result keeps 8)
-// or 22 (fp32).  For dW, whose sum runs over the rows, X is packed times dloss (one more rounding for bf16, none without
-// dloss), rows left out as zeros; the common factor comes last.
+// Operands are packed as f16 planes of powers-of-two multiples, each row of X and of W by its own largest magnitude (a
+// padding row full of garbage spoils nobody's scale).  bf16 values have 8 bits and one plane holds them exactly; fp32
+// values take two planes.  dL is in [-1, 1] and held times 2^15, rounded to 11 bits (bf16; the result keeps 8) or 22 (fp32).
+// Where a product's sum runs over rows that are scaled differently (dX over W's, dW over X's), dL carries what undoes the
+// scale, and dloss, as a share of the largest such factor, which multiplies the result.
 #pragma once
+
+#include <cmath>
 
 #include "half_gemm.hpp"
 
@@ -43,7 +45,6 @@ int ce_backward(dlmi_ctx *ctx, CeArgs const &a);
 #ifdef DLMI_CE_IMPLEMENTATION
 
 constexpr int kCeBlock = 256;
-constexpr unsigned kCeMaxParts = 1024;     // partial maxima of a piece of W
 constexpr float kCeDl = 32768.0f;         // dL is held times this
 
 template <class T>
@@ -78,123 +79,121 @@ __device__ __forceinline__ float ce_row_weight(CeArgs const &a, size_t b) {
   return a.dloss != nullptr ? a.dloss[b] : 1.0f;
 }
 
-// A wavefront per row: rowmax[row] (may be null) and the largest of all rows per block in parts (may be null); `weighted`:
-// of dloss x instead of x, rows left out not looked at.
-template <class T>
-__global__ __launch_bounds__(kCeBlock) void k_ce_max(CeArgs a, T const *src, size_t rows, size_t cols, float *rowmax, float *parts,
-                                                     int weighted) {
-  __shared__ float lds[kCeBlock / 64];
-  int const lane = threadIdx.x & 63;
-  float all = 0.0f;
-  for (size_t r = static_cast<size_t>(blockIdx.x) * (kCeBlock / 64) + (threadIdx.x >> 6); r < rows;
-       r += static_cast<size_t>(gridDim.x) * (kCeBlock / 64)) {
-    float const g = weighted ? ce_row_weight(a, r) : 1.0f;
-    float m = 0.0f;
-    if (g != 0.0f) {
-      T const *const row = src + r * cols;
-      size_t c = static_cast<size_t>(lane) * 8;
-      for (; c + 8 <= cols; c += 512) {
-        CeOct<T> const o = *reinterpret_cast<CeOct<T> const *>(row + c);
-#pragma unroll
-        for (int t = 0; t < 8; ++t) m = ce_finite_max(m, static_cast<float>(o.v[t]) * g);
-      }
-      for (; c < cols; ++c) m = ce_finite_max(m, static_cast<float>(row[c]) * g);
-    }
-    m = ce_wave_max(m);
-    if (rowmax != nullptr && lane == 0) rowmax[r] = m;
-    all = fmaxf(all, m);
-  }
-  if (parts == nullptr) return;
-  if (lane == 0) lds[threadIdx.x >> 6] = all;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < kCeBlock / 64; ++w) all = fmaxf(all, lds[w]);
-    parts[blockIdx.x] = all;
-  }
+// The largest of n values, the same in all lanes of a wavefront.
+__device__ __forceinline__ float ce_largest(float const *v, unsigned n, int lane) {
+  float m = 0.0f;
+#pragma unroll 4
+  for (unsigned q = lane; q < n; q += 64) m = fmaxf(m, v[q]);
+  return ce_wave_max(m);
 }
 
-// A 64 x 64 tile of src [rows, cols], scaled and packed as it stands (`as`: row r, k = c) and / or transposed (`across`: row
-// c, k = r), padding zero.  The scale: of the row (rowmax) or of the largest of parts[nparts]; its inverse goes to
-// unscale (one value per row, or one).  weighted: times dloss of the row, rows left out zero.
-template <class T, int NP>
+// Rows of src [rows, cols], each scaled by its own largest magnitude and packed as it stands (`as`: row r, k = c) and / or
+// transposed (`across`: row c, k = r), padding zero.  unscale[r]: the inverse scale; parts[workgroup]: the largest of weight
+// times unscale of the workgroup's rows.  LABELS (X): the weight is ce_row_weight, and rows left out are zero in `across`;
+// otherwise (W) it is 1.
+// A wavefront takes 8 rows, a lane 8 columns of one of them at a time, twice over the row: for the largest magnitude and for
+// the values (from the L2).  A lane's octet is a piece of a fragment as it stands; for the transposed ones the wavefront
+// turns 8 x 64 values through 2 KiB of LDS that only it uses.  ROWS = 32: each wavefront its own rows; 8: the four share the
+// columns of the same 8 rows (where there are too few rows to fill the device otherwise).
+template <class T, int NP, int ROWS, bool LABELS>
 __global__ __launch_bounds__(kCeBlock) void k_ce_pack(CeArgs a, T const *src, size_t rows, size_t cols, unsigned kblocks_as,
-                                                      unsigned kblocks_across, float const *rowmax, float const *parts, unsigned nparts,
-                                                      float *unscale, int weighted, char *as, char *across) {
-  __shared__ float tile[64][65];
-  __shared__ float lds[kCeBlock / 64];
-  int const lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  float scale = 1.0f;
-  if (parts != nullptr) {
-    float m = 0.0f;
+                                                      unsigned kblocks_across, float *unscale, float *parts, char *as, char *across) {
+  __shared__ float turn[4][8][68];
+  __shared__ float top[4][8];
+  int const lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int const r8 = lane >> 3, c8 = (lane & 7) * 8;
+  size_t const r0 = static_cast<size_t>(blockIdx.x) * ROWS + (ROWS == 32 ? wave * 8 : 0), r = r0 + r8;
+  unsigned const tiles = kblocks_as / 4;  // of 64 columns, padding included
+  unsigned const t0 = ROWS == 32 ? 0 : wave, step = ROWS == 32 ? 1 : 4;
+  T const *const row = src + (r < rows ? r : rows - 1) * cols;
+  // every load is made, whole (one that hangs over the row's end is moved back to end with it)
+  auto const load = [&](unsigned t) {
+    size_t const c = static_cast<size_t>(t) * 64 + c8;
+    return *reinterpret_cast<CeOct<T> const *>(row + (c + 8 <= cols ? c : cols - 8));
+  };
+  bool const narrow = cols < 8;
+  float m = 0.0f;
+  if (narrow) {
+    for (size_t c = 0; c < cols; ++c) m = ce_finite_max(m, static_cast<float>(row[c]));
+  } else {
+#pragma unroll 4
+    for (unsigned t = t0; t < tiles; t += step) {
+      CeOct<T> const o = load(t);
 #pragma unroll
-    for (unsigned q = 0; q < kCeMaxParts / kCeBlock; ++q) {
-      unsigned const at = q * kCeBlock + threadIdx.x;
-      m = fmaxf(m, at < nparts ? parts[at] : 0.0f);
+      for (int i = 0; i < 8; ++i) m = ce_finite_max(m, static_cast<float>(o.v[i]));
     }
-    m = ce_wave_max(m);
-    if (lane == 0) lds[wave] = m;
+  }
+#pragma unroll
+  for (int o = 1; o < 8; o *= 2) m = fmaxf(m, __shfl_xor(m, o));
+  if constexpr (ROWS == 8) {
+    if ((lane & 7) == 0) top[wave][r8] = m;
     __syncthreads();
-    scale = ce_scale(fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3])));
-    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) unscale[0] = ce_unscale(scale);
+    m = fmaxf(fmaxf(top[0][r8], top[1][r8]), fmaxf(top[2][r8], top[3][r8]));
   }
-  size_t const r0 = static_cast<size_t>(blockIdx.y) * 64, c0 = static_cast<size_t>(blockIdx.x) * 64;
-  // a thread takes 8 columns of two rows
-  int const tc = (threadIdx.x & 7) * 8;
-#pragma unroll
-  for (int q = 0; q < 2; ++q) {
-    int const tr = q * 32 + (threadIdx.x >> 3);
-    size_t const r = r0 + tr, c = c0 + tc;
+  float const scale = ce_scale(m);
+  bool live = r < rows;
+  float weight = live ? 1.0f : 0.0f;
+  if constexpr (LABELS) {
+    int const l = live ? a.labels[r] : -1;
+    live = l >= 0 && static_cast<size_t>(l) < a.V;
+    weight = live ? fabsf(ce_row_weight(a, r)) : 0.0f;
+  }
+  if ((lane & 7) == 0 && r < rows && (ROWS == 32 || wave == 0)) unscale[r] = ce_unscale(scale);
+  if (parts != nullptr) {
+    float const mine = ce_wave_max(weight * ce_unscale(scale));
+    if constexpr (ROWS == 32) {
+      if (lane == 0) top[wave][0] = mine;
+      __syncthreads();
+      if (threadIdx.x == 0) parts[blockIdx.x] = fmaxf(fmaxf(top[0][0], top[1][0]), fmaxf(top[2][0], top[3][0]));
+    } else if (threadIdx.x == 0) {
+      parts[blockIdx.x] = mine;
+    }
+  }
+#pragma unroll 2
+  for (unsigned t = t0; t < tiles; t += step) {
     float x[8];
+    size_t const c = static_cast<size_t>(t) * 64 + c8;
+    if (narrow) {
 #pragma unroll
-    for (int t = 0; t < 8; ++t) x[t] = 0.0f;
-    float s = scale, g = 1.0f;
-    if (r < rows) {
-      if (rowmax != nullptr) {
-        s = ce_scale(rowmax[r]);
-        if (blockIdx.x == 0 && tc == 0) unscale[r] = ce_unscale(s);
-      }
-      bool live = true;
-      if (weighted) {
-        int const l = a.labels[r];
-        live = l >= 0 && static_cast<size_t>(l) < a.V;
-        g = ce_row_weight(a, r);
-      }
-      if (live) {
-        T const *const p = src + r * cols + c;
-        if (c + 8 <= cols) {
-          CeOct<T> const o = *reinterpret_cast<CeOct<T> const *>(p);
+      for (int i = 0; i < 8; ++i) x[i] = r < rows && c + i < cols ? static_cast<float>(row[c + i < cols ? c + i : cols - 1]) * scale : 0.0f;
+    } else {
+      CeOct<T> const o = load(t);
 #pragma unroll
-          for (int t = 0; t < 8; ++t) x[t] = static_cast<float>(o.v[t]) * g * s;
-        } else {
-#pragma unroll
-          for (int t = 0; t < 8; ++t)
-            if (c + t < cols) x[t] = static_cast<float>(p[t]) * g * s;
-        }
+      for (int i = 0; i < 8; ++i) x[i] = r < rows && c + 8 <= cols ? static_cast<float>(o.v[i]) * scale : 0.0f;
+      if (c < cols && c + 8 > cols && r < rows) {  // the row's end: the octet was moved back by c + 8 - cols
+        for (int i = 0; i < 8; ++i)
+          if (c + i < cols) x[i] = static_cast<float>(row[c + i]) * scale;
       }
     }
+    auto const pack = [&](float const (&v)[8], char *dst) {
+      half8 hi, lo;
 #pragma unroll
-    for (int t = 0; t < 8; ++t) tile[tr][tc + t] = x[t];
-  }
-  __syncthreads();
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    int const f = q * 4 + wave;  // 16 fragments: 8 as it stands, 8 transposed
-    bool const flip = f >= 8;
-    if (flip ? across == nullptr : as == nullptr) continue;
-    int const rb = (f >> 2) & 1, kb = f & 3;
-    half8 hi, lo;
-#pragma unroll
-    for (int t = 0; t < 8; ++t) {
-      int const row = rb * 32 + (lane & 31), k = kb * 16 + (lane >> 5) * 8 + t;
-      float const x = flip ? tile[k][row] : tile[row][k];
-      _Float16 const h = static_cast<_Float16>(x);
-      hi[t] = h;
-      if constexpr (NP == 2) lo[t] = static_cast<_Float16>(x - static_cast<float>(h));
+      for (int i = 0; i < 8; ++i) {
+        float y = v[i];
+        if constexpr (NP == 2) asm("" : "+v"(y));  // (one value for both planes)
+        _Float16 const h = static_cast<_Float16>(y);
+        hi[i] = h;
+        if constexpr (NP == 2) lo[i] = static_cast<_Float16>(y - static_cast<float>(h));
+      }
+      *reinterpret_cast<half8 *>(dst) = hi;
+      if constexpr (NP == 2) *reinterpret_cast<half8 *>(dst + kFragBytes) = lo;
+    };
+    if (as != nullptr) {
+      size_t const frag = (r / 32) * kblocks_as + t * 4 + (lane & 7) / 2;
+      pack(x, as + frag * NP * kFragBytes + ((lane & 1) * 32 + (r & 31)) * 16);
     }
-    size_t const frag = flip ? (c0 / 32 + rb) * kblocks_across + r0 / 16 + kb : (r0 / 32 + rb) * kblocks_as + c0 / 16 + kb;
-    char *const dst = (flip ? across : as) + frag * NP * kFragBytes + lane * 16;
-    *reinterpret_cast<half8 *>(dst) = hi;
-    if constexpr (NP == 2) *reinterpret_cast<half8 *>(dst + kFragBytes) = lo;
+    if (across != nullptr) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) turn[wave][r8][c8 + i] = live ? x[i] : 0.0f;
+      __builtin_amdgcn_wave_barrier();
+      float y[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = turn[wave][i][lane];
+      __builtin_amdgcn_wave_barrier();
+      size_t const f = static_cast<size_t>(t) * 64 + lane;
+      size_t const frag = (f / 32) * kblocks_across + r0 / 16;
+      pack(y, across + frag * NP * kFragBytes + ((r0 / 8 & 1) * 32 + (f & 31)) * 16);
+    }
   }
 }
 
@@ -212,8 +211,10 @@ __device__ __forceinline__ float ce_join_factor(float m, float most) { return m 
 // The logits of a tile: classes i of the piece (P = W packed), rows j of the batch (Q = X packed).
 struct CeLogits {
   char const *P, *Q;
-  float const *unscale_x, *unscale_w;
-  unsigned ni, nj, kblocks, stages;  // kblocks: of a row block in memory
+  float const *unscale_x, *unscale_w;  // of the rows of the batch, of the piece's classes
+  float const *parts_x, *parts_w;      // their workgroups' largest (backward)
+  unsigned nparts_x, nparts_w;
+  unsigned ni, nj, kblocks, stages;    // kblocks: of a row block in memory
   size_t v0, vn;                     // first class of the piece, classes in it
 };
 
@@ -236,6 +237,18 @@ __device__ __forceinline__ f32x16 ce_biases(CeArgs const &a, CeLogits const &g, 
   return v;
 }
 
+// What undoes the scale of those classes.
+__device__ __forceinline__ f32x16 ce_unscales(CeLogits const &g, size_t c0, int lane) {
+  f32x16 v;
+  size_t const c1 = c0 + 4 * (lane >> 5);
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    size_t const c = c1 + 8 * (r >> 2) + (r & 3);
+    v[r] = g.unscale_w[c < g.vn ? c : g.vn - 1];
+  }
+  return v;
+}
+
 // part[half tile of classes][Bp] = (max, sum of exp(z - max)); target[b] = the label's logit.
 template <int T, int NP>
 __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_stats(CeArgs a, CeLogits g, float2 *part, size_t part_stride, size_t part_row0,
@@ -247,7 +260,6 @@ __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_stats(CeArgs a, Ce
   HalfAcc<H> acc;
   half_gemm<H>(acc, g.P + ti * (T / 32) * rs, g.Q + tj * (T / 32) * rs, rs, rs, g.stages);
   int const lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  float const uw = g.unscale_w[0];
   size_t const c0 = static_cast<size_t>(ti) * T + (wave >> 1) * (T / 2);
   size_t const b0 = static_cast<size_t>(tj) * T + (wave & 1) * (T / 2) + (lane & 31);
   float ux[H::kNB];
@@ -255,11 +267,11 @@ __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_stats(CeArgs a, Ce
   for (int n = 0; n < H::kNB; ++n) ux[n] = g.unscale_x[b0 + n * 32 < a.B ? b0 + n * 32 : a.B - 1];
 #pragma unroll
   for (int m = 0; m < H::kMB; ++m) {
-    f32x16 const bias = ce_biases(a, g, c0 + m * 32, lane);
+    f32x16 const bias = ce_biases(a, g, c0 + m * 32, lane), uw = ce_unscales(g, c0 + m * 32, lane);
 #pragma unroll
     for (int n = 0; n < H::kNB; ++n)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) acc.v[m][n][r] = acc.v[m][n][r] * ux[n] * uw + bias[r];
+      for (int r = 0; r < 16; ++r) acc.v[m][n][r] = acc.v[m][n][r] * ux[n] * uw[r] + bias[r];
   }
 #pragma unroll
   for (int n = 0; n < H::kNB; ++n) {
@@ -622,8 +634,9 @@ __device__ __forceinline__ float ce_scatter_sum(f32x16 const &v, int lane) {
   return d + ce_dpp<0xB1>(d);                 // lane ^ 1
 }
 
-// dL of a tile, packed for dX (rows of the batch, k = classes) and for dW (rows are classes, k = rows of the batch);
-// DB: also the sums of dloss dL over each half tile of rows.
+// dL of a tile, packed for dX (rows of the batch, k = classes; times what undoes the scale of W's row, as a share of the
+// piece's largest: a power of two) and for dW (rows are classes, k = rows of the batch; times dloss and what undoes the scale
+// of X's row, as a share of the largest): the factors of the products' k that do not come out of their sums.  DB: also the sums of dloss dL over each half tile of rows.
 template <int T, int NP, bool DB>
 __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_grad(CeArgs a, CeLogits g, char *dlb, char *dlv, unsigned kblocks_v,
                                                                   unsigned kblocks_b, float *dbpart, size_t dbpart_stride) {
@@ -635,12 +648,12 @@ __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_grad(CeArgs a, CeL
   half_gemm<H>(acc, g.P + ti * (T / 32) * rs, g.Q + tj * (T / 32) * rs, rs, rs, g.stages);
   int const lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   half8 const id0 = half_identity(0, lane), id1 = half_identity(1, lane);
-  float const uw = g.unscale_w[0];
+  float const most_w = ce_largest(g.parts_w, g.nparts_w, lane), most_x = ce_largest(g.parts_x, g.nparts_x, lane);
   size_t const c0 = static_cast<size_t>(ti) * T + (wave >> 1) * (T / 2);
   size_t const b0 = static_cast<size_t>(tj) * T + (wave & 1) * (T / 2);
   size_t const rb = static_cast<size_t>(kblocks_v) * NP * kFragBytes, rv = static_cast<size_t>(kblocks_b) * NP * kFragBytes;
-  // of this lane's rows of the batch: unscale, lse, weight, and the label's class from c0 on (-1: none here)
-  float ux[H::kNB], lse[H::kNB], weight[H::kNB];
+  // of this lane's rows of the batch: unscale, lse, weight, share of the largest, and the label's class from c0 on (-1: none here)
+  float ux[H::kNB], lse[H::kNB], weight[H::kNB], fx[H::kNB];
   int at[H::kNB];
   bool live[H::kNB];
 #pragma unroll
@@ -649,14 +662,16 @@ __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_grad(CeArgs a, CeL
     int const label = a.labels[in];
     ux[n] = g.unscale_x[in];
     lse[n] = a.lse_in[in];
-    weight[n] = DB && a.dloss != nullptr ? a.dloss[in] : 1.0f;
+    weight[n] = a.dloss != nullptr ? a.dloss[in] : 1.0f;
+    fx[n] = most_x > 0.0f ? weight[n] * ux[n] / most_x * kCeDl : 0.0f;
     live[n] = b < a.B && label >= 0 && static_cast<size_t>(label) < a.V;
     long long const c = static_cast<long long>(label) - static_cast<long long>(g.v0 + c0);
     at[n] = live[n] && c >= 0 && c < T / 2 ? static_cast<int>(c) : -1;
   }
 #pragma unroll
   for (int m = 0; m < H::kMB; ++m) {
-    f32x16 const bias = ce_biases(a, g, c0 + m * 32, lane);
+    f32x16 const bias = ce_biases(a, g, c0 + m * 32, lane), uw = ce_unscales(g, c0 + m * 32, lane);
+    f32x16 const fw = uw * (kCeDl / most_w);
     f32x16 sum = {};
     bool const whole = c0 + m * 32 + 32 <= g.vn;
 #pragma unroll
@@ -665,16 +680,15 @@ __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_grad(CeArgs a, CeL
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         int const c = m * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
-        float p = __expf(z[r] * ux[n] * uw + bias[r] - lse[n]);
+        float p = __expf(z[r] * ux[n] * uw[r] + bias[r] - lse[n]);
         p -= at[n] == c ? 1.0f : 0.0f;
         // (a class beyond the piece: its logit is -infinity, but a row's lse may be too)
         z[r] = live[n] && (whole || c0 + c < g.vn) ? p : 0.0f;
         if constexpr (DB) sum[r] += live[n] ? weight[n] * z[r] : 0.0f;
       }
       size_t const ib = c0 / 32 + m, jb = b0 / 32 + n;
-      HalfBlock<NP> const blk = half_split<NP>(z * kCeDl);
-      half_store<NP>(dlb + jb * rb + ib * 2 * NP * kFragBytes, blk, lane);
-      half_store<NP>(dlv + ib * rv + jb * 2 * NP * kFragBytes, half_flip<NP>(blk, id0, id1), lane);
+      half_store<NP>(dlb + jb * rb + ib * 2 * NP * kFragBytes, half_split<NP>(z * fw), lane);
+      half_store<NP>(dlv + ib * rv + jb * 2 * NP * kFragBytes, half_flip<NP>(half_split<NP>(z * fx[n]), id0, id1), lane);
     }
     if constexpr (DB) {
       float const s = ce_scatter_sum(sum, lane);
@@ -721,10 +735,10 @@ __device__ __forceinline__ void ce_block_out(f32x16 const &v, float factor, O *o
   }
 }
 
-// dW of a piece: classes i (P = dL packed by classes), features j (Q = dloss X packed by features), times `scale`.
+// dW of a piece: classes i (P = dL packed by classes), features j (Q = X packed by features), times `scale`.
 template <int T, int NP, class O>
 __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_dw(char const *P, char const *Q, unsigned ni, unsigned nj, unsigned kblocks,
-                                                                unsigned stages, float const *unscale, float scale, O *out, size_t rows,
+                                                                unsigned stages, float const *parts, unsigned nparts, float scale, O *out, size_t rows,
                                                                 size_t cols, int accumulate) {
   using H = HalfTile<T, T, NP>;
   unsigned ti, tj;
@@ -733,7 +747,7 @@ __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_dw(char const *P, 
   HalfAcc<H> acc;
   half_gemm<H>(acc, P + ti * (T / 32) * rs, Q + tj * (T / 32) * rs, rs, rs, stages);
   int const lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  float const factor = unscale[0] * (scale * (1.0f / kCeDl));
+  float const factor = ce_largest(parts, nparts, lane) * (scale * (1.0f / kCeDl));
 #pragma unroll
   for (int m = 0; m < H::kMB; ++m)
 #pragma unroll
@@ -746,7 +760,7 @@ __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_dw(char const *P, 
 // over the piece's classes of the slice into out [slice][rows][cols]; the first piece writes, later ones add.
 template <int T, int NP>
 __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_dx(char const *P, char const *Q, unsigned ni, unsigned nj, unsigned kblocks,
-                                                                unsigned stages, unsigned per_slice, float const *unscale, float *out,
+                                                                unsigned stages, unsigned per_slice, float const *parts, unsigned nparts, float *out,
                                                                 size_t rows, size_t cols, int first) {
   using H = HalfTile<T, T, NP>;
   unsigned ti, tj;
@@ -759,7 +773,7 @@ __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_dx(char const *P, 
   HalfAcc<H> acc;
   half_gemm<H>(acc, P + ti * (T / 32) * rs + skip, Q + tj * (T / 32) * rs + skip, rs, rs, count);
   int const lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  float const factor = unscale[0] * (1.0f / kCeDl);
+  float const factor = ce_largest(parts, nparts, lane) * (1.0f / kCeDl);
   out += slice * rows * cols;
 #pragma unroll
   for (int m = 0; m < H::kMB; ++m)
@@ -796,15 +810,30 @@ struct CePlan {
   int T;
   size_t Bp, Kp, Vc, pieces;       // padded rows and features; classes of a piece (a multiple of T)
   unsigned slices, per_slice;      // of dX
-  size_t row_blocks, wparts;
+  int rows_x, rows_w;              // rows of a packing workgroup (8 or 32)
+  unsigned nparts_x, nparts_w;
   // offsets in the scratch
-  size_t xp, xg, wp, wt, dlb, dlv, rowmax, parts, unscale, part, target, dxacc, dbpart, bytes;
+  size_t xp, xt, wp, wt, dlb, dlv, parts_x, parts_w, unscale_x, unscale_w, part, target, dxacc, dbpart, bytes;
 };
 
 template <int NP>
 CePlan ce_plan(dlmi_ctx const *ctx, size_t B, size_t K, size_t V, bool back) {
   CePlan p = {};
-  p.T = B > 512 ? 256 : (B > 64 ? 128 : 64);
+  // The tile with the least estimated time of all products: rounds of tiles over the CUs, the depth of their K loops, and what
+  // an element of a tile costs (measured relative rates; 128 x 128 tiles run two to a CU).  dX is cut into slices, so only
+  // its size counts.
+  double least = 0.0;
+  for (int t : {256, 128, 64}) {
+    double const cu = ctx->num_cu, cost = t == 256 ? 1.0 : t == 128 ? 1.25 : 2.5, d = t, b = dlmi_ceil_div(B, t), k = dlmi_ceil_div(K, t),
+                 v = dlmi_ceil_div(V, t);
+    auto const rounds = [&](double tiles) { return tiles <= cu ? 1.0 : tiles / cu < 4.0 ? std::ceil(tiles / cu) : tiles / cu; };
+    double time = rounds(b * v) * d * d * cost * static_cast<double>(dlmi_ceil_div(K, 64) * 64);
+    if (back) time += rounds(v * k) * d * d * cost * static_cast<double>(dlmi_ceil_div(B, 64) * 64) + b * k * v * d * d * d * cost / cu;
+    if (t == 256 || time < least) {
+      least = time;
+      p.T = t;
+    }
+  }
   size_t const T = p.T;
   auto const up = [](size_t x, size_t m) { return dlmi_ceil_div(x, m) * m; };
   p.Bp = up(B, T);
@@ -827,14 +856,20 @@ CePlan ce_plan(dlmi_ctx const *ctx, size_t B, size_t K, size_t V, bool back) {
   };
   p.xp = take(packed_bytes(p.Bp, p.Kp, NP));
   p.wp = take(packed_bytes(p.Vc, p.Kp, NP));
-  p.rowmax = take(B * sizeof(float));
-  p.parts = take(2 * kCeMaxParts * sizeof(float));
-  p.unscale = take((B + 2) * sizeof(float));
+  // 8 rows of a packing workgroup until those of 32 would give every CU two
+  auto const rows_of = [&](size_t n) { return n / 32 >= static_cast<size_t>(ctx->num_cu) * 2 ? 32 : 8; };
+  p.rows_x = rows_of(p.Bp);
+  p.rows_w = rows_of(p.Vc);
+  p.nparts_x = static_cast<unsigned>(p.Bp / p.rows_x);
+  p.unscale_x = take(B * sizeof(float));
+  p.unscale_w = take(p.Vc * sizeof(float));
+  p.parts_x = take(p.nparts_x * sizeof(float));
+  p.parts_w = take(p.Vc / p.rows_w * sizeof(float));
   if (!back) {
     p.part = take(dlmi_ceil_div(V, T) * 2 * p.Bp * sizeof(float2));
     p.target = take(B * sizeof(float));
   } else {
-    p.xg = take(packed_bytes(p.Kp, p.Bp, NP));
+    p.xt = take(packed_bytes(p.Kp, p.Bp, NP));
     p.wt = take(packed_bytes(p.Kp, p.Vc, NP));
     p.dlb = take(packed_bytes(p.Bp, p.Vc, NP));
     p.dlv = take(packed_bytes(p.Vc, p.Bp, NP));
@@ -863,47 +898,35 @@ struct CeRun {
   static unsigned ce_stages(int T, size_t k) { return static_cast<unsigned>(dlmi_ceil_div(k, (T == 64 ? 64 : 32) / NP)); }
   float *floats(size_t at) const { return reinterpret_cast<float *>(s + at); }
 
-  int pack_rows() const {
-    unsigned const blocks = static_cast<unsigned>(dlmi_ceil_div(a.B, 4) < kCeMaxParts ? dlmi_ceil_div(a.B, 4) : kCeMaxParts);
-    E const *const x = static_cast<E const *>(a.X);
-    hipLaunchKernelGGL(k_ce_max<E>, dim3(blocks), dim3(kCeBlock), 0, ctx->stream, a, x, a.B, a.K, floats(p.rowmax), nullptr, 0);
-    DLMI_LAUNCH_CHECK(ctx, "k_ce_max");
-    dim3 const grid(static_cast<unsigned>(p.Kp / 64), static_cast<unsigned>(p.Bp / 64));
-    hipLaunchKernelGGL((k_ce_pack<E, NP>), grid, dim3(kCeBlock), 0, ctx->stream, a, x, a.B, a.K, static_cast<unsigned>(p.Kp / 16), 0u,
-                       floats(p.rowmax), nullptr, 0u, floats(p.unscale) + 2, 0, s + p.xp, nullptr);
+  template <int ROWS, bool LABELS>
+  int pack(E const *src, size_t rows, size_t padded, size_t unscale, size_t parts, char *as, char *across) const {
+    hipLaunchKernelGGL((k_ce_pack<E, NP, ROWS, LABELS>), dim3(static_cast<unsigned>(padded / ROWS)), dim3(kCeBlock), 0, ctx->stream, a, src, rows,
+                       a.K, static_cast<unsigned>(p.Kp / 16), static_cast<unsigned>(padded / 16), floats(unscale), floats(parts), as, across);
     DLMI_LAUNCH_CHECK(ctx, "k_ce_pack");
     return DLMI_OK;
   }
-  int pack_rows_weighted() const {
-    unsigned const blocks = static_cast<unsigned>(dlmi_ceil_div(a.B, 4) < kCeMaxParts ? dlmi_ceil_div(a.B, 4) : kCeMaxParts);
+  int pack_rows(bool back) const {
     E const *const x = static_cast<E const *>(a.X);
-    float *const parts = floats(p.parts) + kCeMaxParts;
-    hipLaunchKernelGGL(k_ce_max<E>, dim3(blocks), dim3(kCeBlock), 0, ctx->stream, a, x, a.B, a.K, nullptr, parts, 1);
-    DLMI_LAUNCH_CHECK(ctx, "k_ce_max");
-    dim3 const grid(static_cast<unsigned>(p.Kp / 64), static_cast<unsigned>(p.Bp / 64));
-    hipLaunchKernelGGL((k_ce_pack<E, NP>), grid, dim3(kCeBlock), 0, ctx->stream, a, x, a.B, a.K, 0u, static_cast<unsigned>(p.Bp / 16), nullptr,
-                       parts, blocks, floats(p.unscale) + 1, 1, nullptr, s + p.xg);
-    DLMI_LAUNCH_CHECK(ctx, "k_ce_pack");
-    return DLMI_OK;
+    char *const across = back && a.dW != nullptr ? s + p.xt : nullptr;
+    if (p.rows_x == 32) return pack<32, true>(x, a.B, p.Bp, p.unscale_x, p.parts_x, s + p.xp, across);
+    return pack<8, true>(x, a.B, p.Bp, p.unscale_x, p.parts_x, s + p.xp, across);
   }
   int pack_classes(size_t v0, size_t vn, size_t vp, bool back) const {
-    unsigned const blocks = static_cast<unsigned>(dlmi_ceil_div(vn, 4) < kCeMaxParts ? dlmi_ceil_div(vn, 4) : kCeMaxParts);
     E const *const w = static_cast<E const *>(a.W) + v0 * a.K;
-    hipLaunchKernelGGL(k_ce_max<E>, dim3(blocks), dim3(kCeBlock), 0, ctx->stream, a, w, vn, a.K, nullptr, floats(p.parts), 0);
-    DLMI_LAUNCH_CHECK(ctx, "k_ce_max");
-    dim3 const grid(static_cast<unsigned>(p.Kp / 64), static_cast<unsigned>(vp / 64));
-    hipLaunchKernelGGL((k_ce_pack<E, NP>), grid, dim3(kCeBlock), 0, ctx->stream, a, w, vn, a.K, static_cast<unsigned>(p.Kp / 16),
-                       static_cast<unsigned>(vp / 16), nullptr, floats(p.parts), blocks, floats(p.unscale), 0, s + p.wp,
-                       back ? s + p.wt : nullptr);
-    DLMI_LAUNCH_CHECK(ctx, "k_ce_pack");
-    return DLMI_OK;
+    char *const across = back && a.dX != nullptr ? s + p.wt : nullptr;
+    if (p.rows_w == 32) return pack<32, false>(w, vn, vp, p.unscale_w, p.parts_w, s + p.wp, across);
+    return pack<8, false>(w, vn, vp, p.unscale_w, p.parts_w, s + p.wp, across);
   }
   CeLogits logits(size_t v0, size_t vn, size_t vp) const {
     CeLogits g = {};
     g.P = s + p.wp;
     g.Q = s + p.xp;
-    g.unscale_w = floats(p.unscale);
-    g.unscale_x = floats(p.unscale) + 2;
+    g.unscale_w = floats(p.unscale_w);
+    g.unscale_x = floats(p.unscale_x);
+    g.parts_w = floats(p.parts_w);
+    g.parts_x = floats(p.parts_x);
+    g.nparts_w = static_cast<unsigned>(vp / p.rows_w);
+    g.nparts_x = p.nparts_x;
     g.ni = static_cast<unsigned>(vp / p.T);
     g.nj = static_cast<unsigned>(p.Bp / p.T);
     g.kblocks = static_cast<unsigned>(p.Kp / 16);
@@ -915,7 +938,7 @@ struct CeRun {
 
   template <int T>
   int forward() const {
-    int rc = pack_rows();
+    int rc = pack_rows(false);
     for (size_t v0 = 0; rc == DLMI_OK && v0 < a.V; v0 += p.Vc) {
       size_t const vn = a.V - v0 < p.Vc ? a.V - v0 : p.Vc, vp = dlmi_ceil_div(vn, T) * T;
       rc = pack_classes(v0, vn, vp, false);
@@ -934,8 +957,7 @@ struct CeRun {
 
   template <int T>
   int backward() const {
-    int rc = pack_rows();
-    if (rc == DLMI_OK) rc = pack_rows_weighted();
+    int rc = pack_rows(true);
     unsigned const nb = static_cast<unsigned>(p.Bp / T), nk = static_cast<unsigned>(p.Kp / T), kb = static_cast<unsigned>(p.Bp / 16);
     for (size_t v0 = 0; rc == DLMI_OK && v0 < a.V; v0 += p.Vc) {
       size_t const vn = a.V - v0 < p.Vc ? a.V - v0 : p.Vc, vp = dlmi_ceil_div(vn, T) * T;
@@ -957,12 +979,12 @@ struct CeRun {
       }
       if (a.dX != nullptr) {
         hipLaunchKernelGGL((k_ce_dx<T, NP>), dim3(nb * nk * p.slices), dim3(256), 0, ctx->stream, s + p.dlb, s + p.wt, nb, nk, kv, ce_stages(T, vp),
-                           p.per_slice, floats(p.unscale), floats(p.dxacc), a.B, a.K, v0 == 0 ? 1 : 0);
+                           p.per_slice, g.parts_w, g.nparts_w, floats(p.dxacc), a.B, a.K, v0 == 0 ? 1 : 0);
         DLMI_LAUNCH_CHECK(ctx, "k_ce_dx");
       }
       if (a.dW != nullptr) {
-        hipLaunchKernelGGL((k_ce_dw<T, NP, E>), dim3(g.ni * nk), dim3(256), 0, ctx->stream, s + p.dlv, s + p.xg, g.ni, nk, kb,
-                           ce_stages(T, a.B), floats(p.unscale) + 1, a.scale, static_cast<E *>(a.dW) + v0 * a.K, vn, a.K,
+        hipLaunchKernelGGL((k_ce_dw<T, NP, E>), dim3(g.ni * nk), dim3(256), 0, ctx->stream, s + p.dlv, s + p.xt, g.ni, nk, kb,
+                           ce_stages(T, a.B), g.parts_x, g.nparts_x, a.scale, static_cast<E *>(a.dW) + v0 * a.K, vn, a.K,
                            a.accumulate);
         DLMI_LAUNCH_CHECK(ctx, "k_ce_dw");
       }
