@@ -368,8 +368,12 @@ struct HalfBlock {
 // value one of fp32 before it is rounded: the compiler may otherwise fold a product before it into one of the two uses of
 // `hi` (a multiplication that rounds to f16 at once), and a value near a tie then loses a whole step of its first plane.
 template <int NP>
-__device__ __forceinline__ HalfBlock<NP> half_split(f32x16 const &v) {
-  half4 h[4], l[4];
+struct HalfQuads {
+  half4 h[NP][4];  // [plane][r >> 2][r & 3]
+};
+template <int NP>
+__device__ __forceinline__ HalfQuads<NP> half_planes(f32x16 const &v) {
+  HalfQuads<NP> o;
 #pragma unroll
   for (int q = 0; q < 4; ++q)
 #pragma unroll
@@ -377,17 +381,24 @@ __device__ __forceinline__ HalfBlock<NP> half_split(f32x16 const &v) {
       float x = v[q * 4 + t];
       if constexpr (NP == 2) asm("" : "+v"(x));
       _Float16 const hi = static_cast<_Float16>(x);
-      h[q][t] = hi;
-      if constexpr (NP == 2) l[q][t] = static_cast<_Float16>(x - static_cast<float>(hi));
+      o.h[0][q][t] = hi;
+      if constexpr (NP == 2) o.h[1][q][t] = static_cast<_Float16>(x - static_cast<float>(hi));
     }
+  return o;
+}
+template <int NP>
+__device__ __forceinline__ HalfBlock<NP> half_joined(HalfQuads<NP> const &q) {
   HalfBlock<NP> b;
-  b.pl[0].k0 = half_join(h[0], h[1]);
-  b.pl[0].k1 = half_join(h[2], h[3]);
-  if constexpr (NP == 2) {
-    b.pl[1].k0 = half_join(l[0], l[1]);
-    b.pl[1].k1 = half_join(l[2], l[3]);
+#pragma unroll
+  for (int p = 0; p < NP; ++p) {
+    b.pl[p].k0 = half_join(q.h[p][0], q.h[p][1]);
+    b.pl[p].k1 = half_join(q.h[p][2], q.h[p][3]);
   }
   return b;
+}
+template <int NP>
+__device__ __forceinline__ HalfBlock<NP> half_split(f32x16 const &v) {
+  return half_joined<NP>(half_planes<NP>(v));
 }
 
 // dst: fragment (row block of j, k block of i) of the packed matrix; the block's second k block follows its planes.

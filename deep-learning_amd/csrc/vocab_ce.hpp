@@ -14,7 +14,8 @@
 // padding row full of garbage spoils nobody's scale).  bf16 values have 8 bits and one plane holds them exactly; fp32
 // values take two planes.  dL is in [-1, 1] and held times 2^15, rounded to 11 bits (bf16; the result keeps 8) or 22 (fp32).
 // Where a product's sum runs over rows that are scaled differently (dX over W's, dW over X's), dL carries what undoes the
-// scale, and dloss, as a share of the largest such factor, which multiplies the result.
+// scale, as a share of the largest such factor, which multiplies the result.  For dW X is packed times dloss (one more
+// rounding for bf16, none without dloss).
 #pragma once
 
 #include <cmath>
@@ -82,89 +83,87 @@ __device__ __forceinline__ float ce_row_weight(CeArgs const &a, size_t b) {
 // The largest of n values, the same in all lanes of a wavefront.
 __device__ __forceinline__ float ce_largest(float const *v, unsigned n, int lane) {
   float m = 0.0f;
-#pragma unroll 4
+#pragma unroll 16
   for (unsigned q = lane; q < n; q += 64) m = fmaxf(m, v[q]);
   return ce_wave_max(m);
 }
 
 // Rows of src [rows, cols], each scaled by its own largest magnitude and packed as it stands (`as`: row r, k = c) and / or
-// transposed (`across`: row c, k = r), padding zero.  unscale[r]: the inverse scale; parts[workgroup]: the largest of weight
-// times unscale of the workgroup's rows.  LABELS (X): the weight is ce_row_weight, and rows left out are zero in `across`;
-// otherwise (W) it is 1.
-// A wavefront takes 8 rows, a lane 8 columns of one of them at a time, twice over the row: for the largest magnitude and for
-// the values (from the L2).  A lane's octet is a piece of a fragment as it stands; for the transposed ones the wavefront
-// turns 8 x 64 values through 2 KiB of LDS that only it uses.  ROWS = 32: each wavefront its own rows; 8: the four share the
-// columns of the same 8 rows (where there are too few rows to fill the device otherwise).
-template <class T, int NP, int ROWS, bool LABELS>
-__global__ __launch_bounds__(kCeBlock) void k_ce_pack(CeArgs a, T const *src, size_t rows, size_t cols, unsigned kblocks_as,
-                                                      unsigned kblocks_across, float *unscale, float *parts, char *as, char *across) {
+// transposed (`across`: row c, k = r), padding zero.  unscale[r]: the inverse scale of `as`, unscale_across[r] that of
+// `across` (padding rows have entries too).  LABELS (X): `across` holds the row times ce_row_weight, scaled by its own
+// largest, and zeros in rows left out; otherwise (W) the two are the same.  The largest unscale_across of a piece of W goes to
+// most.w[piece] by an integer maximum in memory (positive floats order like integers, and no order changes a maximum), which
+// packing X has cleared; X's are left per workgroup and joined by the first workgroup that packs W.
+// The four wavefronts of a workgroup share the columns of 8 rows at a time, a lane 8 columns of one of them; up to KEEP
+// octets of a lane stay in registers between the search for the largest and the packing (wider rows are read twice).  An
+// octet is a piece of a fragment as it stands; for the transposed ones the wavefront turns 8 x 64 values through 2 KiB of
+// LDS that only it uses.
+constexpr unsigned kCePackBlocks = 1024;
+
+// (All null in the forward pass.)
+struct CeMost {
+  float *w;          // of each piece
+  float *x, *parts;  // of X; of its packing workgroups
+  unsigned nparts, piece, pieces;
+};
+
+template <class T, int NP, int KEEP, bool LABELS>
+__global__ __launch_bounds__(kCeBlock) void k_ce_pack(CeArgs a, T const *src, size_t rows, size_t padded, size_t cols, unsigned kblocks_as,
+                                                      unsigned kblocks_across, float *unscale, float *unscale_across, CeMost most, char *as, char *across) {
   __shared__ float turn[4][8][68];
-  __shared__ float top[4][8];
+  __shared__ float top[2][4][8];
   int const lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int const r8 = lane >> 3, c8 = (lane & 7) * 8;
-  size_t const r0 = static_cast<size_t>(blockIdx.x) * ROWS + (ROWS == 32 ? wave * 8 : 0), r = r0 + r8;
   unsigned const tiles = kblocks_as / 4;  // of 64 columns, padding included
-  unsigned const t0 = ROWS == 32 ? 0 : wave, step = ROWS == 32 ? 1 : 4;
-  T const *const row = src + (r < rows ? r : rows - 1) * cols;
-  // every load is made, whole (one that hangs over the row's end is moved back to end with it)
-  auto const load = [&](unsigned t) {
-    size_t const c = static_cast<size_t>(t) * 64 + c8;
-    return *reinterpret_cast<CeOct<T> const *>(row + (c + 8 <= cols ? c : cols - 8));
-  };
-  bool const narrow = cols < 8;
-  float m = 0.0f;
-  if (narrow) {
-    for (size_t c = 0; c < cols; ++c) m = ce_finite_max(m, static_cast<float>(row[c]));
-  } else {
-#pragma unroll 4
-    for (unsigned t = t0; t < tiles; t += step) {
-      CeOct<T> const o = load(t);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) m = ce_finite_max(m, static_cast<float>(o.v[i]));
-    }
-  }
-#pragma unroll
-  for (int o = 1; o < 8; o *= 2) m = fmaxf(m, __shfl_xor(m, o));
-  if constexpr (ROWS == 8) {
-    if ((lane & 7) == 0) top[wave][r8] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(top[0][r8], top[1][r8]), fmaxf(top[2][r8], top[3][r8]));
-  }
-  float const scale = ce_scale(m);
-  bool live = r < rows;
-  float weight = live ? 1.0f : 0.0f;
-  if constexpr (LABELS) {
-    int const l = live ? a.labels[r] : -1;
-    live = l >= 0 && static_cast<size_t>(l) < a.V;
-    weight = live ? fabsf(ce_row_weight(a, r)) : 0.0f;
-  }
-  if ((lane & 7) == 0 && r < rows && (ROWS == 32 || wave == 0)) unscale[r] = ce_unscale(scale);
-  if (parts != nullptr) {
-    float const mine = ce_wave_max(weight * ce_unscale(scale));
-    if constexpr (ROWS == 32) {
-      if (lane == 0) top[wave][0] = mine;
-      __syncthreads();
-      if (threadIdx.x == 0) parts[blockIdx.x] = fmaxf(fmaxf(top[0][0], top[1][0]), fmaxf(top[2][0], top[3][0]));
-    } else if (threadIdx.x == 0) {
-      parts[blockIdx.x] = mine;
-    }
-  }
-#pragma unroll 2
-  for (unsigned t = t0; t < tiles; t += step) {
-    float x[8];
-    size_t const c = static_cast<size_t>(t) * 64 + c8;
+  bool const narrow = cols < 8, kept = (tiles + 3) / 4 <= KEEP;
+  float mine = 0.0f;
+  int flip = 0;
+  for (size_t r0 = static_cast<size_t>(blockIdx.x) * 8; r0 < padded; r0 += static_cast<size_t>(gridDim.x) * 8) {
+    size_t const r = r0 + r8;
+    T const *const row = src + (r < rows ? r : rows - 1) * cols;
+    // every load is made, whole (one that hangs over the row's end is moved back to end with it)
+    auto const load = [&](unsigned t) {
+      size_t const c = static_cast<size_t>(t) * 64 + c8;
+      return *reinterpret_cast<CeOct<T> const *>(row + (c + 8 <= cols ? c : cols - 8));
+    };
+    CeOct<T> keep[KEEP];
+    float m = 0.0f;
     if (narrow) {
+      for (size_t c = 0; c < cols; ++c) m = ce_finite_max(m, static_cast<float>(row[c]));
+    } else if (kept) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = r < rows && c + i < cols ? static_cast<float>(row[c + i < cols ? c + i : cols - 1]) * scale : 0.0f;
+      for (int k = 0; k < KEEP; ++k) keep[k] = load(wave + 4 * k < tiles ? wave + 4 * k : 0);
+#pragma unroll
+      for (int k = 0; k < KEEP; ++k)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = ce_finite_max(m, static_cast<float>(keep[k].v[i]));
     } else {
-      CeOct<T> const o = load(t);
+#pragma unroll 4
+      for (unsigned t = wave; t < tiles; t += 4) {
+        CeOct<T> const o = load(t);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = r < rows && c + 8 <= cols ? static_cast<float>(o.v[i]) * scale : 0.0f;
-      if (c < cols && c + 8 > cols && r < rows) {  // the row's end: the octet was moved back by c + 8 - cols
-        for (int i = 0; i < 8; ++i)
-          if (c + i < cols) x[i] = static_cast<float>(row[c + i]) * scale;
+        for (int i = 0; i < 8; ++i) m = ce_finite_max(m, static_cast<float>(o.v[i]));
       }
     }
+#pragma unroll
+    for (int o = 1; o < 8; o *= 2) m = fmaxf(m, __shfl_xor(m, o));
+    if ((lane & 7) == 0) top[flip][wave][r8] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(top[flip][0][r8], top[flip][1][r8]), fmaxf(top[flip][2][r8], top[flip][3][r8]));
+    flip ^= 1;
+    float const scale = ce_scale(m);
+    // across = as * ratio, ratio = weight * scale_across / scale
+    float ratio = r < rows ? 1.0f : 0.0f, un = ce_unscale(scale);
+    if ((lane & 7) == 0 && wave == 0) unscale[r] = un;
+    if constexpr (LABELS) {
+      int const l = r < rows ? a.labels[r] : -1;
+      float const w = l >= 0 && static_cast<size_t>(l) < a.V ? ce_row_weight(a, r) : 0.0f;
+      float const s2 = ce_scale(fabsf(w) * m);
+      ratio = l >= 0 && static_cast<size_t>(l) < a.V ? w * (s2 * un) : 0.0f;
+      un = w != 0.0f ? ce_unscale(s2) : 0.0f;
+      if ((lane & 7) == 0 && wave == 0) unscale_across[r] = un;
+    }
+    mine = fmaxf(mine, r < rows ? un : 0.0f);
     auto const pack = [&](float const (&v)[8], char *dst) {
       half8 hi, lo;
 #pragma unroll
@@ -178,21 +177,58 @@ __global__ __launch_bounds__(kCeBlock) void k_ce_pack(CeArgs a, T const *src, si
       *reinterpret_cast<half8 *>(dst) = hi;
       if constexpr (NP == 2) *reinterpret_cast<half8 *>(dst + kFragBytes) = lo;
     };
-    if (as != nullptr) {
-      size_t const frag = (r / 32) * kblocks_as + t * 4 + (lane & 7) / 2;
-      pack(x, as + frag * NP * kFragBytes + ((lane & 1) * 32 + (r & 31)) * 16);
+    auto const tile = [&](unsigned t, CeOct<T> const &o) {
+      float x[8];
+      size_t const c = static_cast<size_t>(t) * 64 + c8;
+      if (narrow) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = r < rows && c + i < cols ? static_cast<float>(row[c + i < cols ? c + i : cols - 1]) * scale : 0.0f;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = r < rows && c + 8 <= cols ? static_cast<float>(o.v[i]) * scale : 0.0f;
+        if (c < cols && c + 8 > cols && r < rows) {  // the row's end: the octet was moved back by c + 8 - cols
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (c + i < cols) x[i] = static_cast<float>(row[c + i]) * scale;
+        }
+      }
+      if (as != nullptr) {
+        size_t const frag = (r / 32) * kblocks_as + t * 4 + (lane & 7) / 2;
+        pack(x, as + frag * NP * kFragBytes + ((lane & 1) * 32 + (r & 31)) * 16);
+      }
+      if (across != nullptr) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) turn[wave][r8][c8 + i] = !LABELS || ratio != 0.0f ? x[i] * (LABELS ? ratio : 1.0f) : 0.0f;
+        __builtin_amdgcn_wave_barrier();
+        float y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = turn[wave][i][lane];
+        __builtin_amdgcn_wave_barrier();
+        size_t const f = static_cast<size_t>(t) * 64 + lane;
+        size_t const frag = (f / 32) * kblocks_across + r0 / 16;
+        pack(y, across + frag * NP * kFragBytes + ((r0 / 8 & 1) * 32 + (f & 31)) * 16);
+      }
+    };
+    if (kept) {
+#pragma unroll
+      for (int k = 0; k < KEEP; ++k)
+        if (wave + 4 * k < tiles) tile(wave + 4 * k, keep[k]);
+    } else {
+#pragma unroll 2
+      for (unsigned t = wave; t < tiles; t += 4) tile(t, narrow ? CeOct<T>{} : load(t));
     }
-    if (across != nullptr) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) turn[wave][r8][c8 + i] = live ? x[i] : 0.0f;
-      __builtin_amdgcn_wave_barrier();
-      float y[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = turn[wave][i][lane];
-      __builtin_amdgcn_wave_barrier();
-      size_t const f = static_cast<size_t>(t) * 64 + lane;
-      size_t const frag = (f / 32) * kblocks_across + r0 / 16;
-      pack(y, across + frag * NP * kFragBytes + ((r0 / 8 & 1) * 32 + (f & 31)) * 16);
+  }
+  if (most.w == nullptr) return;
+  mine = ce_wave_max(mine);  // (the wavefronts have seen the same rows)
+  if constexpr (LABELS) {
+    if (threadIdx.x == 0) most.parts[blockIdx.x] = mine;
+    if (blockIdx.x == 0)
+      for (unsigned q = threadIdx.x; q < most.pieces; q += kCeBlock) most.w[q] = 0.0f;
+  } else {
+    if (threadIdx.x == 0) atomicMax(reinterpret_cast<unsigned *>(most.w) + most.piece, __float_as_uint(mine));
+    if (most.piece == 0 && blockIdx.x == 0 && wave == 0) {
+      float const x = ce_largest(most.parts, most.nparts, lane);
+      if (lane == 0) most.x[0] = x;
     }
   }
 }
@@ -212,8 +248,8 @@ __device__ __forceinline__ float ce_join_factor(float m, float most) { return m 
 struct CeLogits {
   char const *P, *Q;
   float const *unscale_x, *unscale_w;  // of the rows of the batch, of the piece's classes
-  float const *parts_x, *parts_w;      // their workgroups' largest (backward)
-  unsigned nparts_x, nparts_w;
+  // backward: what undoes the scale of X's rows times dloss; the largest of those and of unscale_w
+  float const *unscale_xw, *most_x, *most_w;
   unsigned ni, nj, kblocks, stages;    // kblocks: of a row block in memory
   size_t v0, vn;                     // first class of the piece, classes in it
 };
@@ -237,14 +273,14 @@ __device__ __forceinline__ f32x16 ce_biases(CeArgs const &a, CeLogits const &g, 
   return v;
 }
 
-// What undoes the scale of those classes.
+// What undoes the scale of those classes (padding has entries too).
 __device__ __forceinline__ f32x16 ce_unscales(CeLogits const &g, size_t c0, int lane) {
   f32x16 v;
-  size_t const c1 = c0 + 4 * (lane >> 5);
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    size_t const c = c1 + 8 * (r >> 2) + (r & 3);
-    v[r] = g.unscale_w[c < g.vn ? c : g.vn - 1];
+  for (int q = 0; q < 4; ++q) {
+    f32x4 const x = *reinterpret_cast<f32x4 const *>(g.unscale_w + c0 + 4 * (lane >> 5) + 8 * q);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) v[q * 4 + t] = x[t];
   }
   return v;
 }
@@ -635,8 +671,9 @@ __device__ __forceinline__ float ce_scatter_sum(f32x16 const &v, int lane) {
 }
 
 // dL of a tile, packed for dX (rows of the batch, k = classes; times what undoes the scale of W's row, as a share of the
-// piece's largest: a power of two) and for dW (rows are classes, k = rows of the batch; times dloss and what undoes the scale
-// of X's row, as a share of the largest): the factors of the products' k that do not come out of their sums.  DB: also the sums of dloss dL over each half tile of rows.
+// piece's largest) and for dW (rows are classes, k = rows of the batch; times what undoes the scale of X's row, as a share of
+// the largest): the factors of the products' k that do not come out of their sums, powers of two, so that the planes are
+// rounded once and multiplied in f16.  DB: also the sums of dloss dL over each half tile of rows.
 template <int T, int NP, bool DB>
 __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_grad(CeArgs a, CeLogits g, char *dlb, char *dlv, unsigned kblocks_v,
                                                                   unsigned kblocks_b, float *dbpart, size_t dbpart_stride) {
@@ -648,12 +685,14 @@ __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_grad(CeArgs a, CeL
   half_gemm<H>(acc, g.P + ti * (T / 32) * rs, g.Q + tj * (T / 32) * rs, rs, rs, g.stages);
   int const lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   half8 const id0 = half_identity(0, lane), id1 = half_identity(1, lane);
-  float const most_w = ce_largest(g.parts_w, g.nparts_w, lane), most_x = ce_largest(g.parts_x, g.nparts_x, lane);
+  // (powers of two, so their inverses are exact)
+  float const inv_w = 1.0f / g.most_w[0], most_x = g.most_x[0], inv_x = most_x > 0.0f ? 1.0f / most_x : 0.0f;
   size_t const c0 = static_cast<size_t>(ti) * T + (wave >> 1) * (T / 2);
   size_t const b0 = static_cast<size_t>(tj) * T + (wave & 1) * (T / 2);
   size_t const rb = static_cast<size_t>(kblocks_v) * NP * kFragBytes, rv = static_cast<size_t>(kblocks_b) * NP * kFragBytes;
   // of this lane's rows of the batch: unscale, lse, weight, share of the largest, and the label's class from c0 on (-1: none here)
-  float ux[H::kNB], lse[H::kNB], weight[H::kNB], fx[H::kNB];
+  float ux[H::kNB], lse[H::kNB], weight[H::kNB];
+  _Float16 fx[H::kNB];
   int at[H::kNB];
   bool live[H::kNB];
 #pragma unroll
@@ -663,7 +702,7 @@ __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_grad(CeArgs a, CeL
     ux[n] = g.unscale_x[in];
     lse[n] = a.lse_in[in];
     weight[n] = a.dloss != nullptr ? a.dloss[in] : 1.0f;
-    fx[n] = most_x > 0.0f ? weight[n] * ux[n] / most_x * kCeDl : 0.0f;
+    fx[n] = static_cast<_Float16>(g.unscale_xw[in] * inv_x);
     live[n] = b < a.B && label >= 0 && static_cast<size_t>(label) < a.V;
     long long const c = static_cast<long long>(label) - static_cast<long long>(g.v0 + c0);
     at[n] = live[n] && c >= 0 && c < T / 2 ? static_cast<int>(c) : -1;
@@ -671,7 +710,9 @@ __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_grad(CeArgs a, CeL
 #pragma unroll
   for (int m = 0; m < H::kMB; ++m) {
     f32x16 const bias = ce_biases(a, g, c0 + m * 32, lane), uw = ce_unscales(g, c0 + m * 32, lane);
-    f32x16 const fw = uw * (kCeDl / most_w);
+    half4 fw[4];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) fw[r >> 2][r & 3] = static_cast<_Float16>(uw[r] * inv_w);
     f32x16 sum = {};
     bool const whole = c0 + m * 32 + 32 <= g.vn;
 #pragma unroll
@@ -687,8 +728,17 @@ __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_grad(CeArgs a, CeL
         if constexpr (DB) sum[r] += live[n] ? weight[n] * z[r] : 0.0f;
       }
       size_t const ib = c0 / 32 + m, jb = b0 / 32 + n;
-      half_store<NP>(dlb + jb * rb + ib * 2 * NP * kFragBytes, half_split<NP>(z * fw), lane);
-      half_store<NP>(dlv + ib * rv + jb * 2 * NP * kFragBytes, half_flip<NP>(half_split<NP>(z * fx[n]), id0, id1), lane);
+      HalfQuads<NP> const q = half_planes<NP>(z * kCeDl);
+      HalfQuads<NP> qb, qv;
+#pragma unroll
+      for (int p = 0; p < NP; ++p)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          qb.h[p][k] = q.h[p][k] * fw[k];
+          qv.h[p][k] = q.h[p][k] * fx[n];
+        }
+      half_store<NP>(dlb + jb * rb + ib * 2 * NP * kFragBytes, half_joined<NP>(qb), lane);
+      half_store<NP>(dlv + ib * rv + jb * 2 * NP * kFragBytes, half_flip<NP>(half_joined<NP>(qv), id0, id1), lane);
     }
     if constexpr (DB) {
       float const s = ce_scatter_sum(sum, lane);
@@ -735,10 +785,10 @@ __device__ __forceinline__ void ce_block_out(f32x16 const &v, float factor, O *o
   }
 }
 
-// dW of a piece: classes i (P = dL packed by classes), features j (Q = X packed by features), times `scale`.
+// dW of a piece: classes i (P = dL packed by classes), features j (Q = dloss X packed by features), times `scale`.
 template <int T, int NP, class O>
 __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_dw(char const *P, char const *Q, unsigned ni, unsigned nj, unsigned kblocks,
-                                                                unsigned stages, float const *parts, unsigned nparts, float scale, O *out, size_t rows,
+                                                                unsigned stages, float const *most, float scale, O *out, size_t rows,
                                                                 size_t cols, int accumulate) {
   using H = HalfTile<T, T, NP>;
   unsigned ti, tj;
@@ -747,7 +797,7 @@ __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_dw(char const *P, 
   HalfAcc<H> acc;
   half_gemm<H>(acc, P + ti * (T / 32) * rs, Q + tj * (T / 32) * rs, rs, rs, stages);
   int const lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  float const factor = ce_largest(parts, nparts, lane) * (scale * (1.0f / kCeDl));
+  float const factor = most[0] * (scale * (1.0f / kCeDl));
 #pragma unroll
   for (int m = 0; m < H::kMB; ++m)
 #pragma unroll
@@ -760,7 +810,7 @@ __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_dw(char const *P, 
 // over the piece's classes of the slice into out [slice][rows][cols]; the first piece writes, later ones add.
 template <int T, int NP>
 __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_dx(char const *P, char const *Q, unsigned ni, unsigned nj, unsigned kblocks,
-                                                                unsigned stages, unsigned per_slice, float const *parts, unsigned nparts, float *out,
+                                                                unsigned stages, unsigned per_slice, float const *most, float *out,
                                                                 size_t rows, size_t cols, int first) {
   using H = HalfTile<T, T, NP>;
   unsigned ti, tj;
@@ -773,7 +823,7 @@ __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_dx(char const *P, 
   HalfAcc<H> acc;
   half_gemm<H>(acc, P + ti * (T / 32) * rs + skip, Q + tj * (T / 32) * rs + skip, rs, rs, count);
   int const lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  float const factor = ce_largest(parts, nparts, lane) * (1.0f / kCeDl);
+  float const factor = most[0] * (1.0f / kCeDl);
   out += slice * rows * cols;
 #pragma unroll
   for (int m = 0; m < H::kMB; ++m)
@@ -810,10 +860,9 @@ struct CePlan {
   int T;
   size_t Bp, Kp, Vc, pieces;       // padded rows and features; classes of a piece (a multiple of T)
   unsigned slices, per_slice;      // of dX
-  int rows_x, rows_w;              // rows of a packing workgroup (8 or 32)
-  unsigned nparts_x, nparts_w;
+  unsigned pack_x, pack_w;         // packing workgroups
   // offsets in the scratch
-  size_t xp, xt, wp, wt, dlb, dlv, parts_x, parts_w, unscale_x, unscale_w, part, target, dxacc, dbpart, bytes;
+  size_t xp, xt, wp, wt, dlb, dlv, parts_x, unscale_x, unscale_xw, unscale_w, most_x, most_w, part, target, dxacc, dbpart, bytes;
 };
 
 template <int NP>
@@ -856,15 +905,15 @@ CePlan ce_plan(dlmi_ctx const *ctx, size_t B, size_t K, size_t V, bool back) {
   };
   p.xp = take(packed_bytes(p.Bp, p.Kp, NP));
   p.wp = take(packed_bytes(p.Vc, p.Kp, NP));
-  // 8 rows of a packing workgroup until those of 32 would give every CU two
-  auto const rows_of = [&](size_t n) { return n / 32 >= static_cast<size_t>(ctx->num_cu) * 2 ? 32 : 8; };
-  p.rows_x = rows_of(p.Bp);
-  p.rows_w = rows_of(p.Vc);
-  p.nparts_x = static_cast<unsigned>(p.Bp / p.rows_x);
-  p.unscale_x = take(B * sizeof(float));
+  auto const blocks_of = [](size_t n) { return static_cast<unsigned>(n / 8 < kCePackBlocks ? n / 8 : kCePackBlocks); };
+  p.pack_x = blocks_of(p.Bp);
+  p.pack_w = blocks_of(p.Vc);
+  p.unscale_x = take(p.Bp * sizeof(float));
+  p.unscale_xw = take(p.Bp * sizeof(float));
   p.unscale_w = take(p.Vc * sizeof(float));
-  p.parts_x = take(p.nparts_x * sizeof(float));
-  p.parts_w = take(p.Vc / p.rows_w * sizeof(float));
+  p.parts_x = take(p.pack_x * sizeof(float));
+  p.most_x = take(sizeof(float));
+  p.most_w = take(p.pieces * sizeof(float));
   if (!back) {
     p.part = take(dlmi_ceil_div(V, T) * 2 * p.Bp * sizeof(float2));
     p.target = take(B * sizeof(float));
@@ -898,24 +947,28 @@ struct CeRun {
   static unsigned ce_stages(int T, size_t k) { return static_cast<unsigned>(dlmi_ceil_div(k, (T == 64 ? 64 : 32) / NP)); }
   float *floats(size_t at) const { return reinterpret_cast<float *>(s + at); }
 
-  template <int ROWS, bool LABELS>
-  int pack(E const *src, size_t rows, size_t padded, size_t unscale, size_t parts, char *as, char *across) const {
-    hipLaunchKernelGGL((k_ce_pack<E, NP, ROWS, LABELS>), dim3(static_cast<unsigned>(padded / ROWS)), dim3(kCeBlock), 0, ctx->stream, a, src, rows,
-                       a.K, static_cast<unsigned>(p.Kp / 16), static_cast<unsigned>(padded / 16), floats(unscale), floats(parts), as, across);
+  template <int KEEP, bool LABELS>
+  int pack(E const *src, size_t rows, size_t padded, unsigned blocks, size_t unscale, size_t piece, bool back, char *as, char *across) const {
+    CeMost most = {};
+    if (back) most = {floats(p.most_w), floats(p.most_x), floats(p.parts_x), p.pack_x, static_cast<unsigned>(piece), static_cast<unsigned>(p.pieces)};
+    hipLaunchKernelGGL((k_ce_pack<E, NP, KEEP, LABELS>), dim3(blocks), dim3(kCeBlock), 0, ctx->stream, a, src, rows, padded, a.K,
+                       static_cast<unsigned>(p.Kp / 16), static_cast<unsigned>(padded / 16), floats(unscale), floats(p.unscale_xw),
+                       most, as, across);
     DLMI_LAUNCH_CHECK(ctx, "k_ce_pack");
     return DLMI_OK;
   }
   int pack_rows(bool back) const {
     E const *const x = static_cast<E const *>(a.X);
     char *const across = back && a.dW != nullptr ? s + p.xt : nullptr;
-    if (p.rows_x == 32) return pack<32, true>(x, a.B, p.Bp, p.unscale_x, p.parts_x, s + p.xp, across);
-    return pack<8, true>(x, a.B, p.Bp, p.unscale_x, p.parts_x, s + p.xp, across);
+    if (p.Kp <= 1024) return pack<4, true>(x, a.B, p.Bp, p.pack_x, p.unscale_x, 0, back, s + p.xp, across);
+    return pack<8, true>(x, a.B, p.Bp, p.pack_x, p.unscale_x, 0, back, s + p.xp, across);
   }
+  unsigned pack_w(size_t vp) const { return vp / 8 < p.pack_w ? static_cast<unsigned>(vp / 8) : p.pack_w; }
   int pack_classes(size_t v0, size_t vn, size_t vp, bool back) const {
     E const *const w = static_cast<E const *>(a.W) + v0 * a.K;
     char *const across = back && a.dX != nullptr ? s + p.wt : nullptr;
-    if (p.rows_w == 32) return pack<32, false>(w, vn, vp, p.unscale_w, p.parts_w, s + p.wp, across);
-    return pack<8, false>(w, vn, vp, p.unscale_w, p.parts_w, s + p.wp, across);
+    if (p.Kp <= 1024) return pack<4, false>(w, vn, vp, pack_w(vp), p.unscale_w, v0 / p.Vc, back, s + p.wp, across);
+    return pack<8, false>(w, vn, vp, pack_w(vp), p.unscale_w, v0 / p.Vc, back, s + p.wp, across);
   }
   CeLogits logits(size_t v0, size_t vn, size_t vp) const {
     CeLogits g = {};
@@ -923,10 +976,9 @@ struct CeRun {
     g.Q = s + p.xp;
     g.unscale_w = floats(p.unscale_w);
     g.unscale_x = floats(p.unscale_x);
-    g.parts_w = floats(p.parts_w);
-    g.parts_x = floats(p.parts_x);
-    g.nparts_w = static_cast<unsigned>(vp / p.rows_w);
-    g.nparts_x = p.nparts_x;
+    g.unscale_xw = floats(p.unscale_xw);
+    g.most_x = floats(p.most_x);
+    g.most_w = floats(p.most_w) + v0 / p.Vc;
     g.ni = static_cast<unsigned>(vp / p.T);
     g.nj = static_cast<unsigned>(p.Bp / p.T);
     g.kblocks = static_cast<unsigned>(p.Kp / 16);
@@ -979,12 +1031,12 @@ struct CeRun {
       }
       if (a.dX != nullptr) {
         hipLaunchKernelGGL((k_ce_dx<T, NP>), dim3(nb * nk * p.slices), dim3(256), 0, ctx->stream, s + p.dlb, s + p.wt, nb, nk, kv, ce_stages(T, vp),
-                           p.per_slice, g.parts_w, g.nparts_w, floats(p.dxacc), a.B, a.K, v0 == 0 ? 1 : 0);
+                           p.per_slice, g.most_w, floats(p.dxacc), a.B, a.K, v0 == 0 ? 1 : 0);
         DLMI_LAUNCH_CHECK(ctx, "k_ce_dx");
       }
       if (a.dW != nullptr) {
         hipLaunchKernelGGL((k_ce_dw<T, NP, E>), dim3(g.ni * nk), dim3(256), 0, ctx->stream, s + p.dlv, s + p.xt, g.ni, nk, kb,
-                           ce_stages(T, a.B), g.parts_x, g.nparts_x, a.scale, static_cast<E *>(a.dW) + v0 * a.K, vn, a.K,
+                           ce_stages(T, a.B), g.most_x, a.scale, static_cast<E *>(a.dW) + v0 * a.K, vn, a.K,
                            a.accumulate);
         DLMI_LAUNCH_CHECK(ctx, "k_ce_dw");
       }
