@@ -138,6 +138,7 @@ class Dlmi:
             raise DlmiError("dlmi_ctx_create failed with %d" % rc)
         self.ctx = ctx
         self._stream = stream
+        self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # the stream's handle, without an object made for it
         self._types = {torch.float32: DTYPE["F32"], torch.bfloat16: DTYPE["BF16"]}
 
     def close(self):
@@ -176,13 +177,22 @@ class Dlmi:
         assert t.dtype in self._types, "float32 or bfloat16 tensors, not %s" % t.dtype
         return self._types[t.dtype]
 
+    def _current(self):
+        """Whether the context's stream is the current one: outputs made by torch belong to it then."""
+        if self._raw_stream is not None:
+            return self._raw_stream(self.device.index) == self._stream
+        return self.torch.cuda.current_stream(self.device).cuda_stream == self._stream
+
     def _out(self, dtype, *shape):
         """An output that belongs to the context's stream, whichever stream is current."""
         torch = self.torch
-        if torch.cuda.current_stream(self.device).cuda_stream == self._stream:
+        if self._current():
             return torch.empty(shape, dtype=dtype, device=self.device)
         with torch.cuda.stream(torch.cuda.ExternalStream(self._stream, device=self.device)):
             return torch.empty(shape, dtype=dtype, device=self.device)
+
+    def _out_like(self, t):
+        return self.torch.empty_like(t) if t.is_contiguous() and self._current() else self._out(t.dtype, *t.shape)
 
     def empty(self, *shape, dtype=None):
         return self.torch.empty(*shape, dtype=dtype or self.torch.float32, device=self.device)
@@ -642,8 +652,8 @@ class Dlmi:
         """y = residual_scale x + branch_scale f(gate) post(u), h = pre(y) (dlmi_block_norm_fwd).  Returns (y, h)."""
         B, H = u.shape
         kind, dtype = self._type(u), u.dtype
-        y = y if y is not None else self._out(dtype, B, H)
-        h = h if h is not None else self._out(dtype, B, H)
+        y = y if y is not None else self._out_like(u)
+        h = h if h is not None else self._out_like(u)
         for t, what in ((u, "u"), (x, "x"), (y, "y"), (h, "h")):
             self._chk_is(t, what, dtype, B, H)
         if gate is not None and desc.gate_rows:
@@ -660,9 +670,9 @@ class Dlmi:
         is not there; grads: a dict of fp32 tensors for the last four (needed to accumulate), made where missing."""
         B, H = u.shape
         kind, dtype = self._type(u), u.dtype
-        dx = dx if dx is not None else self._out(dtype, B, H)
-        du = du if du is not None else self._out(dtype, B, H)
-        dgate = dgate if dgate is not None or gate is None else self._out(dtype, *gate.shape)
+        dx = dx if dx is not None else self._out_like(u)
+        du = du if du is not None else self._out_like(u)
+        dgate = dgate if dgate is not None or gate is None else self._out_like(gate)
         o = dict(dx=dx, du=du, dgate=dgate)
         params = dict(dw_post=w_post, db_post=b_post, dw_pre=w_pre, db_pre=b_pre)
         given = grads or {}
