@@ -368,43 +368,44 @@ __global__ __launch_bounds__(64 * kParts) void k_ce_join(CeArgs a, float2 const 
 // Forward for up to 64 rows of the batch (NB blocks of 32), bound by reading W: packing it would move it three times.  A
 // workgroup takes 32 VB classes at a time; its NW wavefronts share the features between them (every NW-th 64 bytes of a
 // lane's row), multiply the tensors' own type (bf16, or fp32 on the fp32 matrix pipe, which keeps up with memory at 64 rows) and
-// join in LDS.  A lane holds 64 consecutive bytes of its row, so that whole lines are requested at once; the products'
-// k order is permuted alike on both sides.  The last workgroup to finish joins all partial sums, in a fixed order.
+// join in LDS.  The last workgroup to finish joins all partial sums, in a fixed order.
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
-// 64 bytes of a row, as four registers of four words; at any alignment.
+// A lane's 64 bytes of a step: four pieces of 16, 16 G apart (G lanes share a row, so that a load takes 16 G consecutive
+// bytes of it); at any alignment.
 struct CeLine {
   u32x4 q[4];
 };
 template <class E>
-struct __attribute__((packed, aligned(sizeof(E)))) CeLineAt {
-  u32x4 q[4];
+struct __attribute__((packed, aligned(sizeof(E)))) CePiece {
+  u32x4 q;
 };
 
-template <class E>
+template <class E, int G>
 __device__ __forceinline__ CeLine ce_line(E const *p) {
-  CeLineAt<E> const v = *reinterpret_cast<CeLineAt<E> const *>(p);
   CeLine r;
 #pragma unroll
-  for (int t = 0; t < 4; ++t) r.q[t] = v.q[t];
+  for (int t = 0; t < 4; ++t) r.q[t] = reinterpret_cast<CePiece<E> const *>(p + t * (G * 16 / static_cast<int>(sizeof(E))))->q;
   return r;
 }
 // The same where the row ends at K; what lies beyond counts as zero.
-template <class E>
+template <class E, int G>
 __device__ CeLine ce_line_tail(E const *row, size_t k, size_t K) {
-  constexpr int N = 64 / sizeof(E);
+  constexpr int N = 16 / sizeof(E);
   union {
-    E e[N];
+    E e[4 * N];
     CeLine l;
   } u;
 #pragma unroll
-  for (int i = 0; i < N; ++i) u.e[i] = k + i < K ? row[k + i] : static_cast<E>(0.0f);
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int i = 0; i < N; ++i) u.e[t * N + i] = k + t * G * N + i < K ? row[k + t * G * N + i] : static_cast<E>(0.0f);
   return u.l;
 }
 
 // Blocks of RB classes x RB rows of the batch: RB = 32 or, for up to 16 rows of the batch, 16 (fp32 products of 32 columns
-// cost 3.5 us where four rows of the batch wait for 20 MB).  A lane holds class lane % RB and, of every step, the line
-// lane / RB; its results are column lane % RB.
+// cost 3.5 us where four rows of the batch wait for 20 MB).  A lane holds class lane % RB, and piece lane / RB of every G =
+// 64 / RB of its row; its results are column lane % RB.
 template <int RB>
 struct CeShape;
 template <>
@@ -463,14 +464,14 @@ __global__ __launch_bounds__(NW * 64, 2) void k_ce_direct(CeArgs a, float2 *part
   };
   // G lines of every row are a step; the wavefront's next step is on its way meanwhile, also
   // across blocks of classes
-  size_t const steps = a.K / (G * N), mine = static_cast<size_t>(lane / RB) * N;
+  size_t const steps = a.K / (G * N), mine = static_cast<size_t>(lane / RB) * (N / 4);
   bool const tail = a.K % (G * N) != 0 && static_cast<int>(steps % NW) == wave;
   CeLine lw[VB], lx[NB];
   auto const load = [&](size_t s) {
 #pragma unroll
-    for (int m = 0; m < VB; ++m) lw[m] = ce_line<E>(w[m] + s * G * N + mine);
+    for (int m = 0; m < VB; ++m) lw[m] = ce_line<E, G>(w[m] + s * G * N + mine);
 #pragma unroll
-    for (int n = 0; n < NB; ++n) lx[n] = ce_line<E>(x[n] + s * G * N + mine);
+    for (int n = 0; n < NB; ++n) lx[n] = ce_line<E, G>(x[n] + s * G * N + mine);
   };
   auto const join = [](float2 &p, float2 q) {
     float const most = fmaxf(p.x, q.x);
@@ -497,9 +498,9 @@ __global__ __launch_bounds__(NW * 64, 2) void k_ce_direct(CeArgs a, float2 *part
     if (tail) {
       CeLine tw[VB], tx[NB];
 #pragma unroll
-      for (int m = 0; m < VB; ++m) tw[m] = ce_line_tail<E>(w[m], steps * G * N + mine, a.K);
+      for (int m = 0; m < VB; ++m) tw[m] = ce_line_tail<E, G>(w[m], steps * G * N + mine, a.K);
 #pragma unroll
-      for (int n = 0; n < NB; ++n) tx[n] = ce_line_tail<E>(x[n], steps * G * N + mine, a.K);
+      for (int n = 0; n < NB; ++n) tx[n] = ce_line_tail<E, G>(x[n], steps * G * N + mine, a.K);
       multiply(tw, tx);
     }
     CeLine cw[VB], cx[NB];
