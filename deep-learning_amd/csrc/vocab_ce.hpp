@@ -153,14 +153,15 @@ __global__ __launch_bounds__(kCeBlock) void k_ce_pack(CeArgs a, T const *src, si
     flip ^= 1;
     float const scale = ce_scale(m);
     // across = as * ratio, ratio = weight * scale_across / scale
-    float ratio = r < rows ? 1.0f : 0.0f, un = ce_unscale(scale);
+    // (a row of zeros has no share in a product, so none in the largest either)
+    float ratio = r < rows ? 1.0f : 0.0f, un = m > 0.0f ? ce_unscale(scale) : 0.0f;
     if ((lane & 7) == 0 && wave == 0) unscale[r] = un;
     if constexpr (LABELS) {
       int const l = r < rows ? a.labels[r] : -1;
       float const w = l >= 0 && static_cast<size_t>(l) < a.V ? ce_row_weight(a, r) : 0.0f;
       float const s2 = ce_scale(fabsf(w) * m);
-      ratio = l >= 0 && static_cast<size_t>(l) < a.V ? w * (s2 * un) : 0.0f;
-      un = w != 0.0f ? ce_unscale(s2) : 0.0f;
+      ratio = l >= 0 && static_cast<size_t>(l) < a.V ? w * (s2 * ce_unscale(scale)) : 0.0f;
+      un = w != 0.0f && m > 0.0f ? ce_unscale(s2) : 0.0f;
       if ((lane & 7) == 0 && wave == 0) unscale_across[r] = un;
     }
     mine = fmaxf(mine, r < rows ? un : 0.0f);
@@ -687,7 +688,8 @@ __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_grad(CeArgs a, CeL
   int const lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   half8 const id0 = half_identity(0, lane), id1 = half_identity(1, lane);
   // (powers of two, so their inverses are exact)
-  float const inv_w = 1.0f / g.most_w[0], most_x = g.most_x[0], inv_x = most_x > 0.0f ? 1.0f / most_x : 0.0f;
+  float const most_w = g.most_w[0], most_x = g.most_x[0];
+  float const inv_w = most_w > 0.0f ? 1.0f / most_w : 0.0f, inv_x = most_x > 0.0f ? 1.0f / most_x : 0.0f;
   size_t const c0 = static_cast<size_t>(ti) * T + (wave >> 1) * (T / 2);
   size_t const b0 = static_cast<size_t>(tj) * T + (wave & 1) * (T / 2);
   size_t const rb = static_cast<size_t>(kblocks_v) * NP * kFragBytes, rv = static_cast<size_t>(kblocks_b) * NP * kFragBytes;

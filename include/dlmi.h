@@ -311,8 +311,10 @@ int dlmi_loss_seed(dlmi_ctx *ctx, dlmi_loss loss, dlmi_accuracy accu, float accu
  *   z = X W^T + bias;  lse[b] = log sum_v exp z[b,v];  loss[b] = lse[b] - z[b, labels[b]].
  * X [B, K], W [V, K] of `type`; bias [V] fp32 or NULL; labels [B] int32: a label outside [0, V) leaves its row out (loss
  * 0, no gradient; its lse is still that of its logits).  loss, lse [B] fp32.  fp32 tensors are multiplied to the precision
- * of fp32 products, bf16 ones exactly, sums in fp32.  The vocabulary is walked in pieces; the context's scratch holds
- * one piece's operands (at most about 1 GiB), the rows of X and 8 bytes per row and 128 classes, never [B, V]. */
+ * of fp32 products, bf16 ones exactly, sums in fp32.  A non-finite row of X makes its own loss and lse NaN.  The vocabulary
+ * is walked in pieces; the context's scratch holds one piece's operands (at most about 1 GiB), the rows of X and 8 bytes
+ * per row and 32 to 128 classes, never [B, V].  As with every call that uses the scratch, graphs recorded from one context
+ * must not be replayed at the same time. */
 #define DLMI_VOCAB_CE_MAX_ROWS 262144
 #define DLMI_VOCAB_CE_MAX_FEATURES 65536
 int dlmi_vocab_ce_fwd(dlmi_ctx *ctx, dlmi_dtype type, size_t B, size_t K, size_t V, void const *X, void const *W,
@@ -321,7 +323,7 @@ int dlmi_vocab_ce_fwd(dlmi_ctx *ctx, dlmi_dtype type, size_t B, size_t K, size_t
 /* Its gradient.  g[b] = scale * dloss[b] (dloss NULL: scale), 0 for rows left out; lse from the forward.
  *   dL[b,v] = exp(z[b,v] - lse[b]) - [v == labels[b]];  dX = g dL W;  dW (+)= (g dL)^T X;  db (+)= sum_b g[b] dL[b,.]
  * dX [B, K], dW [V, K] of `type`, db [V] fp32; each may be NULL.  dX is written (zero in rows left out); accumulate != 0
- * adds into dW and db.  The logits are formed again, piece by piece.  All sums are taken in an order that depends on the
+ * adds into dW and db.  B, K and V must not be 0.  The logits are formed again, piece by piece.  All sums are taken in an order that depends on the
  * sizes only. */
 int dlmi_vocab_ce_bwd(dlmi_ctx *ctx, dlmi_dtype type, size_t B, size_t K, size_t V, void const *X, void const *W,
                       float const *bias, int32_t const *labels, float const *lse, float const *dloss, float scale, void *dX,

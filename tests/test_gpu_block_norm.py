@@ -207,6 +207,66 @@ def test_nonfinite_rows_stay_alone(dl, pkg):
 
 
 @pytest.mark.gpu
+def test_captured_and_replayed(pkg):
+    """Forward and backward recorded into a HIP graph and replayed with eager work between: the eager bits every time."""
+    d = pkg.Dlmi(0)
+    try:
+        stream = torch.cuda.Stream()
+        d.set_stream(stream)
+        t = dev(make(60, 300, BF16, "RMS", "LAYER", 7, True, True, 2))
+        desc = pkg.Dlmi.block_norm_desc(post=1, pre=2, gate_rows=7, gate_act=pkg.GATE_ACT["TANH"])
+        params = {k: t[k] for k in ("w_post", "b_post", "w_pre", "b_pre")}
+        new = lambda: (dict(y=torch.empty_like(t["x"]), h=torch.empty_like(t["x"])),
+                       dict(dx=torch.empty_like(t["x"]), du=torch.empty_like(t["x"]), dgate=torch.empty_like(t["gate"]),
+                            grads={k: torch.empty(300, device="cuda") for k in ("dw_post", "db_post", "dw_pre", "db_pre")}))
+        xs = [torch.randn_like(t["x"]) for _ in range(4)]
+        def step(x, o, g):
+            d.block_norm_fwd(desc, x, t["u"], gate=t["gate"], **params, **o)
+            d.block_norm_bwd(desc, t["u"], o["y"], t["dy"], t["dh"], gate=t["gate"], **params, **g)
+        flat = lambda o, g: list(o.values()) + [g["dx"], g["du"], g["dgate"]] + list(g["grads"].values())
+        (eo, eg), (go, gg), x = new(), new(), t["x"].clone()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            step(x, eo, eg)
+            stream.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                step(x, go, gg)
+            for v in xs:
+                x.copy_(v)
+                step(v, eo, eg)
+                graph.replay()
+                stream.synchronize()
+                assert all(torch.equal(p, q) for p, q in zip(flat(eo, eg), flat(go, gg)))
+    finally:
+        torch.cuda.synchronize()
+        d.close()
+
+
+@pytest.mark.gpu
+def test_outputs_belong_to_the_contexts_stream(pkg):
+    """A context on a stream that is not the current one: results are right once that stream is waited for."""
+    d = pkg.Dlmi(0)
+    try:
+        stream = torch.cuda.Stream()
+        d.set_stream(stream)
+        t = dev(make(40, 200, F32, "RMS", "RMS", 0, True, False, 2))
+        torch.cuda.synchronize()
+        desc = pkg.Dlmi.block_norm_desc()
+        y, h = d.block_norm_fwd(desc, t["x"], t["u"], w_post=t["w_post"], w_pre=t["w_pre"])
+        g = d.block_norm_bwd(desc, t["u"], y, t["dy"], t["dh"], w_post=t["w_post"], w_pre=t["w_pre"])
+        stream.synchronize()
+        d.set_stream(torch.cuda.current_stream())
+        y2, h2 = d.block_norm_fwd(desc, t["x"], t["u"], w_post=t["w_post"], w_pre=t["w_pre"])
+        g2 = d.block_norm_bwd(desc, t["u"], y2, t["dy"], t["dh"], w_post=t["w_post"], w_pre=t["w_pre"])
+        torch.cuda.synchronize()
+        assert torch.equal(y, y2) and torch.equal(h, h2) and torch.equal(g["dx"], g2["dx"]) and torch.equal(g["dw_pre"], g2["dw_pre"])
+    finally:
+        torch.cuda.synchronize()
+        d.close()
+
+
+@pytest.mark.gpu
 def test_refusals(dl, pkg):
     x = torch.ones(4, 8, device="cuda")
     w = torch.ones(8, device="cuda")

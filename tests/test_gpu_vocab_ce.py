@@ -171,6 +171,29 @@ def test_masked_classes_and_far_rows(dl):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", [F32, BF16])
+def test_rows_of_zeros(dl, kind):
+    """Rows of X and of W that are zero, or all of X or W: they scale nobody's planes."""
+    for what in ("some", "X", "W"):
+        X, W, b, labels = make(90, 70, 600, kind, True, 0.1, 21)
+        if what == "some":
+            X[5] = X[6] = W[3] = W[500] = 0
+        else:
+            {"X": X, "W": W}[what].zero_()
+        loss, lse = dl.vocab_ce_fwd(X, W, labels, bias=b)
+        g = torch.full((90,), 0.25, device="cuda")
+        eloss, else_, edX, edW, edb, mags, mX, mW, mb, floor = exact(X, W, b, labels, g)
+        dz = dz_of(kind, 70, mags)
+        within(lse, else_, dz + 2.0 ** -22 + 2.0 ** -24 * else_.abs().max().item(), "lse")
+        dX, dW, db = dl.vocab_ce_bwd(X, W, labels, lse, bias=b, scale=0.25)
+        rel = 2 * dz + 2.0 ** -20 + (2.0 ** -12 if kind == BF16 else 0.0)
+        half = 2.0 ** -8 if kind == BF16 else 0.0
+        within(dX, edX, (rel + 600 * 2.0 ** -24) * mX + half * edX.abs() + floor[0], "dX")
+        within(dW, edW, (rel + 90 * 2.0 ** -24) * mW + half * edW.abs() + floor[1], "dW")
+        within(db, edb, (2 * dz + 2.0 ** -20 + 90 * 2.0 ** -24) * mb + floor[2], "db")
+
+
+@pytest.mark.gpu
 def test_nonfinite_rows_stay_alone_forward(dl):
     X, W, b, labels = make(80, 33, 500, F32, False, 0.0, 5)
     loss, lse = dl.vocab_ce_fwd(X, W, labels)
@@ -309,4 +332,5 @@ def test_refusals(dl, pkg):
     assert f(dl.ctx, 0, sz(0), sz(16), sz(40), None, None, None, None, None, None) == 0
     g = lib.dlmi_vocab_ce_bwd
     assert g(dl.ctx, 0, sz(8), sz(16), sz(40), p(X), p(W), None, p(labels), p(lse), None, ctypes.c_float(1), None, None, None, 0) == -1
+    assert g(dl.ctx, 0, sz(0), sz(16), sz(40), p(X), p(W), None, p(labels), p(lse), None, ctypes.c_float(1), p(X.clone()), None, None, 0) == -1
     assert g(dl.ctx, 0, sz(8), sz(16), sz(40), p(X), p(W), None, p(labels), None, None, ctypes.c_float(1), p(X.clone()), None, None, 0) == -1
