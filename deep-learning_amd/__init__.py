@@ -188,7 +188,8 @@ class Dlmi:
         torch = self.torch
         if self._current():
             return torch.empty(shape, dtype=dtype, device=self.device)
-        with torch.cuda.stream(torch.cuda.ExternalStream(self._stream, device=self.device)):
+        own = torch.cuda.ExternalStream(self._stream, device=self.device) if self._stream else torch.cuda.default_stream(self.device)
+        with torch.cuda.stream(own):
             return torch.empty(shape, dtype=dtype, device=self.device)
 
     def _out_like(self, t):

@@ -457,18 +457,16 @@ __global__ __launch_bounds__(NT, NT <= 512 && C * N <= 8 ? 4 : 1) void k_block_n
       t[c][i] *= a.rs;
       u[c][i] = uh;
     }
-bn_store(static_cast<T *>(a.dx) + at, t, at_);
+    bn_store(static_cast<T *>(a.dx) + at, t, at_);
     if (a.post != DLMI_ROW_NORM_NONE) {
       bn_sums<NT>(p, lds, flip);
       weight(kW1, w);
       float const c1 = a.post == DLMI_ROW_NORM_LAYER ? p[0] * inv_h : 0.0f, c2 = p[1] * inv_h;
       BN_EACH e[c][i] = ru_ * (e[c][i] * w[c][i] - c1 - u[c][i] * c2);
     }
-bn_store(static_cast<T *>(a.du) + at, e, at_);
+    bn_store(static_cast<T *>(a.du) + at, e, at_);
     if constexpr (GATE == kBnGateEach) {
-      if (a.dgate != nullptr) {
-bn_store(static_cast<T *>(a.dgate) + at, dg, at_);
-      }
+      if (a.dgate != nullptr) bn_store(static_cast<T *>(a.dgate) + at, dg, at_);
     }
     if constexpr (GATE == kBnGateShared) {
       if (a.direct && ((r + 1) % a.gate_rows == 0 || r + 1 == a.B)) {
@@ -476,7 +474,7 @@ bn_store(static_cast<T *>(a.dgate) + at, dg, at_);
         BN_EACH dg[c][i] *= bn_gate_slope(a.act, f[c][i]);
         if (a.dgate != nullptr) {
           T *const out = static_cast<T *>(a.dgate) + r / a.gate_rows * static_cast<size_t>(H);
-bn_store(out, dg, at_);
+          bn_store(out, dg, at_);
         }
         BN_EACH dg[c][i] = 0.0f;
       }
@@ -628,12 +626,30 @@ static BnArgs bn_args(dlmi_block_norm_desc const *d, size_t B, size_t H) {
   a.post = d->post;
   a.pre = d->pre;
   a.act = d->gate_act;
-  a.gate_rows = d->gate_rows;
+  a.gate_rows = d->gate_rows < B ? d->gate_rows : B;  // one row for all, whatever lies beyond
   a.rs = d->residual_scale;
   a.bs = d->branch_scale;
   a.eps_post = d->eps_post;
   a.eps_pre = d->eps_pre;
   return a;
+}
+
+// No rows: sums over none of them.
+static int bn_no_rows(dlmi_ctx *ctx, size_t B, size_t H, float *dw_post, float *db_post, float *dw_pre, float *db_pre, int accumulate) {
+  if (B != 0 || H == 0 || accumulate) return DLMI_OK;
+  DLMI_REQUIRE_DEVICE(ctx);
+  BnReduce r = {};
+  float *const params[4] = {dw_post, db_post, dw_pre, db_pre};
+  unsigned sums = 0;
+  for (int k = 0; k < 4; ++k) {
+    r.plane[k] = params[k] != nullptr ? static_cast<int>(sums++) : -1;
+    r.out[k] = params[k];
+  }
+  if (sums == 0) return DLMI_OK;
+  r.H = static_cast<int>(H);
+  hipLaunchKernelGGL(k_block_norm_reduce<float>, dim3(static_cast<unsigned>(dlmi_ceil_div(H, 64)), sums), dim3(1024), 0, ctx->stream, r, sums);
+  DLMI_LAUNCH_CHECK(ctx, "k_block_norm_reduce");
+  return DLMI_OK;
 }
 
 }  // namespace dlmi
@@ -653,7 +669,12 @@ int dlmi_block_norm_fwd(dlmi_ctx *ctx, dlmi_dtype type, dlmi_block_norm_desc con
   if (B * H == 0) return DLMI_OK;
   DLMI_REQUIRE_DEVICE(ctx);
   DLMI_REQUIRE(ctx, x != nullptr && u != nullptr && y != nullptr && h != nullptr, "null pointer");
+  size_t const row = H * (type == DLMI_F32 ? 4 : 2);
   BnArgs a = bn_args(desc, B, H);
+  dlmi_span const spans[] = {{y, B * row, true},  {h, B * row, true},       {x, B * row, true},      {u, B * row, true},
+                             {gate, a.gate_rows != 0 ? dlmi_ceil_div(B, a.gate_rows) * row : 0, false}, {w_post, H * 4, false},
+                             {b_post, H * 4, false}, {w_pre, H * 4, false}, {b_pre, H * 4, false}};
+  DLMI_REQUIRE(ctx, !dlmi_spans_collide(spans, 2, 9), "an output overlaps another array");
   a.x = x;
   a.u = u;
   a.gate = gate;
@@ -682,12 +703,20 @@ int dlmi_block_norm_bwd(dlmi_ctx *ctx, dlmi_dtype type, dlmi_block_norm_desc con
   DLMI_REQUIRE(ctx, desc->pre != DLMI_ROW_NORM_NONE || (dw_pre == nullptr && db_pre == nullptr), "gradients of a norm before the block that is not there");
   DLMI_REQUIRE(ctx, desc->gate_rows != 0 || dgate == nullptr, "the gradient of a gate that is not there");
   if (H > DLMI_BLOCK_NORM_MAX_WIDTH) return dlmi_fail(ctx, DLMI_E_UNSUPPORTED, "%s: rows wider than %d", __func__, kBnMaxWidth);
-  if (B * H == 0) return DLMI_OK;
+  if (B * H == 0) return bn_no_rows(ctx, B, H, dw_post, db_post, dw_pre, db_pre, accumulate);
   DLMI_REQUIRE_DEVICE(ctx);
   DLMI_REQUIRE(ctx, u != nullptr && dx != nullptr && du != nullptr, "null pointer");
   DLMI_REQUIRE(ctx, dy != nullptr || dh != nullptr, "no gradient to start from");
   DLMI_REQUIRE(ctx, y != nullptr || dh == nullptr || desc->pre == DLMI_ROW_NORM_NONE, "null pointer");
   BnArgs a = bn_args(desc, B, H);
+  size_t const row = H * (type == DLMI_F32 ? 4 : 2);
+  size_t const gr = a.gate_rows != 0 ? a.gate_rows : 1;
+  size_t const runs = dlmi_ceil_div(B, gr);
+  dlmi_span const spans[] = {{dx, B * row, true}, {du, B * row, true}, {dgate, runs * row, false}, {dw_post, H * 4, false},
+                             {db_post, H * 4, false}, {dw_pre, H * 4, false}, {db_pre, H * 4, false}, {u, B * row, true},
+                             {y, B * row, true}, {dy, B * row, true}, {dh, B * row, true}, {gate, runs * row, false},
+                             {w_post, H * 4, false}, {b_post, H * 4, false}, {w_pre, H * 4, false}};
+  DLMI_REQUIRE(ctx, !dlmi_spans_collide(spans, 7, 15), "an output overlaps another array");
   a.u = u;
   a.y = const_cast<void *>(y);
   a.gate = gate;
@@ -707,9 +736,7 @@ int dlmi_block_norm_bwd(dlmi_ctx *ctx, dlmi_dtype type, dlmi_block_norm_desc con
   size_t const nt = static_cast<size_t>(bn_threads(a.H, bn_each(type, true)));
   size_t const most = static_cast<size_t>(ctx->num_cu) * (nt < 1024 ? 1024 / nt : 1);
   size_t want = dlmi_ceil_div(B, most);
-  if ((sums != 0 || desc->gate_rows > 1) && want < 4) want = 4;
-  size_t const gr = desc->gate_rows != 0 ? desc->gate_rows : 1;
-  size_t const runs = dlmi_ceil_div(B, gr);
+  if ((sums != 0 || gr > 1) && want < 4) want = 4;
   size_t blocks;
   a.slices = 1;
   a.direct = gr <= want ? 1 : 0;

@@ -117,6 +117,23 @@ inline int dlmi_fail(dlmi_ctx *ctx, int code, char const *fmt, ...) {
       return dlmi_fail((ctx), DLMI_E_INVALID, "%s: the context's device is not current", __func__); \
   } while (0)
 
+// An array a call reads or writes, and whether the first outputs of a call collide with it: an output may overlap no other
+// array, but be one of the arrays marked `same` (read before it is written, element by element).
+struct dlmi_span {
+  void const *p;
+  size_t bytes;
+  bool same;
+};
+inline bool dlmi_spans_collide(dlmi_span const *s, int outputs, int all) {
+  for (int i = 0; i < outputs; ++i)
+    for (int k = i + 1; k < all; ++k) {
+      uintptr_t const x = reinterpret_cast<uintptr_t>(s[i].p), y = reinterpret_cast<uintptr_t>(s[k].p);
+      if (x == 0 || y == 0 || x >= y + s[k].bytes || y >= x + s[i].bytes) continue;
+      if (k < outputs || !s[i].same || !s[k].same || x != y) return true;
+    }
+  return false;
+}
+
 // Makes sure the context's scratch holds at least `bytes`.
 // Growing allocates (and synchronizes the stream): it is refused while the
 // stream is being captured into a HIP graph.

@@ -22,6 +22,10 @@ int dlmi_vocab_ce_fwd(dlmi_ctx *ctx, dlmi_dtype type, size_t B, size_t K, size_t
   DLMI_REQUIRE_DEVICE(ctx);
   DLMI_REQUIRE(ctx, K != 0 && V != 0, "no features or no classes");
   DLMI_REQUIRE(ctx, X != nullptr && W != nullptr && labels != nullptr && loss != nullptr && lse != nullptr, "null pointer");
+  size_t const e = type == DLMI_F32 ? 4 : 2;
+  dlmi_span const spans[] = {{loss, B * 4, false}, {lse, B * 4, false}, {X, B * K * e, false}, {W, V * K * e, false}, {bias, V * 4, false},
+                             {labels, B * 4, false}};
+  DLMI_REQUIRE(ctx, !dlmi_spans_collide(spans, 2, 6), "an output must not be written over another array");
   CeArgs a = {};
   a.B = B;
   a.K = K;
@@ -45,7 +49,10 @@ int dlmi_vocab_ce_bwd(dlmi_ctx *ctx, dlmi_dtype type, size_t B, size_t K, size_t
   DLMI_REQUIRE_DEVICE(ctx);
   DLMI_REQUIRE(ctx, X != nullptr && W != nullptr && labels != nullptr && lse != nullptr, "null pointer");
   DLMI_REQUIRE(ctx, dX != nullptr || dW != nullptr || db != nullptr, "no gradient asked for");
-  DLMI_REQUIRE(ctx, dX != X && dW != W && (dX == nullptr || dX != W) && (dW == nullptr || dW != X), "a gradient must not be written over X or W");
+  size_t const e = type == DLMI_F32 ? 4 : 2;
+  dlmi_span const spans[] = {{dX, B * K * e, false}, {dW, V * K * e, false}, {db, V * 4, false},   {X, B * K * e, false}, {W, V * K * e, false},
+                             {bias, V * 4, false},   {labels, B * 4, false}, {lse, B * 4, false}, {dloss, B * 4, false}};
+  DLMI_REQUIRE(ctx, !dlmi_spans_collide(spans, 3, 9), "a gradient must not be written over another array");
   CeArgs a = {};
   a.B = B;
   a.K = K;

@@ -161,7 +161,7 @@ __global__ __launch_bounds__(kCeBlock) void k_ce_pack(CeArgs a, T const *src, si
       float const w = l >= 0 && static_cast<size_t>(l) < a.V ? ce_row_weight(a, r) : 0.0f;
       float const s2 = ce_scale(fabsf(w) * m);
       ratio = l >= 0 && static_cast<size_t>(l) < a.V ? w * (s2 * ce_unscale(scale)) : 0.0f;
-      un = w != 0.0f && m > 0.0f ? ce_unscale(s2) : 0.0f;
+      un = fabsf(w) * m > 0.0f ? ce_unscale(s2) : 0.0f;
       if ((lane & 7) == 0 && wave == 0) unscale_across[r] = un;
     }
     mine = fmaxf(mine, r < rows ? un : 0.0f);

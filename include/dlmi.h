@@ -323,8 +323,10 @@ int dlmi_vocab_ce_fwd(dlmi_ctx *ctx, dlmi_dtype type, size_t B, size_t K, size_t
 /* Its gradient.  g[b] = scale * dloss[b] (dloss NULL: scale), 0 for rows left out; lse from the forward.
  *   dL[b,v] = exp(z[b,v] - lse[b]) - [v == labels[b]];  dX = g dL W;  dW (+)= (g dL)^T X;  db (+)= sum_b g[b] dL[b,.]
  * dX [B, K], dW [V, K] of `type`, db [V] fp32; each may be NULL.  dX is written (zero in rows left out); accumulate != 0
- * adds into dW and db.  B, K and V must not be 0.  The logits are formed again, piece by piece.  All sums are taken in an order that depends on the
- * sizes only. */
+ * adds into dW and db.  B, K and V must not be 0; a gradient must not overlap another array.  The logits are formed again,
+ * piece by piece.  All sums are taken in an order that depends on the sizes only.
+ * dX is as exact as a sum of terms of the size of W's largest row, dW as one of the largest |dloss| |X| of a row that counts
+ * (so a padding row of W must hold values of ordinary size; rows of X that are left out may hold anything). */
 int dlmi_vocab_ce_bwd(dlmi_ctx *ctx, dlmi_dtype type, size_t B, size_t K, size_t V, void const *X, void const *W,
                       float const *bias, int32_t const *labels, float const *lse, float const *dloss, float scale, void *dX,
                       void *dW, float *db, int accumulate);
@@ -472,7 +474,7 @@ int dlmi_fused_norm_act_infer(dlmi_ctx *ctx, dlmi_fused_desc const *desc, size_t
  * bias [H] (each may be NULL).  f: DLMI_ACT_LINEAR, SIGMOID or TANH.  gate [ceil(B / gate_rows), H]: gate_rows
  * consecutive rows share one of its rows (1: one each, B: one for all); gate_rows == 0 and gate == NULL: no gate.
  * x, u, gate, y, h [B, H] are of `type`, weights and biases fp32; a row is computed in fp32 and rounded once, h from the
- * y before rounding.  y may alias x, h may alias u.  H up to DLMI_BLOCK_NORM_MAX_WIDTH (DLMI_E_UNSUPPORTED beyond). */
+ * y before rounding.  y and h may each be x or u; nothing else may overlap them.  H up to DLMI_BLOCK_NORM_MAX_WIDTH (DLMI_E_UNSUPPORTED beyond). */
 typedef enum { DLMI_ROW_NORM_NONE = 0, DLMI_ROW_NORM_RMS = 1, DLMI_ROW_NORM_LAYER = 2 } dlmi_row_norm;
 #define DLMI_BLOCK_NORM_MAX_WIDTH 16384
 typedef struct {
@@ -490,7 +492,8 @@ int dlmi_block_norm_fwd(dlmi_ctx *ctx, dlmi_dtype type, dlmi_block_norm_desc con
  * (the statistics are formed again from u and y; y may be NULL where dh is or pre is NONE).  dx, du [B, H] and dgate
  * [ceil(B / gate_rows), H] (may be NULL) are written; the weights' and biases' gradients (fp32 [H], each may be NULL) are
  * added to where accumulate != 0, written otherwise.  All sums over rows are taken in an order that depends on the sizes
- * only.  dx may alias dy, du may alias dh. */
+ * only.  dx and du may each be u, y, dy or dh; nothing else may overlap what is written.
+ * Of no rows (B = 0) the weights' and biases' gradients are 0. */
 int dlmi_block_norm_bwd(dlmi_ctx *ctx, dlmi_dtype type, dlmi_block_norm_desc const *desc, size_t B, size_t H, void const *u,
                         void const *y, void const *gate, float const *w_post, float const *b_post, float const *w_pre,
                         void const *dy, void const *dh, void *dx, void *du, void *dgate, float *dw_post, float *db_post,
@@ -552,8 +555,7 @@ int dlmi_opt_irprop_plus(dlmi_ctx *ctx, size_t n, float *params, float *grads, f
  * vectors: `steps` times A = X X^T, X <- a X + (b A + c A A) X, on the shorter side of the matrix.  The usual values are
  * a, b, c = 3.4445, -4.7750, 2.0315 in 5 steps.  Computed to the precision of fp32 products; the last step of a bf16 result in
  * 11 bits.  Coefficients that would take a singular value s of [0, 1], its square or a + b s^2 + c s^4 beyond 8 on the way are
- * refused.  A
- * zero matrix gives zero; a non-finite element makes every element of the result non-finite. */
+ * refused.  A zero matrix gives zero; a non-finite element makes every element of the result non-finite. */
 typedef struct {
   float a, b, c;
   int steps;  /* 1 .. 64 */
@@ -569,7 +571,7 @@ int dlmi_orthogonalize(dlmi_ctx *ctx, dlmi_dtype type, size_t rows, size_t cols,
  * p -= lr * orthogonalize(u) + wd*p; the gradient is zeroed.  fp32, updated in place.  Matrices of the same shape
  * share their launches.  No two of the arrays may overlap.  `problems` is a host array; the pointers in it are device.
  * The context's scratch grows to about 20 bytes per element of the matrices launched together (at most 2 GiB of it,
- * more for a single larger matrix). */
+ * more for a single larger matrix), plus 128 MiB for large ones. */
 typedef struct {
   size_t rows, cols;
   float *params, *grads, *momentum; /* [rows, cols] each */

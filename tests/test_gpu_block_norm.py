@@ -244,6 +244,46 @@ def test_captured_and_replayed(pkg):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", [F32, BF16])
+@pytest.mark.parametrize("H", [5, 130])
+def test_outputs_over_inputs(dl, pkg, kind, H):
+    """What the documentation lets an output be: the bits are those of separate outputs."""
+    t = dev(make(37, H, kind, "RMS", "LAYER", 5, True, True, 3))
+    desc = pkg.Dlmi.block_norm_desc(post=1, pre=2, gate_rows=5, gate_act=pkg.GATE_ACT["SIGMOID"])
+    params = {k: t[k] for k in ("w_post", "b_post", "w_pre", "b_pre")}
+    y, h = dl.block_norm_fwd(desc, t["x"], t["u"], gate=t["gate"], **params)
+    for names in (("x", "u"), ("u", "x")):
+        x, u = t["x"].clone(), t["u"].clone()
+        o = dict(x=x, u=u)
+        dl.block_norm_fwd(desc, x, u, gate=t["gate"], y=o[names[0]], h=o[names[1]], **params)
+        assert torch.equal(o[names[0]], y) and torch.equal(o[names[1]], h)
+    g = dl.block_norm_bwd(desc, t["u"], y, t["dy"], t["dh"], gate=t["gate"], **params)
+    for names in (("dy", "dh"), ("dh", "dy"), ("u", "y")):
+        o = dict(u=t["u"].clone(), y=y.clone(), dy=t["dy"].clone(), dh=t["dh"].clone())
+        r = dl.block_norm_bwd(desc, o["u"], o["y"], o["dy"], o["dh"], gate=t["gate"], dx=o[names[0]], du=o[names[1]], **params)
+        assert all(torch.equal(r[k], g[k]) for k in g)
+
+
+@pytest.mark.gpu
+def test_a_gate_for_all_and_no_rows(dl, pkg):
+    """gate_rows beyond B: one row of the gate for all.  B = 0: the parameters' gradients are 0, or stay."""
+    t = dev(make(9, 64, F32, "RMS", "RMS", 9, True, False, 2))
+    w = dict(w_post=t["w_post"], w_pre=t["w_pre"])
+    both = []
+    for rows in (9, 2 ** 64 - 1):
+        desc = pkg.Dlmi.block_norm_desc(gate_rows=rows)
+        y, h = dl.block_norm_fwd(desc, t["x"], t["u"], gate=t["gate"], **w)
+        g = dl.block_norm_bwd(desc, t["u"], y, t["dy"], t["dh"], gate=t["gate"], **w)
+        both.append([y, h, g["dx"], g["du"], g["dgate"], g["dw_post"], g["dw_pre"]])
+    assert all(torch.equal(p, q) for p, q in zip(*both))
+    e = torch.empty(0, 64, device="cuda")
+    for accumulate, left in ((False, 0.0), (True, 3.0)):
+        grads = dict(dw_post=torch.full((64,), 3.0, device="cuda"), dw_pre=torch.full((64,), 3.0, device="cuda"))
+        dl.block_norm_bwd(pkg.Dlmi.block_norm_desc(), e, e, e, e, grads=grads, accumulate=accumulate, **w)
+        assert bool((grads["dw_post"] == left).all()) and bool((grads["dw_pre"] == left).all())
+
+
+@pytest.mark.gpu
 def test_outputs_belong_to_the_contexts_stream(pkg):
     """A context on a stream that is not the current one: results are right once that stream is waited for."""
     d = pkg.Dlmi(0)
@@ -296,6 +336,23 @@ def test_refusals(dl, pkg):
         dl.block_norm_fwd(D(), x, x.clone(), w_pre=w.double())
     with pytest.raises(AssertionError):
         dl.block_norm_fwd(D(), x, torch.ones(8, 4, device="cuda").t())
+    flat = torch.ones(40, device="cuda")
+    a, c = flat[:32].view(4, 8), flat[8:].view(4, 8)
+    u = x.clone()
+    for over in (dict(y=a, h=a), dict(y=a, h=c)):
+        with pytest.raises(pkg.DlmiError, match="overlaps"):
+            dl.block_norm_fwd(D(), x, u, **over)
+    with pytest.raises(pkg.DlmiError, match="overlaps"):
+        dl.block_norm_fwd(D(), a, u, y=c)
+    with pytest.raises(pkg.DlmiError, match="overlaps"):
+        dl.block_norm_fwd(D(gate_rows=1), x, u, gate=a, h=a)
+    with pytest.raises(pkg.DlmiError, match="overlaps"):
+        dl.block_norm_fwd(D(), x, u, w_pre=flat[:8], h=a)
+    for over in (dict(dx=a, du=a), dict(dx=a, du=c), dict(dx=a, grads=dict(dw_post=flat[:8])), dict(grads=dict(dw_post=w))):
+        with pytest.raises(pkg.DlmiError, match="overlaps"):
+            dl.block_norm_bwd(D(), u, x, x.clone(), None, w_post=w, **over)
+    with pytest.raises(pkg.DlmiError, match="overlaps"):
+        dl.block_norm_bwd(D(gate_rows=1), u, x, x.clone(), None, gate=a, dgate=a)
     e = torch.empty(0, 8, device="cuda")
     y, h = dl.block_norm_fwd(D(), e, e.clone())
     assert y.shape == (0, 8)

@@ -171,6 +171,21 @@ def test_masked_classes_and_far_rows(dl):
 
 
 @pytest.mark.gpu
+def test_weights_that_underflow(dl):
+    """A row whose dloss X is below every fp32 value counts nothing, and costs the others nothing."""
+    X, W, b, labels = make(70, 48, 300, F32, True, 0.0, 23)
+    X[9] *= 1e-30
+    g = torch.ones(70, device="cuda")
+    g[9] = 1e-25
+    eloss, else_, edX, edW, edb, mags, mX, mW, mb, floor = exact(X, W, b, labels, g)
+    loss, lse = dl.vocab_ce_fwd(X, W, labels, bias=b)
+    dX, dW, db = dl.vocab_ce_bwd(X, W, labels, lse, bias=b, dloss=g)
+    rel = 2 * dz_of(F32, 48, mags) + 2.0 ** -20
+    within(dW, edW, (rel + 70 * 2.0 ** -24) * mW + floor[1], "dW")
+    within(dX, edX, (rel + 300 * 2.0 ** -24) * mX + floor[0], "dX")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind", [F32, BF16])
 def test_rows_of_zeros(dl, kind):
     """Rows of X and of W that are zero, or all of X or W: they scale nobody's planes."""
@@ -320,6 +335,15 @@ def test_refusals(dl, pkg):
         dl.vocab_ce_bwd(X, W, labels, lse, bias=b, accumulate=True)
     with pytest.raises(pkg.DlmiError, match="written over"):
         dl.vocab_ce_bwd(X, W, labels, lse, dX=X)
+    both = torch.zeros(8 * 16 + 40 * 16, device="cuda")
+    for over in (dict(dX=both[:128].view(8, 16), dW=both[120:760].view(40, 16)), dict(dW=W), dict(dX=lse.new_zeros(8, 16), dW=W),
+                 dict(db=b), dict(db=W.flatten()[:40])):
+        with pytest.raises(pkg.DlmiError, match="written over"):
+            dl.vocab_ce_bwd(X, W, labels, lse, bias=b, **over)
+    with pytest.raises(pkg.DlmiError, match="written over"):
+        dl.vocab_ce_fwd(X, W, labels, bias=b, loss=loss, lse=loss)
+    with pytest.raises(pkg.DlmiError, match="written over"):
+        dl.vocab_ce_fwd(X, W, labels, bias=b, loss=loss, lse=X.flatten()[4:12])
     sz, p = ctypes.c_size_t, lambda t: ctypes.c_void_p(t.data_ptr())
     lib = dl.lib
     f = lib.dlmi_vocab_ce_fwd
