@@ -158,6 +158,59 @@ __device__ __forceinline__ void half_schedule() {
   }
 }
 
+// 64 x 64 tiles: a wavefront has one block, so a k block is three matrix instructions at most, less than an LDS read takes.  The
+// fragments of a whole stage are read while those of the one before are multiplied; who passes the barrier has all of its
+// stage in registers, so the buffer is filled again at once, and up to four stages are on their way.  Loads are made without
+// conditions, beyond the end of the last stage again (of any other order the compiler knows too little, and waits for all
+// loads before it reads LDS).
+template <class T>
+__device__ __forceinline__ void half_gemm_short(HalfAcc<T> &acc, char *buf0, char *buf1, char *buf2, char *buf3, char const *P, char const *Q,
+                                                size_t row_stride_p, size_t row_stride_q, int stages, int wm, int wn, int wave, int lane) {
+  char *const bufs[4] = {buf0, buf1, buf2, buf3};
+  auto const load = [&](char *buf, int t) {
+    t = t < stages ? t : stages - 1;
+    half_stage_load<T>(buf, P + static_cast<size_t>(t) * T::kStep, Q + static_cast<size_t>(t) * T::kStep, row_stride_p, row_stride_q, wave, lane);
+  };
+  HalfFrags<T> cur[T::KS], nxt[T::KS];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) load(bufs[u], u);
+  half_stage_wait<T, 3>();
+#pragma unroll
+  for (int ks = 0; ks < T::KS; ++ks) half_frags_read<T>(cur[ks], bufs[0], ks, wm, wn, lane);
+  auto const step = [&](char *free, char const *next, int t) {
+    half_stage_wait<T, 2>();
+    load(free, t + 4);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int ks = 0; ks < T::KS; ++ks) half_frags_read<T>(nxt[ks], next, ks, wm, wn, lane);
+#pragma unroll
+    for (int ks = 0; ks < T::KS; ++ks) half_mfma<T>(acc, cur[ks]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // (8 reads, 4 or 6 matrix instructions)
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int ks = 0; ks < T::KS; ++ks) cur[ks] = nxt[ks];
+  };
+  int t = 0;
+  for (; t + 4 <= stages; t += 4) {
+    step(buf0, buf1, t);
+    step(buf1, buf2, t + 1);
+    step(buf2, buf3, t + 2);
+    step(buf3, buf0, t + 3);
+  }
+  if (t < stages) {
+    step(buf0, buf1, t);
+    if (t + 1 < stages) {
+      step(buf1, buf2, t + 1);
+      if (t + 2 < stages) step(buf2, buf3, t + 2);
+    }
+  }
+  half_stage_wait<T, 0>();  // nothing may land in LDS that is no longer this workgroup's
+}
+
 // The K loop of one workgroup (256 threads, wavefronts 2 x 2) over `stages` >= 1 stages.  P, Q: the first fragment of the
 // tile's first row block at the first k block; row_stride_*: bytes from one row block to the next.
 template <class T>
@@ -174,6 +227,10 @@ __device__ __forceinline__ void half_gemm(HalfAcc<T> &acc, char const *P, char c
   for (int m = 0; m < T::kMB; ++m)
 #pragma unroll
     for (int n = 0; n < T::kNB; ++n) acc.v[m][n] = f32x16{};
+  if constexpr (T::kMB == 1) {
+    half_gemm_short<T>(acc, buf0, buf1, buf2, buf3, P, Q, row_stride_p, row_stride_q, stages, wm, wn, wave, lane);
+    return;
+  }
 
   auto const load = [&](char *buf, int t) {
     half_stage_load<T>(buf, P + static_cast<size_t>(t) * T::kStep, Q + static_cast<size_t>(t) * T::kStep, row_stride_p, row_stride_q, wave, lane);
