@@ -172,6 +172,13 @@ class Dlmi:
         assert t.device == self.device, "%s must be on %s, is on %s" % (what, self.device, t.device)
         assert t.is_contiguous(), "dlmi takes contiguous device tensors: " + what
 
+    def _chk_all(self, dtype, shape, **tensors):
+        """The same of several tensors alike."""
+        device = self.device
+        for what, t in tensors.items():
+            if t is not None and not (t.dtype is dtype and t.shape == shape and t.device == device and t.is_contiguous()):
+                self._chk_is(t, what, dtype, *shape)
+
     def _type(self, t):
         """dlmi_dtype of a tensor of `type`."""
         assert t.dtype in self._types, "float32 or bfloat16 tensors, not %s" % t.dtype
@@ -651,16 +658,14 @@ class Dlmi:
 
     def block_norm_fwd(self, desc, x, u, gate=None, w_post=None, b_post=None, w_pre=None, b_pre=None, y=None, h=None):
         """y = residual_scale x + branch_scale f(gate) post(u), h = pre(y) (dlmi_block_norm_fwd).  Returns (y, h)."""
-        B, H = u.shape
-        kind, dtype = self._type(u), u.dtype
+        shape, dtype, kind = u.shape, u.dtype, self._type(u)
+        B, H = shape
         y = y if y is not None else self._out_like(u)
         h = h if h is not None else self._out_like(u)
-        for t, what in ((u, "u"), (x, "x"), (y, "y"), (h, "h")):
-            self._chk_is(t, what, dtype, B, H)
+        self._chk_all(dtype, shape, u=u, x=x, y=y, h=h)
         if gate is not None and desc.gate_rows:
             self._chk_is(gate, "gate", dtype, -(-B // desc.gate_rows), H)
-        for t, what in ((w_post, "w_post"), (b_post, "b_post"), (w_pre, "w_pre"), (b_pre, "b_pre")):
-            self._chk_is(t, what, self.torch.float32, H)
+        self._chk_all(self.torch.float32, (H,), w_post=w_post, b_post=b_post, w_pre=w_pre, b_pre=b_pre)
         self._ck(self.lib.dlmi_block_norm_fwd(self.ctx, kind, ctypes.byref(desc), B, H, _a(x), _a(u), _a(gate), _a(w_post),
                                               _a(b_post), _a(w_pre), _a(b_pre), _a(y), _a(h)))
         return y, h
@@ -669,30 +674,23 @@ class Dlmi:
                        dgate=None, grads=None, accumulate=False):
         """Its gradient (dlmi_block_norm_bwd).  Returns dict(dx, du, dgate, dw_post, db_post, dw_pre, db_pre), None for what
         is not there; grads: a dict of fp32 tensors for the last four (needed to accumulate), made where missing."""
-        B, H = u.shape
-        kind, dtype = self._type(u), u.dtype
+        shape, dtype, kind = u.shape, u.dtype, self._type(u)
+        B, H = shape
         dx = dx if dx is not None else self._out_like(u)
         du = du if du is not None else self._out_like(u)
         dgate = dgate if dgate is not None or gate is None else self._out_like(gate)
-        o = dict(dx=dx, du=du, dgate=dgate)
-        params = dict(dw_post=w_post, db_post=b_post, dw_pre=w_pre, db_pre=b_pre)
-        given = grads or {}
-        missing = [k for k, p in params.items() if p is not None and given.get(k) is None]
+        dw_post, db_post, dw_pre, db_pre = grads = [(grads or {}).get(k) for k in ("dw_post", "db_post", "dw_pre", "db_pre")]
+        missing = [i for i, p in enumerate((w_post, b_post, w_pre, b_pre)) if p is not None and grads[i] is None]
         if missing:
             assert not accumulate, "accumulating needs the gradients so far"
-            made = dict(zip(missing, self._out(self.torch.float32, len(missing), H).unbind(0)))
-        for k, p in params.items():
-            o[k] = made[k] if k in missing else given.get(k)
-            self._chk_is(p, k[1:], self.torch.float32, H)
-            self._chk_is(o[k], k, self.torch.float32, H)
-        for t, what in ((u, "u"), (y, "y"), (dy, "dy"), (dh, "dh"), (dx, "dx"), (du, "du")):
-            self._chk_is(t, what, dtype, B, H)
+            for i, t in zip(missing, self._out(self.torch.float32, len(missing), H).unbind(0)):
+                grads[i] = t
+            dw_post, db_post, dw_pre, db_pre = grads
+        self._chk_all(self.torch.float32, (H,), w_post=w_post, b_post=b_post, w_pre=w_pre, b_pre=b_pre, dw_post=dw_post,
+                      db_post=db_post, dw_pre=dw_pre, db_pre=db_pre)
+        self._chk_all(dtype, shape, u=u, y=y, dy=dy, dh=dh, dx=dx, du=du)
         if gate is not None and desc.gate_rows:
-            rows = -(-B // desc.gate_rows)
-            self._chk_is(gate, "gate", dtype, rows, H)
-            self._chk_is(dgate, "dgate", dtype, rows, H)
-        self._ck(self.lib.dlmi_block_norm_bwd(
-            self.ctx, kind, ctypes.byref(desc), B, H, _a(u), _a(y), _a(gate), _a(w_post), _a(b_post), _a(w_pre), _a(dy), _a(dh),
-            _a(dx), _a(du), _a(dgate), _a(o["dw_post"]), _a(o["db_post"]), _a(o["dw_pre"]), _a(o["db_pre"]),
-            1 if accumulate else 0))
-        return o
+            self._chk_all(dtype, (-(-B // desc.gate_rows), H), gate=gate, dgate=dgate)
+        at = [None if t is None else t.data_ptr() for t in (u, y, gate, w_post, b_post, w_pre, dy, dh, dx, du, dgate, *grads)]
+        self._ck(self.lib.dlmi_block_norm_bwd(self.ctx, kind, ctypes.byref(desc), B, H, *at, 1 if accumulate else 0))
+        return dict(dx=dx, du=du, dgate=dgate, dw_post=dw_post, db_post=db_post, dw_pre=dw_pre, db_pre=db_pre)
