@@ -18,6 +18,7 @@
 // rounding for bf16, none without dloss).
 #pragma once
 
+#include <algorithm>
 #include <cmath>
 
 #include "half_gemm.hpp"
@@ -97,7 +98,7 @@ __device__ __forceinline__ float ce_largest(float const *v, unsigned n, int lane
 // The four wavefronts of a workgroup share the columns of 8 rows at a time, a lane 8 columns of one of them; up to KEEP
 // octets of a lane stay in registers between the search for the largest and the packing (wider rows are read twice).  An
 // octet is a piece of a fragment as it stands; for the transposed ones the wavefront turns 8 x 64 values through 2 KiB of
-// LDS that only it uses.
+// LDS that only it uses.  ALONE: rows of up to 64 KEEP columns, a wavefront takes 8 of its own, all their columns.
 constexpr unsigned kCePackBlocks = 1024;
 
 // (All null in the forward pass.)
@@ -107,7 +108,7 @@ struct CeMost {
   unsigned nparts, piece, pieces;
 };
 
-template <class T, int NP, int KEEP, bool LABELS>
+template <class T, int NP, int KEEP, bool LABELS, bool ALONE>
 __global__ __launch_bounds__(kCeBlock) void k_ce_pack(CeArgs a, T const *src, size_t rows, size_t padded, size_t cols, unsigned kblocks_as,
                                                       unsigned kblocks_across, float *unscale, float *unscale_across, CeMost most, char *as, char *across) {
   __shared__ float turn[4][8][68];
@@ -115,10 +116,12 @@ __global__ __launch_bounds__(kCeBlock) void k_ce_pack(CeArgs a, T const *src, si
   int const lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int const r8 = lane >> 3, c8 = (lane & 7) * 8;
   unsigned const tiles = kblocks_as / 4;  // of 64 columns, padding included
-  bool const narrow = cols < 8, kept = (tiles + 3) / 4 <= KEEP;
+  unsigned const step = ALONE ? 1 : 4, first = ALONE ? 0 : wave;  // of a wavefront's tiles
+  bool const narrow = cols < 8, kept = ALONE || (tiles + 3) / 4 <= KEEP;
   float mine = 0.0f;
   int flip = 0;
-  for (size_t r0 = static_cast<size_t>(blockIdx.x) * 8; r0 < padded; r0 += static_cast<size_t>(gridDim.x) * 8) {
+  size_t const at = ALONE ? static_cast<size_t>(blockIdx.x) * 4 + wave : blockIdx.x, stride = static_cast<size_t>(gridDim.x) * (ALONE ? 4 : 1);
+  for (size_t r0 = at * 8; r0 < padded; r0 += stride * 8) {
     size_t const r = r0 + r8;
     T const *const row = src + (r < rows ? r : rows - 1) * cols;
     // every load is made, whole (one that hangs over the row's end is moved back to end with it)
@@ -132,7 +135,7 @@ __global__ __launch_bounds__(kCeBlock) void k_ce_pack(CeArgs a, T const *src, si
       for (size_t c = 0; c < cols; ++c) m = ce_finite_max(m, static_cast<float>(row[c]));
     } else if (kept) {
 #pragma unroll
-      for (int k = 0; k < KEEP; ++k) keep[k] = load(wave + 4 * k < tiles ? wave + 4 * k : 0);
+      for (int k = 0; k < KEEP; ++k) keep[k] = load(first + step * k < tiles ? first + step * k : 0);
 #pragma unroll
       for (int k = 0; k < KEEP; ++k)
 #pragma unroll
@@ -147,22 +150,24 @@ __global__ __launch_bounds__(kCeBlock) void k_ce_pack(CeArgs a, T const *src, si
     }
 #pragma unroll
     for (int o = 1; o < 8; o *= 2) m = fmaxf(m, __shfl_xor(m, o));
-    if ((lane & 7) == 0) top[flip][wave][r8] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(top[flip][0][r8], top[flip][1][r8]), fmaxf(top[flip][2][r8], top[flip][3][r8]));
-    flip ^= 1;
+    if constexpr (!ALONE) {
+      if ((lane & 7) == 0) top[flip][wave][r8] = m;
+      __syncthreads();
+      m = fmaxf(fmaxf(top[flip][0][r8], top[flip][1][r8]), fmaxf(top[flip][2][r8], top[flip][3][r8]));
+      flip ^= 1;
+    }
     float const scale = ce_scale(m);
     // across = as * ratio, ratio = weight * scale_across / scale
     // (a row of zeros has no share in a product, so none in the largest either)
     float ratio = r < rows ? 1.0f : 0.0f, un = m > 0.0f ? ce_unscale(scale) : 0.0f;
-    if ((lane & 7) == 0 && wave == 0) unscale[r] = un;
+    if ((lane & 7) == 0 && (ALONE || wave == 0)) unscale[r] = un;
     if constexpr (LABELS) {
       int const l = r < rows ? a.labels[r] : -1;
       float const w = l >= 0 && static_cast<size_t>(l) < a.V ? ce_row_weight(a, r) : 0.0f;
       float const s2 = ce_scale(fabsf(w) * m);
       ratio = l >= 0 && static_cast<size_t>(l) < a.V ? w * (s2 * ce_unscale(scale)) : 0.0f;
       un = fabsf(w) * m > 0.0f ? ce_unscale(s2) : 0.0f;
-      if ((lane & 7) == 0 && wave == 0) unscale_across[r] = un;
+      if ((lane & 7) == 0 && (ALONE || wave == 0)) unscale_across[r] = un;
     }
     mine = fmaxf(mine, r < rows ? un : 0.0f);
     auto const pack = [&](float const (&v)[8], char *dst) {
@@ -213,14 +218,19 @@ __global__ __launch_bounds__(kCeBlock) void k_ce_pack(CeArgs a, T const *src, si
     if (kept) {
 #pragma unroll
       for (int k = 0; k < KEEP; ++k)
-        if (wave + 4 * k < tiles) tile(wave + 4 * k, keep[k]);
+        if (first + step * k < tiles) tile(first + step * k, keep[k]);
     } else {
 #pragma unroll 2
       for (unsigned t = wave; t < tiles; t += 4) tile(t, narrow ? CeOct<T>{} : load(t));
     }
   }
   if (most.w == nullptr) return;
-  mine = ce_wave_max(mine);  // (the wavefronts have seen the same rows)
+  mine = ce_wave_max(mine);
+  if constexpr (ALONE) {  // (otherwise the wavefronts have seen the same rows)
+    if (lane == 0) top[0][wave][0] = mine;
+    __syncthreads();
+    mine = fmaxf(fmaxf(top[0][0][0], top[0][1][0]), fmaxf(top[0][2][0], top[0][3][0]));
+  }
   if constexpr (LABELS) {
     if (threadIdx.x == 0) most.parts[blockIdx.x] = mine;
     if (blockIdx.x == 0)
@@ -341,25 +351,40 @@ __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_stats(CeArgs a, Ce
   }
 }
 
-// 64 rows of the batch per workgroup: 16 threads each join every 16th partial, then one another's, in a fixed order.
-template <int kParts>
-__global__ __launch_bounds__(64 * kParts) void k_ce_join(CeArgs a, float2 const *part, size_t part_stride, size_t parts, float const *target) {
-  __shared__ float2 lds[kParts][64];
-  size_t const b = static_cast<size_t>(blockIdx.x) * 64 + (threadIdx.x & 63);
-  int const w = threadIdx.x >> 6;
-  float m = -INFINITY, s = 0.0f;
+// kRows rows of the batch per workgroup: 1024 / kRows threads each join every so manieth partial, eight of them on their way
+// at a time, then one another's, in a fixed order.
+template <int kRows>
+__global__ __launch_bounds__(1024) void k_ce_join(CeArgs a, float2 const *part, size_t part_stride, size_t parts, float const *target) {
+  constexpr int kParts = 1024 / kRows;
+  __shared__ float2 lds[kParts][kRows];
+  size_t const b = static_cast<size_t>(blockIdx.x) * kRows + threadIdx.x % kRows, in = b < a.B ? b : a.B - 1;
+  int const w = threadIdx.x / kRows;
+  float2 s = make_float2(-INFINITY, 0.0f);
   auto const join = [&](float2 p) {
-    float const most = fmaxf(m, p.x);
-    s = s * ce_join_factor(m, most) + p.y * ce_join_factor(p.x, most);
-    m = most;
+    float const most = fmaxf(s.x, p.x);
+    s.y = s.y * ce_join_factor(s.x, most) + p.y * ce_join_factor(p.x, most);
+    s.x = most;
   };
-  if (b < a.B)
-    for (size_t p = w; p < parts; p += kParts) join(part[p * part_stride + b]);
-  lds[w][threadIdx.x & 63] = make_float2(m, s);
+  size_t p = w;
+  for (; p + 7 * kParts < parts; p += 8 * kParts) {
+    float2 v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = part[(p + i * kParts) * part_stride + in];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) join(v[i]);
+  }
+  for (; p < parts; p += kParts) join(part[p * part_stride + in]);
+  lds[w][threadIdx.x % kRows] = s;
   __syncthreads();
+  for (int o = kParts / 2; o > 0; o >>= 1) {
+    if (w < o) {
+      join(lds[w + o][threadIdx.x % kRows]);
+      lds[w][threadIdx.x % kRows] = s;
+    }
+    __syncthreads();
+  }
   if (w != 0 || b >= a.B) return;
-  for (int o = 1; o < kParts; ++o) join(lds[o][threadIdx.x & 63]);
-  float const lse = m + logf(s);
+  float const lse = s.x + logf(s.y);
   a.lse[b] = lse;
   int const l = a.labels[b];
   a.loss[b] = l >= 0 && static_cast<size_t>(l) < a.V ? lse - target[b] : 0.0f;
@@ -389,19 +414,36 @@ __device__ __forceinline__ CeLine ce_line(E const *p) {
   for (int t = 0; t < 4; ++t) r.q[t] = reinterpret_cast<CePiece<E> const *>(p + t * (G * 16 / static_cast<int>(sizeof(E))))->q;
   return r;
 }
-// The same where the row ends at K; what lies beyond counts as zero.
+// The same where the row ends at K; what lies beyond counts as zero.  Of bf16 rows a piece over the end is loaded from where it
+// ends with the row and shifted down (16 loads of 2 bytes instead: 22.4 us, not 19.8, for [16 x 1020] against 21246 classes);
+// of fp32 rows the values are loaded one by one (shifted: 57 us, not 50, for [55 x 101] against 114534).
 template <class E, int G>
-__device__ CeLine ce_line_tail(E const *row, size_t k, size_t K) {
+__device__ __forceinline__ CeLine ce_line_tail(E const *row, size_t k, size_t K) {
   constexpr int N = 16 / sizeof(E);
-  union {
-    E e[4 * N];
-    CeLine l;
-  } u;
+  if (sizeof(E) == 4 || K < N) {
+    union {
+      E e[4 * N];
+      CeLine l;
+    } u;
 #pragma unroll
-  for (int t = 0; t < 4; ++t)
+    for (int t = 0; t < 4; ++t)
 #pragma unroll
-    for (int i = 0; i < N; ++i) u.e[t * N + i] = k + t * G * N + i < K ? row[k + t * G * N + i] : static_cast<E>(0.0f);
-  return u.l;
+      for (int i = 0; i < N; ++i) u.e[t * N + i] = k + t * G * N + i < K ? row[k + t * G * N + i] : static_cast<E>(0.0f);
+    return u.l;
+  }
+  CeLine r;
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    size_t const at = k + t * G * N, from = at + N <= K ? at : K - N;
+    r.q[t] = reinterpret_cast<CePiece<E> const *>(row + from)->q;
+  }
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    size_t const at = k + t * G * N, over = at + N <= K ? 0 : at + N - K;
+    unsigned __int128 const v = __builtin_bit_cast(unsigned __int128, r.q[t]);
+    r.q[t] = __builtin_bit_cast(u32x4, over < N ? v >> (static_cast<unsigned>(over) * 8 * static_cast<unsigned>(sizeof(E))) : 0);
+  }
+  return r;
 }
 
 // Blocks of RB classes x RB rows of the batch: RB = 32 or, for up to 16 rows of the batch, 16 (fp32 products of 32 columns
@@ -860,7 +902,7 @@ __global__ __launch_bounds__(kCeBlock) void k_ce_dx_finish(CeArgs a, float const
 
 // ---- host ------------------------------------------------------------------------------------------------------------
 struct CePlan {
-  int T;
+  int T, Tw;                       // tile; of dW (not larger)
   size_t Bp, Kp, Vc, pieces;       // padded rows and features; classes of a piece (a multiple of T)
   unsigned slices, per_slice;      // of dX
   unsigned pack_x, pack_w;         // packing workgroups
@@ -868,19 +910,29 @@ struct CePlan {
   size_t xp, xt, wp, wt, dlb, dlv, parts_x, unscale_x, unscale_xw, unscale_w, most_x, most_w, part, target, dxacc, dbpart, bytes;
 };
 
+// Packing workgroups for n (padded) rows: of 8 rows each, or of 32 narrow ones.
+static unsigned pack_blocks(size_t n, size_t Kp) {
+  size_t const b = Kp <= 256 ? n / 32 : n / 8;
+  return static_cast<unsigned>(b < kCePackBlocks ? b : kCePackBlocks);
+}
+
 template <int NP>
 CePlan ce_plan(dlmi_ctx const *ctx, size_t B, size_t K, size_t V, bool back) {
   CePlan p = {};
-  // The tile with the least estimated time of all products: rounds of tiles over the CUs, the depth of their K loops, and what
-  // an element of a tile costs (measured relative rates; 128 x 128 tiles run two to a CU).  dX is cut into slices, so only
-  // its size counts.
+  // The tile with the least estimated time of all products: rounds of tiles over the CUs, the depth of their K loops, what 16 k
+  // of a tile cost (measured, in us of two planes, of one plane a share of it; 128 and 64 wide tiles run two to a CU, where a CU
+  // has one alone it is done sooner; many 64 wide ones wait for the L2) and its prologue and epilogue.  dX is cut into slices, so only its size counts; dW's tile is its own.
+  double const cu = ctx->num_cu;
+  auto const product = [&](int t, double tiles, size_t k) {
+    double const each = t == 256 ? 1.25 : t == 128 ? 0.35 : tiles <= 3 * cu ? 0.1 : 0.16, alone = t == 256 ? 1.25 : t == 128 ? 0.27 : 0.085, ends = t == 256 ? 12.0 : t == 128 ? 3.0 : 1.5;
+    double const rounds = tiles / cu < 4.0 ? std::ceil(tiles / cu) : tiles / cu, depth = static_cast<double>(dlmi_ceil_div(k, 64) * 4);
+    return rounds * ((tiles <= cu ? alone : each) * depth * (NP == 2 ? 1.0 : t == 256 ? 0.33 : 0.4) + ends);
+  };
+  auto const tiles_of = [](int t, size_t x, size_t y) { return static_cast<double>(dlmi_ceil_div(x, t)) * static_cast<double>(dlmi_ceil_div(y, t)); };
   double least = 0.0;
   for (int t : {256, 128, 64}) {
-    double const cu = ctx->num_cu, cost = t == 256 ? 1.0 : t == 128 ? 1.25 : 2.5, d = t, b = dlmi_ceil_div(B, t), k = dlmi_ceil_div(K, t),
-                 v = dlmi_ceil_div(V, t);
-    auto const rounds = [&](double tiles) { return tiles <= cu ? 1.0 : tiles / cu < 4.0 ? std::ceil(tiles / cu) : tiles / cu; };
-    double time = rounds(b * v) * d * d * cost * static_cast<double>(dlmi_ceil_div(K, 64) * 64);
-    if (back) time += rounds(v * k) * d * d * cost * static_cast<double>(dlmi_ceil_div(B, 64) * 64) + b * k * v * d * d * d * cost / cu;
+    double time = product(t, tiles_of(t, B, V), K);
+    if (back) time += product(t, std::max(tiles_of(t, B, K), cu * (t == 256 ? 1 : 2)), static_cast<size_t>(static_cast<double>(V) * std::min(1.0, tiles_of(t, B, K) / (cu * (t == 256 ? 1 : 2)))));
     if (t == 256 || time < least) {
       least = time;
       p.T = t;
@@ -890,9 +942,9 @@ CePlan ce_plan(dlmi_ctx const *ctx, size_t B, size_t K, size_t V, bool back) {
   auto const up = [](size_t x, size_t m) { return dlmi_ceil_div(x, m) * m; };
   p.Bp = up(B, T);
   p.Kp = back ? up(K, T) : up(K, 64);
-  // a piece: about four rounds of tiles, at most 1 GiB of packed operands
+  // a piece: about four rounds of 256 wide tiles, eight of smaller ones, at most 1 GiB of packed operands
   size_t const nj = p.Bp / T;
-  size_t tiles = dlmi_ceil_div(static_cast<size_t>(ctx->num_cu) * 4, nj);
+  size_t tiles = dlmi_ceil_div(static_cast<size_t>(ctx->num_cu) * (T == 256 ? 4 : 8), nj);
   size_t const row_bytes = 2 * NP * (back ? 2 * (p.Kp + p.Bp) : p.Kp);
   size_t const fit = (size_t(1) << 30) / (row_bytes * T);
   if (tiles > fit) tiles = fit > 0 ? fit : 1;
@@ -900,6 +952,14 @@ CePlan ce_plan(dlmi_ctx const *ctx, size_t B, size_t K, size_t V, bool back) {
   p.pieces = dlmi_ceil_div(all, tiles);
   p.Vc = dlmi_ceil_div(all, p.pieces) * T;
   p.pieces = dlmi_ceil_div(V, p.Vc);
+  for (int t : {256, 128, 64}) {
+    if (t > p.T) continue;
+    double const time = product(t, tiles_of(t, p.Vc, K), B);
+    if (t == p.T || time < least) {
+      least = time;
+      p.Tw = t;
+    }
+  }
   size_t at = 0;
   auto const take = [&](size_t bytes) {
     size_t const o = at;
@@ -908,9 +968,8 @@ CePlan ce_plan(dlmi_ctx const *ctx, size_t B, size_t K, size_t V, bool back) {
   };
   p.xp = take(packed_bytes(p.Bp, p.Kp, NP));
   p.wp = take(packed_bytes(p.Vc, p.Kp, NP));
-  auto const blocks_of = [](size_t n) { return static_cast<unsigned>(n / 8 < kCePackBlocks ? n / 8 : kCePackBlocks); };
-  p.pack_x = blocks_of(p.Bp);
-  p.pack_w = blocks_of(p.Vc);
+  p.pack_x = pack_blocks(p.Bp, p.Kp);
+  p.pack_w = pack_blocks(p.Vc, p.Kp);
   p.unscale_x = take(p.Bp * sizeof(float));
   p.unscale_xw = take(p.Bp * sizeof(float));
   p.unscale_w = take(p.Vc * sizeof(float));
@@ -950,11 +1009,11 @@ struct CeRun {
   static unsigned ce_stages(int T, size_t k) { return static_cast<unsigned>(dlmi_ceil_div(k, (T == 64 ? 64 : 32) / NP)); }
   float *floats(size_t at) const { return reinterpret_cast<float *>(s + at); }
 
-  template <int KEEP, bool LABELS>
+  template <int KEEP, bool LABELS, bool ALONE>
   int pack(E const *src, size_t rows, size_t padded, unsigned blocks, size_t unscale, size_t piece, bool back, char *as, char *across) const {
     CeMost most = {};
     if (back) most = {floats(p.most_w), floats(p.most_x), floats(p.parts_x), p.pack_x, static_cast<unsigned>(piece), static_cast<unsigned>(p.pieces)};
-    hipLaunchKernelGGL((k_ce_pack<E, NP, KEEP, LABELS>), dim3(blocks), dim3(kCeBlock), 0, ctx->stream, a, src, rows, padded, a.K,
+    hipLaunchKernelGGL((k_ce_pack<E, NP, KEEP, LABELS, ALONE>), dim3(blocks), dim3(kCeBlock), 0, ctx->stream, a, src, rows, padded, a.K,
                        static_cast<unsigned>(p.Kp / 16), static_cast<unsigned>(padded / 16), floats(unscale), floats(p.unscale_xw),
                        most, as, across);
     DLMI_LAUNCH_CHECK(ctx, "k_ce_pack");
@@ -963,15 +1022,17 @@ struct CeRun {
   int pack_rows(bool back) const {
     E const *const x = static_cast<E const *>(a.X);
     char *const across = back && a.dW != nullptr ? s + p.xt : nullptr;
-    if (p.Kp <= 1024) return pack<4, true>(x, a.B, p.Bp, p.pack_x, p.unscale_x, 0, back, s + p.xp, across);
-    return pack<8, true>(x, a.B, p.Bp, p.pack_x, p.unscale_x, 0, back, s + p.xp, across);
+    if (p.Kp <= 256) return pack<4, true, true>(x, a.B, p.Bp, p.pack_x, p.unscale_x, 0, back, s + p.xp, across);
+    if (p.Kp <= 1024) return pack<4, true, false>(x, a.B, p.Bp, p.pack_x, p.unscale_x, 0, back, s + p.xp, across);
+    return pack<8, true, false>(x, a.B, p.Bp, p.pack_x, p.unscale_x, 0, back, s + p.xp, across);
   }
-  unsigned pack_w(size_t vp) const { return vp / 8 < p.pack_w ? static_cast<unsigned>(vp / 8) : p.pack_w; }
+  unsigned pack_w(size_t vp) const { return pack_blocks(vp, p.Kp) < p.pack_w ? pack_blocks(vp, p.Kp) : p.pack_w; }
   int pack_classes(size_t v0, size_t vn, size_t vp, bool back) const {
     E const *const w = static_cast<E const *>(a.W) + v0 * a.K;
     char *const across = back && a.dX != nullptr ? s + p.wt : nullptr;
-    if (p.Kp <= 1024) return pack<4, false>(w, vn, vp, pack_w(vp), p.unscale_w, v0 / p.Vc, back, s + p.wp, across);
-    return pack<8, false>(w, vn, vp, pack_w(vp), p.unscale_w, v0 / p.Vc, back, s + p.wp, across);
+    if (p.Kp <= 256) return pack<4, false, true>(w, vn, vp, pack_w(vp), p.unscale_w, v0 / p.Vc, back, s + p.wp, across);
+    if (p.Kp <= 1024) return pack<4, false, false>(w, vn, vp, pack_w(vp), p.unscale_w, v0 / p.Vc, back, s + p.wp, across);
+    return pack<8, false, false>(w, vn, vp, pack_w(vp), p.unscale_w, v0 / p.Vc, back, s + p.wp, across);
   }
   CeLogits logits(size_t v0, size_t vn, size_t vp) const {
     CeLogits g = {};
@@ -1004,9 +1065,19 @@ struct CeRun {
       DLMI_LAUNCH_CHECK(ctx, "k_ce_stats");
     }
     if (rc != DLMI_OK) return rc;
-    hipLaunchKernelGGL(k_ce_join<16>, dim3(static_cast<unsigned>(dlmi_ceil_div(a.B, 64))), dim3(1024), 0, ctx->stream, a,
+    hipLaunchKernelGGL(k_ce_join<16>, dim3(static_cast<unsigned>(dlmi_ceil_div(a.B, 16))), dim3(1024), 0, ctx->stream, a,
                        reinterpret_cast<float2 *>(s + p.part), p.Bp, dlmi_ceil_div(a.V, static_cast<size_t>(T)) * 2, floats(p.target));
     DLMI_LAUNCH_CHECK(ctx, "k_ce_join");
+    return DLMI_OK;
+  }
+
+  // dW of a piece (tiles that are padding alone have no workgroup)
+  template <int T>
+  int weights(CeLogits const &g, size_t v0, size_t vn, unsigned kb) const {
+    unsigned const ni = static_cast<unsigned>(dlmi_ceil_div(vn, T)), nk = static_cast<unsigned>(dlmi_ceil_div(a.K, T));
+    hipLaunchKernelGGL((k_ce_dw<T, NP, E>), dim3(ni * nk), dim3(256), 0, ctx->stream, s + p.dlv, s + p.xt, ni, nk, kb, ce_stages(T, a.B), g.most_x,
+                       a.scale, static_cast<E *>(a.dW) + v0 * a.K, vn, a.K, a.accumulate);
+    DLMI_LAUNCH_CHECK(ctx, "k_ce_dw");
     return DLMI_OK;
   }
 
@@ -1038,10 +1109,12 @@ struct CeRun {
         DLMI_LAUNCH_CHECK(ctx, "k_ce_dx");
       }
       if (a.dW != nullptr) {
-        hipLaunchKernelGGL((k_ce_dw<T, NP, E>), dim3(g.ni * nk), dim3(256), 0, ctx->stream, s + p.dlv, s + p.xt, g.ni, nk, kb,
-                           ce_stages(T, a.B), g.most_x, a.scale, static_cast<E *>(a.dW) + v0 * a.K, vn, a.K,
-                           a.accumulate);
-        DLMI_LAUNCH_CHECK(ctx, "k_ce_dw");
+        if (p.Tw == T)
+          rc = weights<T>(g, v0, vn, kb);
+        else if (p.Tw == 128)
+          rc = weights<128>(g, v0, vn, kb);
+        else
+          rc = weights<64>(g, v0, vn, kb);
       }
     }
     if (rc != DLMI_OK || a.dX == nullptr) return rc;
