@@ -384,6 +384,9 @@ struct MuonPlan {
   size_t bytes(size_t count) const { return per_matrix * count + parts; }
 };
 
+// Stages of a K loop that are worth sharing by the whole device.
+static double muon_long_loop(int tile) { return tile == 128 ? 50.0 : 80.0; }
+
 static MuonPlan muon_plan(dlmi_ctx const *ctx, size_t rows, size_t cols, size_t count) {
   MuonPlan pl;
   pl.flipped = rows > cols;
@@ -403,17 +406,22 @@ static MuonPlan muon_plan(dlmi_ctx const *ctx, size_t rows, size_t cols, size_t 
   pl.nparts = static_cast<unsigned>(dlmi_ceil_div(rows * cols, kMuonBlock * 8));
   if (pl.nparts > 256) pl.nparts = 256;
   pl.per_matrix = 3 * pl.bytes_x + 2 * pl.bytes_a + dlmi_ceil_div(pl.nparts * sizeof(double), 1024) * 1024;
-  // a workgroup of 256 x 256 tiles per CU; their last tiles may be shared out, two parts a workgroup
+  // a workgroup per CU for tiles that are shared out, two parts each
   pl.workgroups = static_cast<unsigned>(ctx->num_cu);
-  pl.parts = pl.tile == 256 ? static_cast<size_t>(pl.workgroups) * 2 * 256 * 256 * sizeof(float) : 0;
+  bool const may = pl.tile == 256 || static_cast<double>(pl.np / (pl.tile == 128 ? 16 : 32)) > muon_long_loop(pl.tile);
+  pl.parts = may ? static_cast<size_t>(pl.workgroups) * 2 * pl.tile * pl.tile * sizeof(float) : 0;
   return pl;
 }
 
-// Whether sharing out the last tiles pays: a round of 256 x 256 tiles that is at most three quarters full is worth the
-// two launches and the parts' way through memory; smaller tiles leave less idle than that costs.
+// Whether sharing out the last tiles pays for the second launch and the parts' way through memory.  256 x 256 tiles: where
+// their round is at most three quarters full.  Smaller ones: where they are too few for the device and their K loops long,
+// which a CU walks at what it takes from the L2, about 0.27 us a stage of 128 x 128 and 0.17 of 64 x 64 (eleven matrices of
+// 112 x 3141: 386 -> 282 us a step; 1531 x 517, whose loops have 48 stages, would go from 146 to 156: a launch and the parts
+// cost as much as 13 us of a loop).
 static HalfShares muon_shares(MuonPlan const &pl, unsigned tiles, unsigned stages, float *parts) {
   unsigned const over = tiles % pl.workgroups;
-  bool const share = pl.tile == 256 && over != 0 && over * 4 <= pl.workgroups * 3;
+  bool share = over != 0 && over * 4 <= pl.workgroups * 3;
+  if (pl.tile != 256) share = tiles < pl.workgroups && stages * (1.0 - static_cast<double>(tiles) / pl.workgroups) > muon_long_loop(pl.tile);
   return half_shares(tiles, stages, share ? pl.workgroups : tiles, parts);
 }
 
@@ -423,14 +431,12 @@ static int muon_symmetric(dlmi_ctx *ctx, MuonSymmetric const &a, HalfShares cons
     hipLaunchKernelGGL((k_muon_symmetric<T, NP, POLY>), dim3(shares.whole), dim3(256), 0, ctx->stream, a, shares.stages);
     DLMI_LAUNCH_CHECK(ctx, "k_muon_symmetric");
   }
-  if constexpr (T == 256) {
-    if (shares.total == 0) return DLMI_OK;
-    hipLaunchKernelGGL((k_muon_symmetric_parts<T, NP>), dim3(shares.grid), dim3(256), 0, ctx->stream, a, shares);
-    DLMI_LAUNCH_CHECK(ctx, "k_muon_symmetric_parts");
-    unsigned const blocks = (shares.tiles - shares.whole) * (T / 32) * (T / 32) / 4;
-    hipLaunchKernelGGL((k_muon_symmetric_join<T, NP, POLY>), dim3(blocks), dim3(256), 0, ctx->stream, a, shares);
-    DLMI_LAUNCH_CHECK(ctx, "k_muon_symmetric_join");
-  }
+  if (shares.total == 0) return DLMI_OK;
+  hipLaunchKernelGGL((k_muon_symmetric_parts<T, NP>), dim3(shares.grid), dim3(256), 0, ctx->stream, a, shares);
+  DLMI_LAUNCH_CHECK(ctx, "k_muon_symmetric_parts");
+  unsigned const blocks = (shares.tiles - shares.whole) * (T / 32) * (T / 32) / 4;
+  hipLaunchKernelGGL((k_muon_symmetric_join<T, NP, POLY>), dim3(blocks), dim3(256), 0, ctx->stream, a, shares);
+  DLMI_LAUNCH_CHECK(ctx, "k_muon_symmetric_join");
   return DLMI_OK;
 }
 
@@ -440,14 +446,12 @@ static int muon_update(dlmi_ctx *ctx, MuonUpdate const &a, MuonBatch const &b, H
     hipLaunchKernelGGL((k_muon_update<T, NP, MODE, O>), dim3(shares.whole), dim3(256), 0, ctx->stream, a, b, shares.stages);
     DLMI_LAUNCH_CHECK(ctx, "k_muon_update");
   }
-  if constexpr (T == 256) {
-    if (shares.total == 0) return DLMI_OK;
-    hipLaunchKernelGGL((k_muon_update_parts<T, NP>), dim3(shares.grid), dim3(256), 0, ctx->stream, a, shares);
-    DLMI_LAUNCH_CHECK(ctx, "k_muon_update_parts");
-    unsigned const blocks = (shares.tiles - shares.whole) * (T / 32) * (T / 32) / 4;
-    hipLaunchKernelGGL((k_muon_update_join<T, NP, MODE, O>), dim3(blocks), dim3(256), 0, ctx->stream, a, b, shares);
-    DLMI_LAUNCH_CHECK(ctx, "k_muon_update_join");
-  }
+  if (shares.total == 0) return DLMI_OK;
+  hipLaunchKernelGGL((k_muon_update_parts<T, NP>), dim3(shares.grid), dim3(256), 0, ctx->stream, a, shares);
+  DLMI_LAUNCH_CHECK(ctx, "k_muon_update_parts");
+  unsigned const blocks = (shares.tiles - shares.whole) * (T / 32) * (T / 32) / 4;
+  hipLaunchKernelGGL((k_muon_update_join<T, NP, MODE, O>), dim3(blocks), dim3(256), 0, ctx->stream, a, b, shares);
+  DLMI_LAUNCH_CHECK(ctx, "k_muon_update_join");
   return DLMI_OK;
 }
 
