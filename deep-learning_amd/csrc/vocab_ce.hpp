@@ -774,6 +774,8 @@ __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_grad(CeArgs a, CeL
       for (int r = 0; r < 16; ++r) {
         int const c = m * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
         float p = __expf(z[r] * ux[n] * uw[r] + bias[r] - lse[n]);
+        // (the forward may have rounded z otherwise: beyond some 10^5 that is more than 1, and e^1 times 2^15 overflows f16; a NaN stays)
+        p = p > 1.0f ? 1.0f : p;
         p -= at[n] == c ? 1.0f : 0.0f;
         // (a class beyond the piece: its logit is -infinity, but a row's lse may be too)
         z[r] = live[n] && (whole || c0 + c < g.vn) ? p : 0.0f;

@@ -322,6 +322,8 @@ int dlmi_vocab_ce_fwd(dlmi_ctx *ctx, dlmi_dtype type, size_t B, size_t K, size_t
 
 /* Its gradient.  g[b] = scale * dloss[b] (dloss NULL: scale), 0 for rows left out; lse from the forward.
  *   dL[b,v] = exp(z[b,v] - lse[b]) - [v == labels[b]];  dX = g dL W;  dW (+)= (g dL)^T X;  db (+)= sum_b g[b] dL[b,.]
+ * exp(z - lse) is taken as at most 1: a logit is formed here to about 2^-22 of the terms it sums, not in the forward's order, and
+ * beyond some 10^5 the two may differ by more than 1 (a gradient of such a row is as exact as that, and finite).
  * dX [B, K], dW [V, K] of `type`, db [V] fp32; each may be NULL.  dX is written (zero in rows left out); accumulate != 0
  * adds into dW and db.  B, K and V must not be 0; a gradient must not overlap another array.  The logits are formed again,
  * piece by piece.  All sums are taken in an order that depends on the sizes only.
