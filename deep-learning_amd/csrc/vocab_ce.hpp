@@ -16,7 +16,9 @@
 // values take two planes.  dL is in [-1, 1] and held times 2^15, rounded to 11 bits (bf16; the result keeps 8) or 22 (fp32).
 // Where a product's sum runs over rows that are scaled differently (dX over W's, dW over X's), dL carries what undoes the
 // scale, as a share of the largest such factor, which multiplies the result.  For dW X is packed times dloss (one more
-// rounding for bf16, none without dloss).
+// rounding for bf16, none without dloss).  Factors more than 2^16 apart would leave no bits to the small ones (a padding row of
+// W that was never set, one row of the batch with a huge dloss): a piece where they are, which the device finds out by itself,
+// keeps dL in fp32 where its planes would lie and multiplies it with the operands as they are on the fp32 matrix pipe.
 #pragma once
 
 #include <algorithm>
@@ -90,12 +92,17 @@ __device__ __forceinline__ float ce_largest(float const *v, unsigned n, int lane
   return ce_wave_max(m);
 }
 
+// Whether factors that undo scales lie far apart: the largest of them times the largest scale (the smallest factor's inverse).
+// Up to here a row's terms keep an absolute error of 2^-40 of the largest factor's, 2^-24 of their own factor's.
+__device__ __forceinline__ bool ce_apart(float const *most, float const *finest) { return most[0] * finest[0] > 65536.0f; }
+
 // Rows of src [rows, cols], each scaled by its own largest magnitude and packed as it stands (`as`: row r, k = c) and / or
 // transposed (`across`: row c, k = r), padding zero.  unscale[r]: the inverse scale of `as`, unscale_across[r] that of
 // `across` (padding rows have entries too).  LABELS (X): `across` holds the row times ce_row_weight, scaled by its own
-// largest, and zeros in rows left out; otherwise (W) the two are the same.  The largest unscale_across of a piece of W goes to
-// most.w[piece] by an integer maximum in memory (positive floats order like integers, and no order changes a maximum), which
-// packing X has cleared; X's are left per workgroup and joined by the first workgroup that packs W.
+// largest, and zeros in rows left out; otherwise (W) the two are the same.  The largest unscale_across of a piece of W and its
+// largest scale go to most.w[piece] and most.w[pieces + piece] by an integer maximum in memory (positive floats order like
+// integers, and no order changes a maximum), which packing X has cleared; X's are left per workgroup and joined by the first
+// workgroup that packs W.
 // The four wavefronts of a workgroup share the columns of 8 rows at a time, a lane 8 columns of one of them; up to KEEP
 // octets of a lane stay in registers between the search for the largest and the packing (wider rows are read twice).  An
 // octet is a piece of a fragment as it stands; for the transposed ones the wavefront turns 8 x 64 values through 2 KiB of
@@ -105,8 +112,8 @@ constexpr unsigned kCePackBlocks = 1024;
 
 // (All null in the forward pass.)
 struct CeMost {
-  float *w;          // of each piece
-  float *x, *parts;  // of X; of its packing workgroups
+  float *w;          // of each piece: the largest factors, then the largest scales
+  float *x, *parts;  // the same two of X; of its packing workgroups
   unsigned nparts, piece, pieces;
 };
 
@@ -120,7 +127,7 @@ __global__ __launch_bounds__(kCeBlock) void k_ce_pack(CeArgs a, T const *src, si
   unsigned const tiles = kblocks_as / 4;  // of 64 columns, padding included
   unsigned const step = ALONE ? 1 : 4, first = ALONE ? 0 : wave;  // of a wavefront's tiles
   bool const narrow = cols < 8, kept = ALONE || (tiles + 3) / 4 <= KEEP;
-  float mine = 0.0f;
+  float mine = 0.0f, finest = 0.0f;
   int flip = 0;
   size_t const at = ALONE ? static_cast<size_t>(blockIdx.x) * 4 + wave : blockIdx.x, stride = static_cast<size_t>(gridDim.x) * (ALONE ? 4 : 1);
   for (size_t r0 = at * 8; r0 < padded; r0 += stride * 8) {
@@ -161,17 +168,18 @@ __global__ __launch_bounds__(kCeBlock) void k_ce_pack(CeArgs a, T const *src, si
     float const scale = ce_scale(m);
     // across = as * ratio, ratio = weight * scale_across / scale
     // (a row of zeros has no share in a product, so none in the largest either)
-    float ratio = r < rows ? 1.0f : 0.0f, un = m > 0.0f ? ce_unscale(scale) : 0.0f;
+    float ratio = r < rows ? 1.0f : 0.0f, un = m > 0.0f ? ce_unscale(scale) : 0.0f, s2 = scale;
     if ((lane & 7) == 0 && (ALONE || wave == 0)) unscale[r] = un;
     if constexpr (LABELS) {
       int const l = r < rows ? a.labels[r] : -1;
       float const w = l >= 0 && static_cast<size_t>(l) < a.V ? ce_row_weight(a, r) : 0.0f;
-      float const s2 = ce_scale(fabsf(w) * m);
+      s2 = ce_scale(fabsf(w) * m);
       ratio = l >= 0 && static_cast<size_t>(l) < a.V ? w * (s2 * ce_unscale(scale)) : 0.0f;
       un = fabsf(w) * m > 0.0f ? ce_unscale(s2) : 0.0f;
       if ((lane & 7) == 0 && (ALONE || wave == 0)) unscale_across[r] = un;
     }
     mine = fmaxf(mine, r < rows ? un : 0.0f);
+    finest = fmaxf(finest, r < rows && un > 0.0f ? s2 : 0.0f);
     auto const pack = [&](float const (&v)[8], char *dst) {
       half8 hi, lo;
 #pragma unroll
@@ -228,20 +236,33 @@ __global__ __launch_bounds__(kCeBlock) void k_ce_pack(CeArgs a, T const *src, si
   }
   if (most.w == nullptr) return;
   mine = ce_wave_max(mine);
+  finest = ce_wave_max(finest);
   if constexpr (ALONE) {  // (otherwise the wavefronts have seen the same rows)
-    if (lane == 0) top[0][wave][0] = mine;
+    if (lane == 0) {
+      top[0][wave][0] = mine;
+      top[0][wave][1] = finest;
+    }
     __syncthreads();
     mine = fmaxf(fmaxf(top[0][0][0], top[0][1][0]), fmaxf(top[0][2][0], top[0][3][0]));
+    finest = fmaxf(fmaxf(top[0][0][1], top[0][1][1]), fmaxf(top[0][2][1], top[0][3][1]));
   }
   if constexpr (LABELS) {
-    if (threadIdx.x == 0) most.parts[blockIdx.x] = mine;
+    if (threadIdx.x == 0) {
+      most.parts[blockIdx.x] = mine;
+      most.parts[most.nparts + blockIdx.x] = finest;
+    }
     if (blockIdx.x == 0)
-      for (unsigned q = threadIdx.x; q < most.pieces; q += kCeBlock) most.w[q] = 0.0f;
+      for (unsigned q = threadIdx.x; q < 2 * most.pieces; q += kCeBlock) most.w[q] = 0.0f;
   } else {
-    if (threadIdx.x == 0) atomicMax(reinterpret_cast<unsigned *>(most.w) + most.piece, __float_as_uint(mine));
-    if (most.piece == 0 && blockIdx.x == 0 && wave == 0) {
-      float const x = ce_largest(most.parts, most.nparts, lane);
-      if (lane == 0) most.x[0] = x;
+    if (threadIdx.x < 2) {
+      // (powers of two, mostly the same ones: who finds at least its own there, however old the value, has nothing to add)
+      unsigned *const to = reinterpret_cast<unsigned *>(most.w) + threadIdx.x * most.pieces + most.piece;
+      unsigned const x = __float_as_uint(threadIdx.x == 0 ? mine : finest);
+      if (__hip_atomic_load(to, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) < x) atomicMax(to, x);
+    }
+    if (most.piece == 0 && blockIdx.x == 0 && wave < 2) {
+      float const x = ce_largest(most.parts + wave * most.nparts, most.nparts, lane);
+      if (lane == 0) most.x[wave] = x;
     }
   }
 }
@@ -261,8 +282,10 @@ __device__ __forceinline__ float ce_join_factor(float m, float most) { return m 
 struct CeLogits {
   char const *P, *Q;
   float const *unscale_x, *unscale_w;  // of the rows of the batch, of the piece's classes
-  // backward: what undoes the scale of X's rows times dloss; the largest of those and of unscale_w
-  float const *unscale_xw, *most_x, *most_w;
+  // backward: what undoes the scale of X's rows times dloss; the largest of those and their largest scale, both of unscale_w
+  float const *unscale_xw, *most_x, *finest_x, *most_w, *finest_w;
+  float *dl;                           // dL [padded rows][dl_stride] in fp32, where the factors lie far apart
+  size_t dl_stride;
   unsigned ni, nj, kblocks, stages;    // kblocks: of a row block in memory
   size_t v0, vn;                     // first class of the piece, classes in it
 };
@@ -725,9 +748,10 @@ __device__ __forceinline__ float ce_scatter_sum(f32x16 const &v, int lane) {
 // the largest): the factors of the products' k that do not come out of their sums, powers of two, so that the planes are
 // rounded once and multiplied in f16.  Bound by the matrix pipe and by writing both packings: 288 us for a piece of 8192
 // classes, [8192 x 2048] BF16, 175 us for [777 x 1000] FP32 against 30011.  DB: also the sums of dloss dL over each half tile of rows.
-template <int T, int NP, bool DB>
-__global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_grad(CeArgs a, CeLogits g, char *dlb, char *dlv, unsigned kblocks_v,
-                                                                  unsigned kblocks_b, float *dbpart, size_t dbpart_stride) {
+// FAR: dL in fp32 instead.
+template <int T, int NP, bool DB, bool FAR>
+__device__ __forceinline__ void ce_grad_tile(CeArgs const &a, CeLogits const &g, char *dlb, char *dlv, unsigned kblocks_v, unsigned kblocks_b,
+                                             float *dbpart, size_t dbpart_stride) {
   using H = HalfTile<T, T, NP>;
   unsigned ti, tj;
   ce_tile(xcd_consecutive(blockIdx.x, gridDim.x), g.ni, g.nj, ti, tj);
@@ -782,6 +806,12 @@ __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_grad(CeArgs a, CeL
         if constexpr (DB) sum[r] += live[n] ? weight[n] * z[r] : 0.0f;
       }
       size_t const ib = c0 / 32 + m, jb = b0 / 32 + n;
+      if constexpr (FAR) {
+        float *const to = g.dl + (b0 + n * 32 + (lane & 31)) * g.dl_stride + c0 + m * 32 + 4 * (lane >> 5);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) *reinterpret_cast<f32x4 *>(to + 8 * k) = f32x4{z[k * 4], z[k * 4 + 1], z[k * 4 + 2], z[k * 4 + 3]};
+        continue;
+      }
       HalfQuads<NP> const q = half_planes<NP>(z * kCeDl);
       HalfQuads<NP> qb, qv;
 #pragma unroll
@@ -801,6 +831,18 @@ __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_grad(CeArgs a, CeL
         dbpart[(tj * 2 + (wave & 1)) * dbpart_stride + c0 + m * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3)] = s;
     }
   }
+}
+
+__device__ __forceinline__ bool ce_far(CeLogits const &g) { return ce_apart(g.most_w, g.finest_w) || ce_apart(g.most_x, g.finest_x); }
+
+template <int T, int NP, bool DB>
+__global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_grad(CeArgs a, CeLogits g, char *dlb, char *dlv, unsigned kblocks_v,
+                                                                  unsigned kblocks_b, float *dbpart, size_t dbpart_stride) {
+  // (chosen before the K loop: with both epilogues behind one, neither has the registers it needs, 319 -> 339 us)
+  if (ce_far(g))
+    ce_grad_tile<T, NP, DB, true>(a, g, dlb, dlv, kblocks_v, kblocks_b, dbpart, dbpart_stride);
+  else
+    ce_grad_tile<T, NP, DB, false>(a, g, dlb, dlv, kblocks_v, kblocks_b, dbpart, dbpart_stride);
 }
 
 static __global__ __launch_bounds__(kCeBlock) void k_ce_db(float const *part, size_t stride, unsigned parts, size_t n, float *db, float scale, int accumulate) {
@@ -839,20 +881,79 @@ __device__ __forceinline__ void ce_block_out(f32x16 const &v, float factor, O *o
   }
 }
 
+// A wavefront's blocks of a product on the fp32 matrix pipe over k = 0 .. count - 1, only where factors lie far apart: p(k, m),
+// q(k, n) give four consecutive k from k on of this lane's row of block m and column of block n (zeros from count on), from the
+// caches, eight k at a time and the next eight on their way.  A step takes about twice as long with it: [777 x 1000] FP32
+// against 30011 classes 1.82 ms instead of 0.74, [8192 x 2048] BF16 against 65536 14.3 instead of 8.2, [152 x 533] BF16 against
+// 1838 167 us instead of 58.  Asking costs every other step 0.4 - 1 % (0.3 us a launch).
+template <class H, class P, class Q>
+__device__ __forceinline__ void ce_far_product(HalfAcc<H> &acc, size_t count, int lane, P &&p, Q &&q) {
+  struct Eight {
+    f32x4 x[H::kMB], y[H::kNB];
+  };
+  auto const load = [&](Eight &e, size_t k) {
+#pragma unroll
+    for (int m = 0; m < H::kMB; ++m) e.x[m] = p(k, m);
+#pragma unroll
+    for (int n = 0; n < H::kNB; ++n) e.y[n] = q(k, n);
+  };
+#pragma unroll
+  for (int m = 0; m < H::kMB; ++m)
+#pragma unroll
+    for (int n = 0; n < H::kNB; ++n) acc.v[m][n] = f32x16{};
+  Eight now, next;
+  load(now, 4 * (lane >> 5));
+  for (size_t k = 0; k < count; k += 8) {
+    load(next, (k + 8 < count ? k + 8 : k) + 4 * (lane >> 5));
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int m = 0; m < H::kMB; ++m)
+#pragma unroll
+        for (int n = 0; n < H::kNB; ++n) acc.v[m][n] = __builtin_amdgcn_mfma_f32_32x32x2f32(now.x[m][t], now.y[n][t], acc.v[m][n], 0, 0, 0);
+    now = next;
+  }
+}
+
 // dW of a piece: classes i (P = dL packed by classes), features j (Q = dloss X packed by features), times `scale`.  216 us for
 // 8192 classes, [8192 x 2048] BF16 = 1270 TFLOP/s.
 template <int T, int NP, class O>
-__global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_dw(char const *P, char const *Q, unsigned ni, unsigned nj, unsigned kblocks,
-                                                                unsigned stages, float const *most, float scale, O *out, size_t rows,
+__global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_dw(CeArgs a, CeLogits g, char const *P, char const *Q, unsigned ni, unsigned nj,
+                                                                unsigned kblocks, unsigned stages, float scale, O *out, size_t rows,
                                                                 size_t cols, int accumulate) {
   using H = HalfTile<T, T, NP>;
   unsigned ti, tj;
   ce_tile(xcd_consecutive(blockIdx.x, gridDim.x), ni, nj, ti, tj);
   size_t const rs = static_cast<size_t>(kblocks) * NP * kFragBytes;
-  HalfAcc<H> acc;
-  half_gemm<H>(acc, P + ti * (T / 32) * rs, Q + tj * (T / 32) * rs, rs, rs, stages);
   int const lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  float const factor = most[0] * (scale * (1.0f / kCeDl));
+  float factor = g.most_x[0] * (scale * (1.0f / kCeDl));
+  HalfAcc<H> acc;
+  if (ce_far(g)) {
+    size_t const i = static_cast<size_t>(ti) * T + (wave >> 1) * (T / 2) + (lane & 31), j = static_cast<size_t>(tj) * T + (wave & 1) * (T / 2) + (lane & 31);
+    O const *const X = static_cast<O const *>(a.X);
+    // (dL has whole tiles of rows, zero in padding and in rows left out, whose X may be anything)
+    ce_far_product(
+        acc, a.B, lane,
+        [&](size_t b, int m) {
+          float const *const d = g.dl + b * g.dl_stride + i + m * 32;
+          return f32x4{d[0], d[g.dl_stride], d[2 * g.dl_stride], d[3 * g.dl_stride]};
+        },
+        [&](size_t b, int n) {
+          size_t const f = j + n * 32 < cols ? j + n * 32 : cols - 1;
+          f32x4 v;
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            size_t const in = b + t < a.B ? b + t : a.B - 1;
+            int const l = a.labels[in];
+            float const x = static_cast<float>(X[in * cols + f]), w = a.dloss != nullptr ? a.dloss[in] : 1.0f;
+            v[t] = b + t < a.B && l >= 0 && static_cast<size_t>(l) < a.V && w != 0.0f ? w * x : 0.0f;
+          }
+          return v;
+        });
+    factor = scale;
+  } else {
+    half_gemm<H>(acc, P + ti * (T / 32) * rs, Q + tj * (T / 32) * rs, rs, rs, stages);
+  }
 #pragma unroll
   for (int m = 0; m < H::kMB; ++m)
 #pragma unroll
@@ -864,9 +965,9 @@ __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_dw(char const *P, 
 // A slice of a piece's share of dX: rows of the batch i (P = dL packed by rows), features j (Q = W packed by features), summed
 // over the piece's classes of the slice into out [slice][rows][cols]; the first piece writes, later ones add.  216 us for 8192
 // classes, [8192 x 2048] BF16 = 1270 TFLOP/s (228 where it adds).
-template <int T, int NP>
-__global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_dx(char const *P, char const *Q, unsigned ni, unsigned nj, unsigned kblocks,
-                                                                unsigned stages, unsigned per_slice, float const *most, float *out,
+template <int T, int NP, class E>
+__global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_dx(CeLogits g, E const *W, char const *P, char const *Q, unsigned ni, unsigned nj,
+                                                                unsigned kblocks, unsigned stages, unsigned per_slice, float *out,
                                                                 size_t rows, size_t cols, int first) {
   using H = HalfTile<T, T, NP>;
   unsigned ti, tj;
@@ -876,10 +977,31 @@ __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_dx(char const *P, 
   if (s0 >= stages) return;  // a shorter last piece (the first has work for every slice)
   unsigned const count = stages - s0 < per_slice ? stages - s0 : per_slice;
   size_t const rs = static_cast<size_t>(kblocks) * NP * kFragBytes, skip = static_cast<size_t>(s0) * H::kStep;
-  HalfAcc<H> acc;
-  half_gemm<H>(acc, P + ti * (T / 32) * rs + skip, Q + tj * (T / 32) * rs + skip, rs, rs, count);
   int const lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  float const factor = most[0] * (1.0f / kCeDl);
+  float factor = g.most_w[0] * (1.0f / kCeDl);
+  HalfAcc<H> acc;
+  if (ce_far(g)) {
+    size_t const i = static_cast<size_t>(ti) * T + (wave >> 1) * (T / 2) + (lane & 31), j = static_cast<size_t>(tj) * T + (wave & 1) * (T / 2) + (lane & 31);
+    size_t const c0 = static_cast<size_t>(s0) * H::KS * 16, left = g.vn > c0 ? g.vn - c0 : 0, most = static_cast<size_t>(count) * H::KS * 16;
+    // (dL has whole tiles of classes, zero in padding; a slice is whole blocks of 16)
+    ce_far_product(
+        acc, left < most ? left : most, lane,
+        [&](size_t c, int m) { return *reinterpret_cast<f32x4 const *>(g.dl + (i + m * 32) * g.dl_stride + c0 + c); },
+        [&](size_t c, int n) {
+          size_t const f = j + n * 32 < cols ? j + n * 32 : cols - 1;
+          f32x4 v;
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            size_t const in = c0 + c + t;
+            float const w = static_cast<float>(W[(in < g.vn ? in : g.vn - 1) * cols + f]);
+            v[t] = in < g.vn ? w : 0.0f;
+          }
+          return v;
+        });
+    factor = 1.0f;
+  } else {
+    half_gemm<H>(acc, P + ti * (T / 32) * rs + skip, Q + tj * (T / 32) * rs + skip, rs, rs, count);
+  }
   out += slice * rows * cols;
 #pragma unroll
   for (int m = 0; m < H::kMB; ++m)
@@ -990,16 +1112,16 @@ CePlan ce_plan(dlmi_ctx const *ctx, size_t B, size_t K, size_t V, bool back) {
   p.unscale_x = take(p.Bp * sizeof(float));
   p.unscale_xw = take(p.Bp * sizeof(float));
   p.unscale_w = take(p.Vc * sizeof(float));
-  p.parts_x = take(p.pack_x * sizeof(float));
-  p.most_x = take(sizeof(float));
-  p.most_w = take(p.pieces * sizeof(float));
+  p.parts_x = take(2 * p.pack_x * sizeof(float));
+  p.most_x = take(2 * sizeof(float));
+  p.most_w = take(2 * p.pieces * sizeof(float));
   if (!back) {
     p.part = take(dlmi_ceil_div(V, T) * 2 * p.Bp * sizeof(float2));
     p.target = take(B * sizeof(float));
   } else {
     p.xt = take(packed_bytes(p.Kp, p.Bp, NP));
     p.wt = take(packed_bytes(p.Kp, p.Vc, NP));
-    p.dlb = take(packed_bytes(p.Bp, p.Vc, NP));
+    p.dlb = take(packed_bytes(p.Bp, p.Vc, NP));  // (dL in fp32 takes the place of both, or of the first where NP is 2)
     p.dlv = take(packed_bytes(p.Vc, p.Bp, NP));
     size_t const dxt = p.Bp / T * (p.Kp / T), stages = dlmi_ceil_div(p.Vc, T == 64 ? 64 / NP : 32 / NP);
     size_t s = static_cast<size_t>(ctx->num_cu) * (T >= 256 ? 1 : 2) / dxt;
@@ -1059,7 +1181,11 @@ struct CeRun {
     g.unscale_x = floats(p.unscale_x);
     g.unscale_xw = floats(p.unscale_xw);
     g.most_x = floats(p.most_x);
+    g.finest_x = g.most_x + 1;
     g.most_w = floats(p.most_w) + v0 / p.Vc;
+    g.finest_w = g.most_w + p.pieces;
+    g.dl = floats(p.dlb);
+    g.dl_stride = vp;
     g.ni = static_cast<unsigned>(vp / p.T);
     g.nj = static_cast<unsigned>(p.Bp / p.T);
     g.kblocks = static_cast<unsigned>(p.Kp / 16);
@@ -1092,7 +1218,7 @@ struct CeRun {
   template <int T>
   int weights(CeLogits const &g, size_t v0, size_t vn, unsigned kb) const {
     unsigned const ni = static_cast<unsigned>(dlmi_ceil_div(vn, T)), nk = static_cast<unsigned>(dlmi_ceil_div(a.K, T));
-    hipLaunchKernelGGL((k_ce_dw<T, NP, E>), dim3(ni * nk), dim3(256), 0, ctx->stream, s + p.dlv, s + p.xt, ni, nk, kb, ce_stages(T, a.B), g.most_x,
+    hipLaunchKernelGGL((k_ce_dw<T, NP, E>), dim3(ni * nk), dim3(256), 0, ctx->stream, a, g, s + p.dlv, s + p.xt, ni, nk, kb, ce_stages(T, a.B),
                        a.scale, static_cast<E *>(a.dW) + v0 * a.K, vn, a.K, a.accumulate);
     DLMI_LAUNCH_CHECK(ctx, "k_ce_dw");
     return DLMI_OK;
@@ -1121,8 +1247,8 @@ struct CeRun {
         DLMI_LAUNCH_CHECK(ctx, "k_ce_db");
       }
       if (a.dX != nullptr) {
-        hipLaunchKernelGGL((k_ce_dx<T, NP>), dim3(nb * nk * p.slices), dim3(256), 0, ctx->stream, s + p.dlb, s + p.wt, nb, nk, kv, ce_stages(T, vp),
-                           p.per_slice, g.most_w, floats(p.dxacc), a.B, a.K, v0 == 0 ? 1 : 0);
+        hipLaunchKernelGGL((k_ce_dx<T, NP, E>), dim3(nb * nk * p.slices), dim3(256), 0, ctx->stream, g, static_cast<E const *>(a.W) + v0 * a.K,
+                           s + p.dlb, s + p.wt, nb, nk, kv, ce_stages(T, vp), p.per_slice, floats(p.dxacc), a.B, a.K, v0 == 0 ? 1 : 0);
         DLMI_LAUNCH_CHECK(ctx, "k_ce_dx");
       }
       if (a.dW != nullptr) {
