@@ -39,8 +39,7 @@ __device__ __forceinline__ unsigned xcd_consecutive(unsigned id, unsigned n) {
 // One step of the K loop reads one stage of LDS: KS k blocks of all planes of the BM + BN rows, four stages in all.  64 x 64
 // tiles take twice the k blocks of the others per stage: their stages are short, and three of them ahead is less than a load
 // takes.
-// NP: planes that are multiplied; MP: planes that lie in memory (of two, the first alone may be read).
-template <int BM, int BN, int NP, int MP = NP>
+template <int BM, int BN, int NP>
 struct HalfTile {
   static constexpr int kPlanes = NP;
   static constexpr int kDepth = BM + BN <= 128 ? 4 : 2;      // fragments of a row block in a stage
@@ -49,9 +48,9 @@ struct HalfTile {
   static constexpr int kFragsA = BM / 32 * kDepth, kFragsB = BN / 32 * kDepth;  // fragments of a stage
   static constexpr int kStageBytes = (kFragsA + kFragsB) * kFragBytes;
   static constexpr int kLoads = (kFragsA + kFragsB) / 4;     // direct loads of a wavefront per stage
-  static constexpr int kStep = KS * MP * kFragBytes;         // bytes from a row block's stage to its next
+  static constexpr int kStep = KS * NP * kFragBytes;         // bytes from a row block's stage to its next
   // where fragment f of an operand's stage lies in its row block: plane f % NP of k block f / NP
-  static __host__ __device__ constexpr int at(int f) { return (f % kDepth / NP * MP + f % NP) * kFragBytes; }
+  static __host__ __device__ constexpr int at(int f) { return f % kDepth * kFragBytes; }
 };
 
 template <class T>

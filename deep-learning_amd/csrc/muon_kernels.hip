@@ -12,9 +12,9 @@
 // Precision.  The polynomial multiplies what lies in weak directions by up to a^steps (485 for 5 steps of 3.4445), the
 // rounding of the operands among it.  With one f16 plane a random matrix ends 1.3e-3 off and a matrix of rank 32 plus 1 %
 // noise 2.7e-2; with two planes (22 bits) 1.8e-6 and 1.2e-5, as far as a computation in fp32 (1.1e-5 and 1.9e-5).  So X,
-// A and a I + b A + c A A keep two planes; only the last step of a bf16 result multiplies the first plane alone (11 bits: 4.5e-4
-// on random matrices, 1.0e-3 on the rank 32 one, under the 1.7e-3 of rounding the result to 8 bits; two such steps would be
-// at 7.5e-4 and 2.5e-3).  16 x 2048 x 2048 FP32: 8.1 - 8.3 ms a step; 4096 x 4096 BF16: 3.4 - 3.5 ms; 1531 x 517 BF16: 141 us;
+// A and a I + b A + c A A keep two planes in every step.  (One plane in the last step of a bf16 result adds 4.5e-4 to 1.0e-3 to
+// the 1.7e-3 of rounding it, in the norm, but rounds one element in five to another value, small ones up to 60 half steps
+// away; it saved a tenth of a 4096 x 4096 call.)  16 x 2048 x 2048 FP32: 8.1 - 8.3 ms a step; 4096 x 4096 BF16: 3.8 ms; 1531 x 517 BF16: 150 us;
 // 128 x 256: 77 - 84 us, 17 launches of 3.5 to 5.5.  Singular values stay below about 1.3 and the polynomial in A between -3 and 4, so all three matrices are held times 2^12: far from the ends of f16's range.
 //
 // X is kept both ways round (rows i, k = j for X X^T; rows j, k = i for the product by X), each written by the product
@@ -204,9 +204,9 @@ __device__ __forceinline__ MuonTile muon_tile(MuonSymmetric const &a, unsigned t
   return t;
 }
 
-template <int T, int NP, bool POLY>
+template <int T, bool POLY>
 __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_muon_symmetric(MuonSymmetric a, unsigned stages) {
-  using H = HalfTile<T, T, NP, 2>;
+  using H = HalfTile<T, T, 2>;
   MuonTile const t = muon_tile(a, xcd_consecutive(blockIdx.x, gridDim.x));
   size_t const rs = static_cast<size_t>(a.kblocks) * 2 * kFragBytes;
   char const *const p = a.P + t.mat * a.stride_p;
@@ -222,10 +222,10 @@ __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_muon_symmetric(MuonSy
                                  acc.v[m][n], id0, id1, lane);
 }
 
-template <int T, int NP>
+template <int T>
 __global__ __launch_bounds__(256, 1) void k_muon_symmetric_parts(MuonSymmetric a, HalfShares shares) {
   size_t const rs = static_cast<size_t>(a.kblocks) * 2 * kFragBytes;
-  half_gemm_parts<HalfTile<T, T, NP, 2>>(shares, rs, rs, [&](unsigned tile, char const *&p, char const *&q) {
+  half_gemm_parts<HalfTile<T, T, 2>>(shares, rs, rs, [&](unsigned tile, char const *&p, char const *&q) {
     MuonTile const t = muon_tile(a, tile);
     p = a.P + t.mat * a.stride_p + t.ti * (T / 32) * rs;
     q = a.P + t.mat * a.stride_p + t.tj * (T / 32) * rs;
@@ -233,9 +233,9 @@ __global__ __launch_bounds__(256, 1) void k_muon_symmetric_parts(MuonSymmetric a
 }
 
 // The blocks of the shared tiles, a wavefront each.
-template <int T, int NP, bool POLY>
+template <int T, bool POLY>
 __global__ __launch_bounds__(256) void k_muon_symmetric_join(MuonSymmetric a, HalfShares shares) {
-  using H = HalfTile<T, T, NP, 2>;
+  using H = HalfTile<T, T, 2>;
   constexpr unsigned kBlocks = (T / 32) * (T / 32), kWave = H::kMB * H::kNB;
   int const lane = threadIdx.x & 63;
   unsigned const id = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), shared = id / kBlocks, block = id % kBlocks;
@@ -319,9 +319,9 @@ __device__ __forceinline__ MuonTile muon_tile(MuonUpdate const &a, unsigned tile
   return t;
 }
 
-template <int T, int NP, int MODE, class O>
+template <int T, int MODE, class O>
 __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_muon_update(MuonUpdate a, MuonBatch b, unsigned stages) {
-  using H = HalfTile<T, T, NP, 2>;
+  using H = HalfTile<T, T, 2>;
   MuonTile const t = muon_tile(a, xcd_consecutive(blockIdx.x, gridDim.x));
   size_t const rs = static_cast<size_t>(a.kbm) * 2 * kFragBytes;
   HalfAcc<H> acc;
@@ -336,19 +336,19 @@ __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_muon_update(MuonUpdat
                                  acc.v[m][n], id0, id1, lane);
 }
 
-template <int T, int NP>
+template <int T>
 __global__ __launch_bounds__(256, 1) void k_muon_update_parts(MuonUpdate a, HalfShares shares) {
   size_t const rs = static_cast<size_t>(a.kbm) * 2 * kFragBytes;
-  half_gemm_parts<HalfTile<T, T, NP, 2>>(shares, rs, rs, [&](unsigned tile, char const *&p, char const *&q) {
+  half_gemm_parts<HalfTile<T, T, 2>>(shares, rs, rs, [&](unsigned tile, char const *&p, char const *&q) {
     MuonTile const t = muon_tile(a, tile);
     p = a.Bm + t.mat * a.stride_b + t.ti * (T / 32) * rs;
     q = a.XT + t.mat * a.stride_x + t.tj * (T / 32) * rs;
   });
 }
 
-template <int T, int NP, int MODE, class O>
+template <int T, int MODE, class O>
 __global__ __launch_bounds__(256) void k_muon_update_join(MuonUpdate a, MuonBatch b, HalfShares shares) {
-  using H = HalfTile<T, T, NP, 2>;
+  using H = HalfTile<T, T, 2>;
   constexpr unsigned kBlocks = (T / 32) * (T / 32), kWave = H::kMB * H::kNB;
   int const lane = threadIdx.x & 63;
   unsigned const id = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), shared = id / kBlocks, block = id % kBlocks;
@@ -426,45 +426,45 @@ static HalfShares muon_shares(MuonPlan const &pl, unsigned tiles, unsigned stage
   return half_shares(tiles, stages, share ? pl.workgroups : tiles, parts);
 }
 
-template <int T, int NP, bool POLY>
+template <int T, bool POLY>
 static int muon_symmetric(dlmi_ctx *ctx, MuonSymmetric const &a, HalfShares const &shares) {
   if (shares.whole != 0) {
-    hipLaunchKernelGGL((k_muon_symmetric<T, NP, POLY>), dim3(shares.whole), dim3(256), 0, ctx->stream, a, shares.stages);
+    hipLaunchKernelGGL((k_muon_symmetric<T, POLY>), dim3(shares.whole), dim3(256), 0, ctx->stream, a, shares.stages);
     DLMI_LAUNCH_CHECK(ctx, "k_muon_symmetric");
   }
   if (shares.total == 0) return DLMI_OK;
-  hipLaunchKernelGGL((k_muon_symmetric_parts<T, NP>), dim3(shares.grid), dim3(256), 0, ctx->stream, a, shares);
+  hipLaunchKernelGGL((k_muon_symmetric_parts<T>), dim3(shares.grid), dim3(256), 0, ctx->stream, a, shares);
   DLMI_LAUNCH_CHECK(ctx, "k_muon_symmetric_parts");
   unsigned const blocks = (shares.tiles - shares.whole) * (T / 32) * (T / 32) / 4;
-  hipLaunchKernelGGL((k_muon_symmetric_join<T, NP, POLY>), dim3(blocks), dim3(256), 0, ctx->stream, a, shares);
+  hipLaunchKernelGGL((k_muon_symmetric_join<T, POLY>), dim3(blocks), dim3(256), 0, ctx->stream, a, shares);
   DLMI_LAUNCH_CHECK(ctx, "k_muon_symmetric_join");
   return DLMI_OK;
 }
 
-template <int T, int NP, int MODE, class O>
+template <int T, int MODE, class O>
 static int muon_update(dlmi_ctx *ctx, MuonUpdate const &a, MuonBatch const &b, HalfShares const &shares) {
   if (shares.whole != 0) {
-    hipLaunchKernelGGL((k_muon_update<T, NP, MODE, O>), dim3(shares.whole), dim3(256), 0, ctx->stream, a, b, shares.stages);
+    hipLaunchKernelGGL((k_muon_update<T, MODE, O>), dim3(shares.whole), dim3(256), 0, ctx->stream, a, b, shares.stages);
     DLMI_LAUNCH_CHECK(ctx, "k_muon_update");
   }
   if (shares.total == 0) return DLMI_OK;
-  hipLaunchKernelGGL((k_muon_update_parts<T, NP>), dim3(shares.grid), dim3(256), 0, ctx->stream, a, shares);
+  hipLaunchKernelGGL((k_muon_update_parts<T>), dim3(shares.grid), dim3(256), 0, ctx->stream, a, shares);
   DLMI_LAUNCH_CHECK(ctx, "k_muon_update_parts");
   unsigned const blocks = (shares.tiles - shares.whole) * (T / 32) * (T / 32) / 4;
-  hipLaunchKernelGGL((k_muon_update_join<T, NP, MODE, O>), dim3(blocks), dim3(256), 0, ctx->stream, a, b, shares);
+  hipLaunchKernelGGL((k_muon_update_join<T, MODE, O>), dim3(blocks), dim3(256), 0, ctx->stream, a, b, shares);
   DLMI_LAUNCH_CHECK(ctx, "k_muon_update_join");
   return DLMI_OK;
 }
 
-// A step of the iteration, NP planes multiplied.
-template <int T, int NP, int MODE, class O>
+// A step of the iteration.
+template <int T, int MODE, class O>
 static int muon_one(dlmi_ctx *ctx, MuonPlan const &pl, MuonBatch const &b, MuonSymmetric const &g, MuonSymmetric const &q, MuonUpdate const &u,
                     unsigned count, float *parts) {
-  constexpr unsigned KS = HalfTile<T, T, NP, 2>::KS;
+  constexpr unsigned KS = HalfTile<T, T, 2>::KS;
   unsigned const tri = u.mt * (u.mt + 1) / 2 * count;
-  int rc = muon_symmetric<T, NP, false>(ctx, g, muon_shares(pl, tri, u.kbn / KS, parts));
-  if (rc == DLMI_OK) rc = muon_symmetric<T, NP, true>(ctx, q, muon_shares(pl, tri, u.kbm / KS, parts));
-  if (rc == DLMI_OK) rc = muon_update<T, NP, MODE, O>(ctx, u, b, muon_shares(pl, u.mt * u.nt * count, u.kbm / KS, parts));
+  int rc = muon_symmetric<T, false>(ctx, g, muon_shares(pl, tri, u.kbn / KS, parts));
+  if (rc == DLMI_OK) rc = muon_symmetric<T, true>(ctx, q, muon_shares(pl, tri, u.kbm / KS, parts));
+  if (rc == DLMI_OK) rc = muon_update<T, MODE, O>(ctx, u, b, muon_shares(pl, u.mt * u.nt * count, u.kbm / KS, parts));
   return rc;
 }
 
@@ -477,13 +477,13 @@ static int muon_iterate(dlmi_ctx *ctx, MuonBatch const &b, MuonPlan const &pl, u
   MuonSymmetric const q{A, Bm, pl.bytes_a, pl.bytes_a, mt, kbm, kbm, coefs[0], coefs[1], coefs[2]};
   MuonUpdate u{Bm, XT, XTn, XP, pl.bytes_a, pl.bytes_x, mt, nt, kbm, kbn, o};
   for (int s = 0; s + 1 < steps; ++s) {
-    int const rc = muon_one<T, 2, kMuonMore, O>(ctx, pl, b, g, q, u, count, parts);
+    int const rc = muon_one<T, kMuonMore, O>(ctx, pl, b, g, q, u, count, parts);
     if (rc != DLMI_OK) return rc;
     char *const x = const_cast<char *>(u.XT);
     u.XT = u.XTn;
     u.XTn = x;
   }
-  return muon_one<T, sizeof(O) == 2 ? 1 : 2, STEP ? kMuonStep : kMuonOut, O>(ctx, pl, b, g, q, u, count, parts);
+  return muon_one<T, STEP ? kMuonStep : kMuonOut, O>(ctx, pl, b, g, q, u, count, parts);
 }
 
 // `count` matrices of one shape, at most kMuonMax of them; the scratch has been reserved.

@@ -557,8 +557,8 @@ int dlmi_opt_irprop_plus(dlmi_ctx *ctx, size_t n, float *params, float *grads, f
 /* ---- Muon: the update of a weight matrix, orthogonalized (no counterpart in the reference) ----------------------
  * The Newton-Schulz iteration that takes the singular values of X = u / (|u|_F + eps) towards 1 and leaves its singular
  * vectors: `steps` times A = X X^T, X <- a X + (b A + c A A) X, on the shorter side of the matrix.  The usual values are
- * a, b, c = 3.4445, -4.7750, 2.0315 in 5 steps.  Computed to the precision of fp32 products; the last step of a bf16 result in
- * 11 bits.  Coefficients that would take a singular value s of [0, 1], its square or a + b s^2 + c s^4 beyond 8 on the way are
+ * a, b, c = 3.4445, -4.7750, 2.0315 in 5 steps.  Computed to the precision of fp32 products and rounded
+ * once.  Coefficients that would take a singular value s of [0, 1], its square or a + b s^2 + c s^4 beyond 8 on the way are
  * refused.  A zero matrix gives zero; a non-finite element makes every element of the result non-finite. */
 typedef struct {
   float a, b, c;
