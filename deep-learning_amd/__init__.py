@@ -633,15 +633,20 @@ class Dlmi:
         self._ck(self.lib.dlmi_vocab_ce_fwd(self.ctx, kind, B, K, V, _a(X), _a(W), _a(bias), _a(labels), _a(loss), _a(lse)))
         return loss, lse
 
-    def vocab_ce_bwd(self, X, W, labels, lse, bias=None, dloss=None, scale=1.0, dX=None, dW=None, db=None, accumulate=False):
+    def vocab_ce_bwd(self, X, W, labels, lse, bias=None, dloss=None, scale=1.0, dX=None, dW=None, db=None, accumulate=False,
+                     needs=("dX", "dW", "db")):
         """Its gradient (dlmi_vocab_ce_bwd), times scale * dloss per row.  Returns (dX, dW, db), made where missing (db only
-        with a bias); accumulate adds into dW and db."""
+        with a bias); accumulate adds into dW and db.  Those not in needs are not formed, and None (a frozen layer: ("dX",))."""
         kind = self._type(X)
         B, K, V = self._chk_vocab_ce(X, W, labels, bias, dict(lse=lse, dloss=dloss))
-        assert not accumulate or (dW is not None and (db is not None or bias is None)), "accumulating needs the gradients so far"
-        dX = dX if dX is not None else self._out(X.dtype, B, K)
-        dW = dW if dW is not None else self._out(X.dtype, V, K)
-        if db is None and bias is not None:
+        assert set(needs) <= {"dX", "dW", "db"}, "needs names dX, dW and db"
+        for what, t in (("dX", dX), ("dW", dW), ("db", db)):
+            assert t is None or what in needs, what + " is given but not needed"
+        wanted_db = "db" in needs and bias is not None
+        assert not accumulate or ((dW is not None or "dW" not in needs) and (db is not None or not wanted_db)), "accumulating needs the gradients so far"
+        dX = dX if dX is not None or "dX" not in needs else self._out(X.dtype, B, K)
+        dW = dW if dW is not None or "dW" not in needs else self._out(X.dtype, V, K)
+        if db is None and wanted_db:
             db = self._out(self.torch.float32, V)
         self._chk_is(dX, "dX", X.dtype, B, K)
         self._chk_is(dW, "dW", X.dtype, V, K)
