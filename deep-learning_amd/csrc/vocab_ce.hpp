@@ -16,7 +16,7 @@
 // values take two planes.  dL is in [-1, 1] and held times 2^15, rounded to 11 bits (bf16; the result keeps 8) or 22 (fp32).
 // Where a product's sum runs over rows that are scaled differently (dX over W's, dW over X's), dL carries what undoes the
 // scale, as a share of the largest such factor, which multiplies the result.  For dW X is packed times dloss (one more
-// rounding for bf16, none without dloss).  Factors more than 2^16 apart would leave no bits to the small ones (a padding row of
+// rounding for bf16, none without dloss).  Factors more than 2^19 apart would leave few bits to the small ones (a padding row of
 // W that was never set, one row of the batch with a huge dloss): a piece where they are, which the device finds out by itself,
 // keeps dL in fp32 where its planes would lie and multiplies it with the operands as they are on the fp32 matrix pipe.
 #pragma once
@@ -93,8 +93,9 @@ __device__ __forceinline__ float ce_largest(float const *v, unsigned n, int lane
 }
 
 // Whether factors that undo scales lie far apart: the largest of them times the largest scale (the smallest factor's inverse).
-// Up to here a row's terms keep an absolute error of 2^-40 of the largest factor's, 2^-24 of their own factor's.
-__device__ __forceinline__ bool ce_apart(float const *most, float const *finest) { return most[0] * finest[0] > 65536.0f; }
+// Up to here a row's terms keep an absolute error of 2^-40 of the largest factor's, 2^-21 of their own factor's.  (Of 8192 normal
+// dloss one batch in twenty has a value this close to 0; at 2^16 it would be one in three.)
+__device__ __forceinline__ bool ce_apart(float const *most, float const *finest) { return most[0] * finest[0] > 524288.0f; }
 
 // Rows of src [rows, cols], each scaled by its own largest magnitude and packed as it stands (`as`: row r, k = c) and / or
 // transposed (`across`: row c, k = r), padding zero.  unscale[r]: the inverse scale of `as`, unscale_across[r] that of
