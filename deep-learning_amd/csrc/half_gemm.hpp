@@ -126,9 +126,10 @@ __device__ __forceinline__ void half_stage_wait() {
 
 // The order of a k block's instructions: the next block's LDS reads and the next stages' loads spread between the matrix
 // instructions.  Left to itself the compiler puts them behind most of these, and the loads right before the next wait: 246
-// us against 221 us for 8192 x 8192 x 2048 in one plane (1242 TFLOP/s), 623 against 603 us in two (1368 TFLOP/s), 50 against
-// 45 us for 2048^3 in two planes with 128 x 128 tiles.  One plane of a 256 x 256 tile has few matrix instructions per read
-// and does best with all reads first (221 against 224 us); everything else with reads and loads spread alike.
+// us against 221 us for 8192 x 8192 x 2048 in one plane (1242 TFLOP/s by itself; 1150 - 1270 in the kernels that use it), 623
+// against 603 us in two (1368 TFLOP/s), 50 against 45 us for 2048^3 in two planes with 128 x 128 tiles.  One plane of a 256 x
+// 256 tile has few matrix instructions per read and does best with all reads first (221 against 224 us); everything else with
+// reads and loads spread alike.
 template <class T, bool LOADS>
 __device__ __forceinline__ void half_schedule() {
   constexpr int kMfma = 0x008, kLoad = 0x020, kRead = 0x100;

@@ -14,8 +14,9 @@
 // noise 2.7e-2; with two planes (22 bits) 1.8e-6 and 1.2e-5, as far as a computation in fp32 (1.1e-5 and 1.9e-5).  So X,
 // A and a I + b A + c A A keep two planes in every step.  (One plane in the last step of a bf16 result adds 4.5e-4 to 1.0e-3 to
 // the 1.7e-3 of rounding it, in the norm, but rounds one element in five to another value, small ones up to 60 half steps
-// away; it saved a tenth of a 4096 x 4096 call.)  16 x 2048 x 2048 FP32: 8.1 - 8.3 ms a step; 4096 x 4096 BF16: 3.8 ms; 1531 x 517 BF16: 150 us;
-// 128 x 256: 77 - 84 us, 17 launches of 3.5 to 5.5.  Singular values stay below about 1.3 and the polynomial in A between -3 and 4, so all three matrices are held times 2^12: far from the ends of f16's range.
+// away; it saved a tenth of a 4096 x 4096 call.)  16 x 2048 x 2048 FP32: 8.1 - 8.3 ms a step; 4096 x 4096 BF16: 3.8 ms; 1531 x
+// 517 BF16: 150 us; 128 x 256: 77 - 87 us, 17 launches of 3.4 to 5.4.  Singular values stay below about 1.3 and the polynomial in
+// A between -3 and 4, so all three matrices are held times 2^12: far from the ends of f16's range.
 //
 // X is kept both ways round (rows i, k = j for X X^T; rows j, k = i for the product by X), each written by the product
 // that makes it: a block of C in registers is a fragment of the transposed matrix as it stands, and two matrix

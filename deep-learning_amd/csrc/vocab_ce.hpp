@@ -5,15 +5,18 @@
 //   dL_bv = exp(z_bv - lse_b) - [v = label_b],  dX = g dL W,  dW = (g dL)^T X,  db = sum_b g_b dL_b,   g_b = scale dloss_b
 //
 // The vocabulary is walked in pieces.  Forward: one product per piece whose epilogue reduces each T / 2 classes of a
-// row to a maximum and a sum of exponentials; nothing of size [B, V] is written.  Backward: per piece the logits again
-// (a third of the work, against B V values kept and read), dL rounded to f16 planes, the two products that read it.
+// row to a maximum and a sum of exponentials; nothing of size [B, V] is written.  Backward: per piece the logits again,
+// dL rounded to f16 planes, the two products that read it.  (For memory's sake: for [8192 x 2048] BF16 against 65536 classes the
+// logits take 1.7 ms again, where writing and reading 2 GiB of them would take 0.85.)
 // Bound by the 16-bit matrix pipe: 2 B K V operations forward, 6 B K V backward, times three for the two planes of an fp32
 // input (half_gemm.hpp); by reading W where there are few rows.  [8192 x 2048] BF16 against 65536 classes, forward and
-// backward: 8.2 - 8.5 ms = 1035 - 1075 TFLOP/s, packing included; [777 x 1000] FP32 against 30011: 762 us.
+// backward: 8.2 - 8.5 ms = 1035 - 1075 TFLOP/s, packing included; [777 x 1000] FP32 against 30011: 740 - 765 us.
 //
 // Operands are packed as f16 planes of powers-of-two multiples, each row of X and of W by its own largest magnitude (a
-// padding row full of garbage spoils nobody's scale).  bf16 values have 8 bits and one plane holds them exactly; fp32
-// values take two planes.  dL is in [-1, 1] and held times 2^15, rounded to 11 bits (bf16; the result keeps 8) or 22 (fp32).
+// padding row full of garbage spoils nobody's scale).  bf16 values have 8 bits and one plane holds them exactly, down
+// to 2^-30 of their row's largest; fp32 values take two planes, whose second has all its bits down to 2^-18 of that.  f16 ends at
+// 2^-24: what is smaller is held to 2^-39 (bf16) or 2^-40 (fp32) of the row's largest.  dL is in [-1, 1] and held times 2^15,
+// rounded to 11 bits (bf16; the result keeps 8) where it is above 2^-29, or 22 (fp32) above 2^-18, and to 2^-40 below.
 // Where a product's sum runs over rows that are scaled differently (dX over W's, dW over X's), dL carries what undoes the
 // scale, as a share of the largest such factor, which multiplies the result.  For dW X is packed times dloss (one more
 // rounding for bf16, none without dloss).  Factors more than 2^19 apart would leave few bits to the small ones (a padding row of
@@ -747,8 +750,9 @@ __device__ __forceinline__ float ce_scatter_sum(f32x16 const &v, int lane) {
 // dL of a tile, packed for dX (rows of the batch, k = classes; times what undoes the scale of W's row, as a share of the
 // piece's largest) and for dW (rows are classes, k = rows of the batch; times what undoes the scale of X's row, as a share of
 // the largest): the factors of the products' k that do not come out of their sums, powers of two, so that the planes are
-// rounded once and multiplied in f16.  Bound by the matrix pipe and by writing both packings: 288 us for a piece of 8192
-// classes, [8192 x 2048] BF16, 175 us for [777 x 1000] FP32 against 30011.  DB: also the sums of dloss dL over each half tile of rows.
+// rounded once and multiplied in f16 (a share of 2^-s costs an element s of the bits above 2^-40).  Bound by the matrix pipe and by
+// writing both packings: 300 - 310 us for a piece of 8192 classes, [8192 x 2048] BF16, 175 - 200 us for [777 x 1000] FP32 against
+// 30011.  DB: also the sums of dloss dL over each half tile of rows.
 // FAR: dL in fp32 instead.
 template <int T, int NP, bool DB, bool FAR>
 __device__ __forceinline__ void ce_grad_tile(CeArgs const &a, CeLogits const &g, char *dlb, char *dlv, unsigned kblocks_v, unsigned kblocks_b,
@@ -916,8 +920,8 @@ __device__ __forceinline__ void ce_far_product(HalfAcc<H> &acc, size_t count, in
   }
 }
 
-// dW of a piece: classes i (P = dL packed by classes), features j (Q = dloss X packed by features), times `scale`.  216 us for
-// 8192 classes, [8192 x 2048] BF16 = 1270 TFLOP/s.
+// dW of a piece: classes i (P = dL packed by classes), features j (Q = dloss X packed by features), times `scale`.  216 - 228 us
+// for 8192 classes, [8192 x 2048] BF16 = 1205 - 1270 TFLOP/s, falling with the clock in a long run.
 template <int T, int NP, class O>
 __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_dw(CeArgs a, CeLogits g, char const *P, char const *Q, unsigned ni, unsigned nj,
                                                                 unsigned kblocks, unsigned stages, float scale, O *out, size_t rows,
@@ -965,7 +969,7 @@ __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_dw(CeArgs a, CeLog
 
 // A slice of a piece's share of dX: rows of the batch i (P = dL packed by rows), features j (Q = W packed by features), summed
 // over the piece's classes of the slice into out [slice][rows][cols]; the first piece writes, later ones add.  216 us for 8192
-// classes, [8192 x 2048] BF16 = 1270 TFLOP/s (228 where it adds).
+// classes, [8192 x 2048] BF16 = 1270 TFLOP/s; 228 - 239 where it adds.
 template <int T, int NP, class E>
 __global__ __launch_bounds__(256, T >= 256 ? 1 : 2) void k_ce_dx(CeLogits g, E const *W, char const *P, char const *Q, unsigned ni, unsigned nj,
                                                                 unsigned kblocks, unsigned stages, unsigned per_slice, float *out,

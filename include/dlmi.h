@@ -311,9 +311,10 @@ int dlmi_loss_seed(dlmi_ctx *ctx, dlmi_loss loss, dlmi_accuracy accu, float accu
  *   z = X W^T + bias;  lse[b] = log sum_v exp z[b,v];  loss[b] = lse[b] - z[b, labels[b]].
  * X [B, K], W [V, K] of `type`; bias [V] fp32 or NULL; labels [B] int32: a label outside [0, V) leaves its row out (loss
  * 0, no gradient; its lse is still that of its logits).  loss, lse [B] fp32.  fp32 tensors are multiplied to the precision
- * of fp32 products, bf16 ones exactly, sums in fp32.  A non-finite row of X makes its own loss and lse NaN.  The vocabulary
- * is walked in pieces; the context's scratch holds one piece's operands (at most about 1 GiB), the rows of X and 8 bytes
- * per row and 32 to 128 classes, never [B, V].  As with every call that uses the scratch, graphs recorded from one context
+ * of fp32 products, bf16 ones exactly, sums in fp32; for more than 64 rows elements below 2^-18 (fp32) or 2^-30 (bf16) of the
+ * largest of their row of X or W count to 2^-39 of that.  A non-finite row of X makes its own loss and lse non-finite.  The vocabulary
+ * is walked in pieces; the context's scratch holds one piece's operands (at most about 1 GiB), the rows of X once more and 8
+ * bytes per row and 32 to 128 classes, never [B, V].  As with every call that uses the scratch, graphs recorded from one context
  * must not be replayed at the same time. */
 #define DLMI_VOCAB_CE_MAX_ROWS 262144
 #define DLMI_VOCAB_CE_MAX_FEATURES 65536
@@ -326,7 +327,9 @@ int dlmi_vocab_ce_fwd(dlmi_ctx *ctx, dlmi_dtype type, size_t B, size_t K, size_t
  * beyond some 10^5 the two may differ by more than 1 (a gradient of such a row is as exact as that, and finite).
  * dX [B, K], dW [V, K] of `type`, db [V] fp32; each may be NULL.  dX is written (zero in rows left out); accumulate != 0
  * adds into dW and db.  B, K and V must not be 0; a gradient must not overlap another array.  The logits are formed again,
- * piece by piece.  All sums are taken in an order that depends on the sizes only.
+ * piece by piece.  All sums are taken in an order that depends on the sizes only (and on what is said of magnitudes below).
+ * Scratch: one piece's operands (W twice, dL twice, at most about 1 GiB), X twice, and 4 bytes per element of X for the sums of
+ * dX (in up to 16 slices, 64 MiB together, where X is small).
  * dL is held to 11 bits (bf16) or 22 (fp32) of itself and, where it is small, absolutely: a term of dX to 2^-40 of W's largest
  * row in its piece, one of dW to 2^-40 of the largest |dloss| |X| of a row that counts.  Where W's rows in a piece, or these
  * magnitudes, lie more than 2^19 apart, dL is held and multiplied in fp32 instead, and the step takes about twice as long.  Rows
