@@ -1,12 +1,37 @@
 """dlmi_vocab_ce_fwd / _bwd at sizes that reach every tile the planner chooses among, as it chooses on 256 CUs, against the
-definition in 64 bits.  Tolerances as derived in test_gpu_vocab_ce.py and test_gpu_vocab_ce_far.py."""
+definition in 64 bits.
+
+Tolerances as derived in test_gpu_vocab_ce.py and test_gpu_vocab_ce_far.py, but for the rounding of a plane of 11 bits: values of
+[1, 2) are 2^-10 apart, half of that is 2^-11 of the value.  It counts once for an element of dL of bf16 tensors and once more,
+in dW, for X times dloss (`plane`); where one term carries a whole sum, it is all there is."""
 import pytest
 import torch
 
-from test_gpu_vocab_ce import BF16, F32, check, dz_of, exact, make, within
+from test_gpu_vocab_ce import BF16, F32, dz_of, exact, make, within
 from test_gpu_vocab_ce_far import held
 
 KINDS = [F32, BF16]
+
+
+def check(dl, B, K, V, kind, bias=True, left_out=0.0, dloss=False, seed=0):
+    X, W, b, labels = make(B, K, V, kind, bias, left_out, seed + B * 7 + K * 3 + V)
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    dl_rows = torch.randn(B, generator=gen, device="cuda") if dloss else None
+    g = torch.full((B,), 0.37, device="cuda") * (dl_rows if dloss else 1.0)
+    loss, lse = dl.vocab_ce_fwd(X, W, labels, bias=b)
+    eloss, else_, edX, edW, edb, mags, mX, mW, mb, floor = exact(X, W, b, labels, g)
+    dz = dz_of(kind, K, mags)
+    top = else_.abs().max().item()
+    within(lse, else_, dz + 2.0 ** -22 + 2.0 ** -24 * top, "lse")
+    within(loss, eloss, 2 * dz + 2.0 ** -22 + 2.0 ** -23 * (top + mags[0]), "loss")
+    dX, dW, db = dl.vocab_ce_bwd(X, W, labels, lse, bias=b, dloss=dl_rows, scale=0.37)
+    plane, half = (2.0 ** -11, 2.0 ** -8) if kind == BF16 else (0.0, 0.0)
+    rel = 2 * dz + 2.0 ** -20
+    within(dX, edX, (rel + plane + V * 2.0 ** -24) * mX + half * edX.abs() + floor[0], "dX")
+    within(dW, edW, (rel + (2 * plane if dloss else plane) + B * 2.0 ** -24) * mW + half * edW.abs() + floor[1], "dW")
+    assert (dX[labels < 0] == 0).all()
+    if bias:
+        within(db, edb, (rel + B * 2.0 ** -24) * mb + floor[2], "db")
 
 
 @pytest.mark.gpu
