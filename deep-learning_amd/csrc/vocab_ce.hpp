@@ -888,9 +888,9 @@ __device__ __forceinline__ void ce_block_out(f32x16 const &v, float factor, O *o
 
 // A wavefront's blocks of a product on the fp32 matrix pipe over k = 0 .. count - 1, only where factors lie far apart: p(k, m),
 // q(k, n) give four consecutive k from k on of this lane's row of block m and column of block n (zeros from count on), from the
-// caches, eight k at a time and the next eight on their way.  A step takes about twice as long with it: [777 x 1000] FP32
+// caches, eight k at a time and the next eight on their way.  A step takes two to three times as long with it: [777 x 1000] FP32
 // against 30011 classes 1.82 ms instead of 0.74, [8192 x 2048] BF16 against 65536 14.3 instead of 8.2, [152 x 533] BF16 against
-// 1838 167 us instead of 58.  Asking costs every other step 0.4 - 1 % (0.3 us a launch).
+// 1838 167 us instead of 58.  Asking costs the other steps 0.3 - 0.6 us a launch: 0.4 - 2.4 %, and 2.5 us of that one's 55.
 template <class H, class P, class Q>
 __device__ __forceinline__ void ce_far_product(HalfAcc<H> &acc, size_t count, int lane, P &&p, Q &&q) {
   struct Eight {

@@ -332,7 +332,7 @@ int dlmi_vocab_ce_fwd(dlmi_ctx *ctx, dlmi_dtype type, size_t B, size_t K, size_t
  * dX (in up to 16 slices, 64 MiB together, where X is small).
  * dL is held to 11 bits (bf16) or 22 (fp32) of itself and, where it is small, absolutely: a term of dX to 2^-40 of W's largest
  * row in its piece, one of dW to 2^-40 of the largest |dloss| |X| of a row that counts.  Where W's rows in a piece, or these
- * magnitudes, lie more than 2^19 apart, dL is held and multiplied in fp32 instead, and the step takes about twice as long.  Rows
+ * magnitudes, lie more than 2^19 apart, dL is held and multiplied in fp32 instead, and the step takes two to three times as long.  Rows
  * of X that are left out may hold anything. */
 int dlmi_vocab_ce_bwd(dlmi_ctx *ctx, dlmi_dtype type, size_t B, size_t K, size_t V, void const *X, void const *W,
                       float const *bias, int32_t const *labels, float const *lse, float const *dloss, float scale, void *dX,
